@@ -219,6 +219,66 @@ int tkv_combine_exchange(const float* acc, const float* m, const float* l, float
                          int64_t ml_row_stride, int64_t ml_slot_stride, void* const* peer_data,
                          void* state, int world, int rank, int wire_floats, void* stream);
 
+/* ---- Paged cache (no reference counterpart: its caches are contiguous) ----
+ * A pool is a cache with pages in the place of sequences: packed (num_pages, HKV, page_size,
+ * D*nbits/8) with scale / zero (num_pages, HKV, page_size, D/gs), or f16 (num_pages, HKV,
+ * page_size, D).  Token n of sequence b is row n % page_size of page
+ * block_table[b*table_stride + n / page_size]; an entry outside [0, num_pages) names no page.
+ * block_table, seq_lens, positions, lengths, parents and reserve are int32 device pointers.
+ *
+ * Decode attention over a paged cache: sequence b attends its first seq_lens[b] tokens (clamped
+ * to max_pages*page_size), without those of entries that name no page; with none left its rows
+ * of out are zero.  q as in tkv_fused_decode; out (B, HQ, D) of out_dtype.  page_size is a
+ * multiple of 16; D is 64 or 128; gs in {16,32,64,128}, at most D. */
+int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_packed, const void* k_scale,
+                     const void* k_zero, const uint8_t* v_packed, const void* v_scale,
+                     const void* v_zero, const int32_t* block_table, int64_t table_stride,
+                     const int32_t* seq_lens, void* out, int out_dtype, int B, int HQ, int HKV,
+                     int num_pages, int page_size, int max_pages, int D, int nbits, int gs,
+                     float sm_scale, void* stream);
+int tkv_paged_fp16_decode(const void* q, int q_dtype, const void* k, const void* v,
+                          const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
+                          void* out, int out_dtype, int B, int HQ, int HKV, int num_pages,
+                          int page_size, int max_pages, int D, float sm_scale, void* stream);
+
+/* Quantise T new tokens per (sequence, head) of K and of V -- element (b, h, t, d) of k at
+ * strides[0]*b + strides[1]*h + strides[2]*t + d, of v with strides[3..5] -- into their pages, at
+ * positions[b] + t (or pos0 + t), for t < lengths[b] (all T if null).  The bytes are those of
+ * tkv_quantize_pack.  nbits = 16: f16 pages, k_packed and v_packed are the pools and scale / zero
+ * are null.  k_values / v_values (null or of in_dtype, value_strides laid out like strides)
+ * receive code*scale + zero.  Positions outside the table and entries that name no page drop
+ * their tokens. */
+int tkv_paged_append(const void* k, const void* v, int in_dtype, const int64_t* strides,
+                     uint8_t* k_packed, void* k_scale, void* k_zero, uint8_t* v_packed,
+                     void* v_scale, void* v_zero, void* k_values, void* v_values,
+                     const int64_t* value_strides, const int32_t* block_table, int64_t table_stride,
+                     const int32_t* positions, int pos0, const int32_t* lengths, int B, int HKV, int T,
+                     int num_pages, int page_size, int max_pages, int D, int nbits, int gs,
+                     void* stream);
+
+/* 32-bit words of device workspace that tkv_pages_fork (B rows of the new table) and
+ * tkv_pages_compact need.  Calls that may run at the same time need workspaces of their own. */
+int tkv_pages_workspace(int B, int num_pages, int64_t* words);
+
+/* New table (B, max_pages) and lengths (B,) whose row b continues row parents[b] of the old ones
+ * (B_old rows of max_pages entries, table_stride apart): full pages shared, a partly filled page
+ * kept by the first row that continues this parent and copied for the others in all n_pools
+ * tensors of page_bytes[i] per page, pages added for reserve[b] (or reserve0) further
+ * tokens.  Fresh pages are the lowest that no kept entry names, in order of (row, position);
+ * `missing` (1,) receives how many the pool was short of.  The outputs must not overlap the
+ * inputs. */
+int tkv_pages_fork(const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
+                   int B_old, const int32_t* parents, const int32_t* reserve, int reserve0, int B,
+                   int max_pages, int num_pages, int page_size, int32_t* new_table, int32_t* new_lens,
+                   int32_t* missing, int32_t* workspace, void* const* pools,
+                   const int64_t* page_bytes, int n_pools, void* stream);
+
+/* With n pages named by the table (B, max_pages), move the k-th named page at or above n to the
+ * k-th unnamed one below n in all pools; new_table has the new numbers, `live` (1,) receives n. */
+int tkv_pages_compact(const int32_t* block_table, int64_t table_stride, int B, int max_pages,
+                      int num_pages, int32_t* new_table, int32_t* live, int32_t* workspace,
+                      void* const* pools, const int64_t* page_bytes, int n_pools, void* stream);
+
 /* Device-side status word of the current device (synchronises with it): 0 = ok,
  * bit 0 = a bounded wait on a copy barrier inside a decode kernel gave up (the kernel then
  * returned early and its output is invalid), bit 1 = a bounded wait for a peer's data in

@@ -1,0 +1,173 @@
+"""What the paged-cache functions refuse, checked without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from tritonkv_b200 import _cabi
+from tritonkv_b200.kernels import paged_decode_attention, paged_fp16_decode_attention
+from tritonkv_b200.paged import append_kv_paged, compact_pages, fork_pages
+from tritonkv_b200.quantize import QuantizedTensor, empty_cache
+
+
+def pool(NP=6, HKV=2, page=16, D=64, nbits=4, gs=32):
+    return empty_cache(NP, HKV, page, D, nbits, gs, "cpu")
+
+
+def i32(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def args(**kw):
+    d = dict(q=torch.zeros(3, 4, 64).half(), kq=pool(), vq=pool(), block_table=i32(3, 5), seq_lens=i32(3))
+    d.update(kw)
+    return d
+
+
+@pytest.mark.parametrize("bad,err,text", [
+    (dict(), RuntimeError, "CUDA"),
+    (dict(vq=pool(gs=16)), ValueError, "same nbits/group_size"),
+    (dict(vq=pool(NP=7)), ValueError, "same shape"),
+    (dict(q=torch.zeros(3, 4, 128).half()), ValueError, "incompatible"),
+    (dict(q=torch.zeros(3, 5, 64).half()), ValueError, "multiple of HKV"),
+    (dict(q=torch.zeros(3, 0, 64).half()), ValueError, "multiple of HKV"),
+    (dict(q=torch.zeros(3, 4).half()), ValueError, "q must be"),
+    (dict(block_table=i32(2, 5)), ValueError, "rows for 3"),
+    (dict(block_table=i32(3, 5).long()), ValueError, "int32"),
+    (dict(block_table=i32(15)), ValueError, "int32"),
+    (dict(block_table=i32(5, 3).T), ValueError, "contiguous"),
+    (dict(seq_lens=i32(4)), ValueError, "seq_lens"),
+    (dict(seq_lens=i32(3).long()), ValueError, "seq_lens"),
+    (dict(out=torch.zeros(3, 4, 32)), ValueError, "out must"),
+    (dict(out=torch.zeros(3, 4, 64).double()), ValueError, "out must"),
+    (dict(out=torch.zeros(3, 64, 4).transpose(1, 2)), ValueError, "out must"),
+    (dict(kq=torch.zeros(6, 2, 16, 64).half()), TypeError, "packed pools"),
+])
+def test_attention_refuses(bad, err, text):
+    with pytest.raises(err, match=text):
+        paged_decode_attention(**args(**bad))
+
+
+@pytest.mark.parametrize("k,err,text", [
+    (torch.zeros(6, 2, 16, 64).half(), RuntimeError, "CUDA"),
+    (torch.zeros(6, 2, 16, 64), TypeError, "float16"),
+    (torch.zeros(6, 2, 64).half(), ValueError, "num_pages"),
+    (torch.zeros(6, 16, 2, 64).half().transpose(1, 2), ValueError, "contiguous"),
+    (pool(), TypeError, "float16 pools"),
+])
+def test_fp16_attention_refuses(k, err, text):
+    with pytest.raises(err, match=text):
+        paged_fp16_decode_attention(torch.zeros(3, 4, 64).half(), k, k, i32(3, 5), i32(3))
+
+
+def test_pools_that_do_not_fit_together():
+    p = pool()
+    for broken, err in ((QuantizedTensor(p.packed, p.scale.float(), p.zero, 4, 32, 64), TypeError),
+                        (QuantizedTensor(p.packed.to(torch.int8), p.scale, p.zero, 4, 32, 64), TypeError),
+                        (QuantizedTensor(p.packed, p.scale[:3], p.zero, 4, 32, 64), ValueError),
+                        (QuantizedTensor(p.packed, p.scale, p.zero, 2, 32, 64), ValueError),
+                        (QuantizedTensor(p.packed, p.scale, p.zero, 4, 16, 64), ValueError),
+                        (QuantizedTensor(p.packed[:, :, ::2], p.scale[:, :, ::2], p.zero[:, :, ::2], 4, 32, 64), ValueError),
+                        (QuantizedTensor(p.packed[0], p.scale[0], p.zero[0], 4, 32, 64), ValueError)):
+        with pytest.raises(err):
+            paged_decode_attention(**args(kq=broken, vq=broken))
+        with pytest.raises(err):
+            compact_pages([broken], i32(3, 5))
+        with pytest.raises(err):
+            append_kv_paged(broken, broken, torch.zeros(3, 2, 1, 64).half(), torch.zeros(3, 2, 1, 64).half(), i32(3, 5), 0)
+
+
+@pytest.mark.parametrize("bad,err,text", [
+    (dict(), RuntimeError, "CUDA"),
+    (dict(v_new=torch.zeros(3, 2, 2, 64).half()), ValueError, "must both"),
+    (dict(v_new=torch.zeros(3, 2, 1, 64)), ValueError, "same dtype"),
+    (dict(k_new=torch.zeros(3, 1, 1, 64).half(), v_new=torch.zeros(3, 1, 1, 64).half()), ValueError, "does not match"),
+    (dict(k_new=torch.zeros(3, 2, 1, 64).double(), v_new=torch.zeros(3, 2, 1, 64).double()), TypeError, "unsupported dtype"),
+    (dict(vq=pool(nbits=2, gs=32)), ValueError, "same format"),
+    (dict(positions=-1), ValueError, "do not fit"),
+    (dict(positions=80), ValueError, "do not fit"),
+    (dict(positions=i32(2)), ValueError, "positions"),
+    (dict(lengths=i32(3).long()), ValueError, "lengths"),
+    (dict(block_table=i32(4, 5)), ValueError, "rows for 3"),
+    (dict(k_values=torch.zeros(3, 2, 1, 64)), ValueError, "k_values"),
+    (dict(v_values=torch.zeros(3, 2, 1, 128).half()[..., ::2]), ValueError, "v_values"),
+])
+def test_append_refuses(bad, err, text):
+    d = dict(kq=pool(), vq=pool(), k_new=torch.zeros(3, 2, 1, 64).half(), v_new=torch.zeros(3, 2, 1, 64).half(),
+             block_table=i32(3, 5), positions=0)
+    d.update(bad)
+    with pytest.raises(err, match=text):
+        append_kv_paged(**d)
+
+
+@pytest.mark.parametrize("bad,err,text", [
+    (dict(), RuntimeError, "CUDA"),
+    (dict(pools=[]), ValueError, "at least one pool"),
+    (dict(pools=[pool(), pool(NP=7)]), ValueError, "same number"),
+    (dict(pools=[pool(), pool(page=32)]), ValueError, "same number"),
+    (dict(pools=[3]), TypeError, "QuantizedTensor"),
+    (dict(seq_lens=i32(2)), ValueError, "seq_lens"),
+    (dict(parents=i32(2, 2)), ValueError, "parents"),
+    (dict(parents=i32(2).long()), ValueError, "parents"),
+    (dict(reserve=-1), ValueError, "reserve"),
+    (dict(reserve=2 ** 31), ValueError, "reserve"),
+    (dict(reserve=i32(3)), ValueError, "reserve"),
+    (dict(out=(i32(2, 4), i32(2), i32(1))), ValueError, r"out\[0\]"),
+    (dict(out=(i32(2, 5), i32(2), i32(2))), ValueError, r"out\[2\]"),
+])
+def test_fork_refuses(bad, err, text):
+    d = dict(pools=[pool()], block_table=i32(3, 5), seq_lens=i32(3), parents=i32(2))
+    d.update(bad)
+    with pytest.raises(err, match=text):
+        fork_pages(**d)
+
+
+def test_compact_refuses():
+    with pytest.raises(RuntimeError, match="CUDA"):
+        compact_pages(pool(), i32(3, 5))
+    with pytest.raises(ValueError, match="int32"):
+        compact_pages(pool(), i32(3, 5).float())
+    t = i32(3, 5)
+    with pytest.raises(ValueError, match="share memory"):
+        compact_pages(pool(), t, out=(t, i32(1)))
+
+
+def test_c_entries_refuse():
+    """Argument errors of the C ABI come back before any launch."""
+    lib, P = _cabi.load(), 4096  # a pointer that nothing follows: every call fails before that
+
+    def decode(q=P, out=P, B=1, HQ=4, HKV=2, NP=8, page=16, W=4, D=64, nbits=4, gs=32, dt=0, scale=P):
+        return lib.tkv_paged_decode(q, dt, P, scale, P, P, P, P, P, W, P, out, 0, B, HQ, HKV, NP, page, W, D, nbits, gs, 1.0, None)
+
+    I, U, A = _cabi.TKV_ERR_INVALID, _cabi.TKV_ERR_UNSUPPORTED, _cabi.TKV_ERR_ALIGN
+    for rc, kw in ((I, dict(q=None)), (I, dict(B=0)), (I, dict(HQ=5)), (I, dict(NP=0)), (I, dict(nbits=3)), (I, dict(dt=7)),
+                   (I, dict(NP=1 << 27)), (I, dict(W=1 << 27)), (U, dict(page=24)), (U, dict(D=96)), (U, dict(gs=8)),
+                   (U, dict(gs=128)), (A, dict(q=P + 8)), (A, dict(scale=P + 2)), (A, dict(out=P + 4))):
+        assert decode(**kw) == rc, (kw, _cabi.last_error())
+    assert lib.tkv_paged_fp16_decode(P, 0, P, None, P, 4, P, P, 0, 1, 4, 2, 8, 16, 4, 64, 1.0, None) == I
+    i6 = (ctypes.c_int64 * 6)(*[64] * 6)
+
+    def append(k=P, st=i6, B=1, T=1, D=64, nbits=4, gs=32, dt=0, val=None, vs=None, scale=P):
+        return lib.tkv_paged_append(k, P, dt, st, P, scale, P, P, P, P, val, None, vs, P, 4, None, 0, None, B, 2, T, 8, 16, 4, D,
+                                    nbits, gs, None)
+
+    odd = (ctypes.c_int64 * 6)(*[63] * 6)
+    for rc, kw in ((I, dict(k=None)), (I, dict(nbits=3)), (I, dict(B=-1)), (I, dict(dt=5)), (I, dict(scale=None)),
+                   (I, dict(val=P)), (U, dict(D=48)), (U, dict(gs=4)), (U, dict(gs=128)), (U, dict(D=16, gs=16, nbits=2)),
+                   (A, dict(st=odd)), (A, dict(k=P + 2)), (I, dict(T=1 << 30, B=4))):
+        assert append(**kw) == rc, (kw, _cabi.last_error())
+    assert append(B=0) == 0 and append(T=0) == 0
+    ptrs, sizes = (ctypes.c_void_p * 1)(P), (ctypes.c_int64 * 1)(64)
+
+    def fork(B=2, Bo=2, W=4, NP=8, page=16, par=P, ws=P, pools=ptrs, n=1):
+        return lib.tkv_pages_fork(P, W, P, Bo, par, None, 0, B, W, NP, page, P, P, P, ws, pools, sizes, n, None)
+
+    for kw in (dict(par=None), dict(ws=None), dict(NP=0), dict(page=0), dict(B=-1), dict(W=1 << 29), dict(pools=None), dict(n=-1)):
+        assert fork(**kw) == I, (kw, _cabi.last_error())
+
+    def compact(B=2, W=4, NP=8, live=P, n=1):
+        return lib.tkv_pages_compact(P, W, B, W, NP, P, live, P, ptrs, sizes, n, None)
+
+    for kw in (dict(B=1 << 16), dict(NP=0), dict(live=None), dict(W=1 << 29), dict(n=-1)):
+        assert compact(**kw) == I, (kw, _cabi.last_error())

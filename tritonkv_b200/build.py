@@ -30,6 +30,9 @@ SOURCES = [
     "tkv_decode_fused.cu",
     "tkv_decode_fp16.cu",
     "tkv_decode_static.cu",
+    "tkv_paged_attn.cu",
+    "tkv_paged_append.cu",
+    "tkv_pages.cu",
 ]
 
 NVCC_FLAGS = [
