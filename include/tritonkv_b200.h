@@ -233,13 +233,20 @@ int tkv_combine_exchange(const float* acc, const float* m, const float* l, float
 int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_packed, const void* k_scale,
                      const void* k_zero, const uint8_t* v_packed, const void* v_scale,
                      const void* v_zero, const int32_t* block_table, int64_t table_stride,
-                     const int32_t* seq_lens, void* out, int out_dtype, int B, int HQ, int HKV,
-                     int num_pages, int page_size, int max_pages, int D, int nbits, int gs,
-                     float sm_scale, void* stream);
+                     const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
+                     int64_t workspace_bytes, int B, int HQ, int HKV, int num_pages, int page_size,
+                     int max_pages, int D, int nbits, int gs, float sm_scale, void* stream);
 int tkv_paged_fp16_decode(const void* q, int q_dtype, const void* k, const void* v,
                           const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
-                          void* out, int out_dtype, int B, int HQ, int HKV, int num_pages,
-                          int page_size, int max_pages, int D, float sm_scale, void* stream);
+                          void* out, int out_dtype, void* workspace, int64_t workspace_bytes, int B,
+                          int HQ, int HKV, int num_pages, int page_size, int max_pages, int D,
+                          float sm_scale, void* stream);
+
+/* Bytes of device workspace (partials of the split history) that the two calls above need on the
+ * current device; nbits = 16 for the f16 form.  Calls that may run at the same time need
+ * workspaces of their own. */
+int tkv_paged_workspace(int B, int HQ, int HKV, int page_size, int D, int nbits, int gs,
+                        int64_t* bytes);
 
 /* Quantise T new tokens per (sequence, head) of K and of V -- element (b, h, t, d) of k at
  * strides[0]*b + strides[1]*h + strides[2]*t + d, of v with strides[3..5] -- into their pages, at

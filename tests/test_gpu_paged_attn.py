@@ -194,18 +194,18 @@ def test_streams_graphs_and_workspaces(nbits):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=s):
             attend(q, k, v, tb, sl, out=out, _workspace=ws)
-        runs.append((g, out, s))
+        runs.append((g, out, s, ws))  # a captured call's workspace lives as long as its graph
     for now in (lens, [1500, 0, 3, 64], [0, 0, 0, 0]):
         sl.copy_(lens_t(now))
         if now is not lens:
             tb.copy_(table[[3, 1, 0, 0]])
         torch.cuda.synchronize()
         for _ in range(3):
-            for g, _, s in runs:
+            for g, _, s, _ in runs:
                 with torch.cuda.stream(s):
                     g.replay()
         torch.cuda.synchronize()
-        for _, out, _ in runs:
+        for _, out, _, _ in runs:
             check(out, q, k, v, tb, now, f"replayed {now}")
         assert torch.equal(runs[0][1], runs[1][1])
         assert torch.equal(attend(q, k, v, tb, sl), runs[0][1])

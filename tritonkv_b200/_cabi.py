@@ -77,11 +77,13 @@ SIGNATURES = {
                                         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                         c_int, c_int, c_int, c_float, c_void_p]),
     "tkv_paged_decode": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                 c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int,
-                                 c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p]),
+                                 c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64,
+                                 c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+                                 c_void_p]),
     "tkv_paged_fp16_decode": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
-                                      c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                      c_float, c_void_p]),
+                                      c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int,
+                                      c_int, c_int, c_int, c_float, c_void_p]),
+    "tkv_paged_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
     "tkv_paged_append": (c_int, [c_void_p, c_void_p, c_int, POINTER(c_int64), c_void_p, c_void_p, c_void_p,
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, POINTER(c_int64),
                                  c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
@@ -261,6 +263,28 @@ def decode_plan(kernel_id: int, nbits: int, D: int, gs: int, B: int, HQ: int, HK
         if len(_plan_cache) < 4096:
             _plan_cache[key] = r
     return r
+
+
+_paged_bytes: dict = {}
+
+
+def paged_workspace(ws: dict | None, B: int, HQ: int, HKV: int, page: int, D: int, nbits: int, gs: int,
+                    device) -> torch.Tensor:
+    """The partials' buffer of a paged decode call, kept in the caller's dict ``ws`` (key ``paged``)."""
+    key = (B, HQ, HKV, page, D, nbits, gs, _current_device())
+    need = _paged_bytes.get(key)
+    if need is None:
+        v = c_int64(0)
+        check(load().tkv_paged_workspace(B, HQ, HKV, page, D, nbits, gs, ctypes.byref(v)))
+        need = v.value
+        if len(_paged_bytes) < 4096:
+            _paged_bytes[key] = need
+    t = None if ws is None else ws.get("paged")
+    if t is None or t.numel() < need or t.device != device:
+        t = torch.empty(need, dtype=torch.uint8, device=device)
+        if ws is not None:
+            ws["paged"] = t
+    return t
 
 
 _wave_cache: dict = {}

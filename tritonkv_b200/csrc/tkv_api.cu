@@ -19,6 +19,8 @@ int fp16_attrs(int D, int* regs, int* smem, int* local, int* ctas);
 int fused_device_status(int* status);
 int fp16_device_status(int* status);
 int exchange_device_status(int* status);
+int paged_device_status(int* status);
+int paged_device_status_clear();
 int fused_device_status_clear();
 int fp16_device_status_clear();
 int exchange_device_status_clear();
@@ -109,14 +111,16 @@ extern "C" int tkv_wave_programs(int kernel_id, int nbits, int D, int gs, int* p
 
 extern "C" int tkv_device_status(int* status) {
   TKV_REQUIRE(status, TKV_ERR_INVALID, "device_status: null output");
-  int a = 0, b = 0, c = 0;
+  int a = 0, b = 0, c = 0, e = 0;
   int rc = fused_device_status(&a);
   if (rc != TKV_OK) return rc;
   rc = fp16_device_status(&b);
   if (rc != TKV_OK) return rc;
+  rc = paged_device_status(&e);
+  if (rc != TKV_OK) return rc;
   rc = exchange_device_status(&c);
   if (rc != TKV_OK) return rc;
-  *status = a | b | (c << 1);
+  *status = a | b | e | (c << 1);
   return TKV_OK;
 }
 
@@ -124,6 +128,8 @@ extern "C" int tkv_device_status_clear(void) {
   int rc = fused_device_status_clear();
   if (rc != TKV_OK) return rc;
   rc = fp16_device_status_clear();
+  if (rc != TKV_OK) return rc;
+  rc = paged_device_status_clear();
   if (rc != TKV_OK) return rc;
   return exchange_device_status_clear();
 }

@@ -53,6 +53,7 @@ struct Fp16Policy {
   // Fill one stage with the 16 tokens starting at global row `row`: 16-byte cp.async per
   // lane into the 128B-swizzled layout (rows past the unit end are zero-filled), then one
   // arrival per lane on the stage barrier that fires when the lane's copies have landed.
+  static constexpr int PIECES = 1;  // paged caches: a tile lies in one page
   struct IssueState {};
   __device__ static __forceinline__ void issue_init(IssueState&, const DecodeParams&, int) {}
   __device__ static __forceinline__ void issue(const IssueState&, const DecodeParams& p,
@@ -72,6 +73,14 @@ struct Fp16Policy {
                  ok ? 16 : 0);
     }
     cp_async_mbar_arrive_noinc(bar);
+  }
+
+  // The same from a paged cache: rows[0] is the tile's first pool row, or negative -- then nothing is
+  // read and the tile is zero.
+  __device__ static __forceinline__ void issue_pieces(const IssueState& is, const DecodeParams& p,
+                                                      const Maps& maps, const int (&rows)[1], int nvalid,
+                                                      uint32_t st, uint32_t bar, int lane) {
+    issue(is, p, maps, max(rows[0], 0), rows[0] < 0 ? 0 : nvalid, st, nullptr, bar, lane);
   }
 
   // query fragments: B operand, k-slots (2t,2t+1) <-> dims 16c+2t, 16c+2t+1 and

@@ -86,11 +86,16 @@ __device__ __forceinline__ __half2 meta_bcast(const MetaRow<NG>& r, int i) {
 // quantised per channel over groups of kTok tokens) instead of D/GS values per token.  With
 // GS == kTok both forms fill the same bytes of a stage, so only the source address of the two
 // K metadata copies and the score arithmetic differ.
+// PIECES (paged caches): a tile arrives in this many runs of consecutive token rows, each from a
+// page of its own.  With two, the codes of a stage lie as [K 0-15 | V 0-15 | K 16-31 | V 16-31], so
+// that one copy still brings a K and a V run; see issue_pieces.
 template <int NBITS, int D_, int GS, bool A16 = true, int TOK_ = 32, int WARPS_ = 4, int STAGES_ = 3,
-          int MIN_CTAS_ = 3, bool PIPELINED_ = true, bool KCHAN_ = false>
+          int MIN_CTAS_ = 3, bool PIPELINED_ = true, bool KCHAN_ = false, int PIECES_ = 1>
 struct FusedPolicy {
   using C = FusedCfg<NBITS, D_, GS, TOK_>;
   static constexpr bool KCHAN = KCHAN_;
+  static constexpr int PIECES = PIECES_;
+  static_assert(PIECES == 1 || (PIECES == 2 && TOK_ == 32 && A16 && !KCHAN_), "a piece is one 16-token MMA block");
   static_assert(!KCHAN || (GS == TOK_ && A16 && D_ / GS > 1),
                 "per-channel keys: value groups of one tile's tokens, 16-byte aligned rows");
   static constexpr int D = D_;
@@ -114,6 +119,7 @@ struct FusedPolicy {
     uint32_t qz0, qz1;    // B operand of the K zero-point MMA: f16 hi / lo parts of
                           // qk_scale * (sum of q over a group), groups 2t and 2t+1
     uint32_t off[MT][C::NPAIR];  // this lane's ldmatrix byte offsets inside a code tile
+    uint32_t off_v[PIECES == 2 ? MT : 1][C::NPAIR];  // in two pieces: of V, in the stage (`off`: of K)
     uint32_t o_row;   // byte offset of token g's row inside a scale array
     uint32_t o_kz;    // byte offset of this lane's K zero-point word (token g)
     uint32_t o_vz;    // byte offset of this lane's first V zero-point (token 2t, group g mod NG)
@@ -125,6 +131,10 @@ struct FusedPolicy {
     float m_true0, m_true1;  // this lane's running maxima (reduced over lanes in finalize)
     float acc[NCH][4];
     float zacc[4];  // rows 0..NG-1: sum_n p_n z_n[group]; row 8: sum_n p_n
+  };
+
+  struct Scores {
+    float s[MT][4];  // [16-token block][(token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)]
   };
 
   __device__ static void report_timeout() { atomicExch(&g_fused_status, 1); }
@@ -215,6 +225,70 @@ struct FusedPolicy {
     (void)st_ptr;
   }
 
+  // Fill one stage from a paged cache: piece h of the tile is the run of 32 / PIECES token rows
+  // that starts at pool row rows[h], or nowhere (negative: nothing is read, scale = zero = 0).  Pool rows
+  // are viewed as 128-byte rows (a page is a multiple of 16 tokens, so runs start on them).
+  static constexpr int PIECE_BYTES = kTok / PIECES * DP;
+  __device__ static __forceinline__ void issue_pieces(const IssueState& is, const DecodeParams& p,
+                                                      const Maps& maps, const int (&rows)[PIECES],
+                                                      int nvalid, uint32_t st, uint32_t bar, int lane) {
+    bool all = true;
+#pragma unroll
+    for (int h = 0; h < PIECES; ++h) all = all && rows[h] >= 0;
+    if (lane == 0) {
+      constexpr int SH = (DP == 64) ? 1 : (DP == 32) ? 2 : 3;
+      int n = 0;
+#pragma unroll
+      for (int h = 0; h < PIECES; ++h) n += rows[h] >= 0 ? 1 : 0;
+      mbar_arrive_expect_tx(bar, n * 2 * PIECE_BYTES);
+#pragma unroll
+      for (int h = 0; h < PIECES; ++h) {
+        if (rows[h] < 0) continue;
+        const uint32_t dst = st + h * 2 * PIECE_BYTES;
+        if (p.kv_one) {
+          tma_load_3d(dst, &maps.k, 0, rows[h] >> SH, 0, bar);
+        } else {
+          tma_load_2d(dst, &maps.k, 0, rows[h] >> SH, bar);
+          tma_load_2d(dst + (PIECES == 2 ? PIECE_BYTES : C::CODE_BYTES), &maps.v, 0, rows[h] >> SH, bar);
+        }
+      }
+    }
+    const uint32_t mst = st + 2 * C::CODE_BYTES;
+    if (NG == 1 && lane == 0)  // no read-back shift (see FusedCfg::META_STRIDE)
+      asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(mst + C::SHIFT_WORD), "r"(0u) : "memory");
+    constexpr int CPP = CPA / PIECES;  // 16-byte chunks of one array that a piece fills
+    const int vbytes = nvalid * NG * 2;
+    all = all && nvalid == kTok;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int i = r * 32 + lane, arr = (i / CPA) & 3, c = i % CPA;
+      const int h = PIECES == 2 ? c / CPP : 0;
+      const int row = (PIECES == 2 && h) ? rows[PIECES - 1] : rows[0];
+      const uint8_t* src = is.src[r] + ((int64_t)row * (NG * 2) - h * CPP * 16);
+      const uint32_t dst = NG == 1 ? mst + arr * C::META_STRIDE + c * 16 : mst + i * 16;
+      if (4 * CPA >= 32 || i < 4 * CPA) {
+        if (all) {
+          cp_async16(dst, src, 16);
+        } else {
+          const int nb = row < 0 ? 0 : min(max(vbytes - c * 16, 0), 16);
+          cp_async16(dst, nb > 0 ? src : is.src[r], nb);
+        }
+      }
+    }
+    cp_async_mbar_arrive_noinc(bar);
+  }
+
+  // Scores of pieces that name no page (bit h of `valid` clear)
+  __device__ static __forceinline__ void mask_pieces(Scores& sc, uint32_t valid) {
+#pragma unroll
+    for (int h = 0; h < PIECES; ++h)
+      if (!((valid >> h) & 1u)) {
+#pragma unroll
+        for (int mt = h * MT / PIECES; mt < (h + 1) * MT / PIECES; ++mt)
+          sc.s[mt][0] = sc.s[mt][1] = sc.s[mt][2] = sc.s[mt][3] = -INFINITY;
+      }
+  }
+
   // Scale/zero of a tile in CS-byte copies: rows that only start on 8- or 4-byte boundaries
   // (odd history lengths), and the last tile of a unit, whose tokens past the end are
   // zero-filled by the copy itself (scale = zero = 0 makes them contribute exact zeros).
@@ -249,6 +323,16 @@ struct FusedPolicy {
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int pr = 0; pr < C::NPAIR; ++pr) {
+        if constexpr (PIECES == 2) {
+          // byte offset of the chunk in the stage; the 128B swizzle goes by address bits 7-9
+          auto at = [&](int second) {
+            const int L = ((2 * mt + second) * PIECE_BYTES + lm_r * DP) / 16 + 2 * pr + lm_b;
+            return (uint32_t)(((L & ~7) | ((L ^ (L >> 3)) & 7)) << 4);
+          };
+          qq.off[mt][pr] = at(p.kv_one && p.k_second);
+          qq.off_v[mt][pr] = at(!(p.kv_one && p.k_second));
+          continue;
+        }
         const int n = 16 * mt + lm_r, blk = 2 * pr + lm_b;
         const int L = n * NBLK + blk;  // linear 16-byte chunk index inside the tile
         int Ls;
@@ -264,8 +348,12 @@ struct FusedPolicy {
     qq.o_kz = (NG >= 2) ? (g * NG + ((2 * t) % NG)) * 2 : g * 2;
     qq.o_vz = ((2 * t) * NG + (g % NG)) * 2;
     qq.ones = (lane < 4) ? 0x3C003C00u : 0u;
-    qq.kofs = (p.kv_one && p.k_second) ? C::CODE_BYTES : 0;
-    qq.vofs = C::CODE_BYTES - qq.kofs;
+    qq.kofs = (PIECES == 1 && p.kv_one && p.k_second) ? C::CODE_BYTES : 0;
+    qq.vofs = PIECES == 1 ? C::CODE_BYTES - qq.kofs : 0;
+  }
+  __device__ static __forceinline__ uint32_t v_off(const Query& qq, int mt, int pr) {
+    if constexpr (PIECES == 2) return qq.off_v[mt][pr];
+    else return qq.off[mt][pr];
   }
 
   // Query fragments of a segment are the same for the four warps: each warp builds the
@@ -364,10 +452,6 @@ struct FusedPolicy {
 #pragma unroll
     for (int i = 0; i < 4; ++i) ac.zacc[i] = 0.f;
   }
-
-  struct Scores {
-    float s[MT][4];  // [16-token block][(token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)]
-  };
 
   // Scores of one tile in stage `st` (scaled by qk_scale, tokens past the unit
   // end set to -inf); `left` = tokens from the tile start to the unit end.
@@ -653,9 +737,9 @@ struct FusedPolicy {
       for (int bb = 0; bb < NBLK; bb += 2) {
         uint32_t r[4];
         if constexpr (NBLK >= 2) {
-          ldmatrix_x4_trans(r, vc + qq.off[mt][bb >> 1]);
+          ldmatrix_x4_trans(r, vc + v_off(qq, mt, bb >> 1));
         } else {
-          ldmatrix_x2_trans(r[0], r[1], vc + qq.off[mt][0]);
+          ldmatrix_x2_trans(r[0], r[1], vc + v_off(qq, mt, 0));
           r[2] = r[3] = 0;
         }
 #pragma unroll

@@ -6,160 +6,753 @@
 // pool that has the layout of the contiguous cache with pages in the place of sequences.  Table
 // entries outside the pool hold no tokens: theirs are not attended.
 //
-// One CTA owns one (sequence, query head) and walks the history in blocks of kTokens tokens with
-// a running maximum and sum in f32: a thread scores one token, then the threads turn to head dims
-// and add the block's weighted values.
-#include "tkv_common.cuh"
+// The tiles, their arithmetic and the per-warp copy rings are those of the contiguous kernels
+// (tkv_fused_policy.cuh, tkv_fp16_policy.cuh); what differs is where a tile comes from and how the
+// work is cut.  A tile of 32 packed tokens is one run of rows where the page is a multiple of 32
+// tokens, else two runs of 16 (PIECES).  When a warp enters a segment its lanes look up the pool
+// rows of the warp's next 32 tiles, one each; an issue takes its row by a shuffle, so the table's
+// latency is paid once per 32 tiles and hidden behind the tiles in flight.
+//
+// Lengths live on the device.  Every CTA builds the prefix of tiles per sequence in shared memory
+// and takes an equal range of the tile sequence, whatever the lengths are; a range that crosses
+// from one unit (sequence, KV head, 8 query heads) to the next is processed segment by segment.  A
+// unit that one CTA has to itself goes straight to the output.  Else segment (unit u, CTA c) leaves
+// its partial (acc, m, l) in slot u + c -- distinct for all segments, since the next unit starts no
+// earlier than in the CTA where this one ends -- and the unit's first CTA notes where its slots
+// begin and how many they are, for the merge that follows.  So the workspace holds units + CTAs
+// partials whatever the lengths, and no slot has to be marked empty.
+#include "tkv_fp16_policy.cuh"
+#include "tkv_fused_policy.cuh"
 
 namespace tkv {
 
-struct PagedArgs {
-  const void* q;
-  const uint8_t *kp, *vp;             // packed pages, or the float16 pages themselves
-  const __half *ks, *kz, *vs, *vz;
+constexpr int kMaxPagedB = 512;  // sequences whose tile prefix a CTA holds; larger batches go in parts
+
+struct PagedParams {
+  DecodeParams d;         // what the tile policies read; d.B sequences of this launch
   const int32_t* table;
-  const int32_t* seq_lens;
-  void* out;
   int64_t table_stride;
-  int q_dtype, out_dtype;
-  int B, HQ, HKV, D, num_pages, page, max_pages, gs;
-  float qk_scale;                     // sm_scale * log2(e)
+  void* out;
+  int out_dtype;
+  int num_pages, page, max_pages, HKVc;
+  FastDiv dpage, dHch, dHKVc;
+  float *acc, *m, *l;     // (slots, 8, D), (slots, 8), (slots, 8)
+  int2* info;             // (units): first slot and number of partials; none: the output is there
 };
 
-constexpr int kTokens = 128;
-
-// Element d of cache row `row` (NBITS == 16: float16 pages)
-template <int NBITS>
-__device__ __forceinline__ float cache_value(const uint8_t* codes, const __half* scale, const __half* zero,
-                                             int64_t row, int d, int D, int gs) {
-  if constexpr (NBITS == 16) {
-    return __half2float(reinterpret_cast<const __half*>(codes)[row * D + d]);
+__device__ __forceinline__ void store_out4(void* out, int dtype, int64_t i, float4 v) {
+  if (dtype == TKV_DTYPE_F32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + i) = v;
+  } else if (dtype == TKV_DTYPE_F16) {
+    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(out) + i) = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
   } else {
-    const int DP = D * NBITS / 8, p = d / DP;
-    const int code = (codes[row * DP + (d - p * DP)] >> (NBITS * p)) & ((1 << NBITS) - 1);
-    const int64_t g = row * (D / gs) + d / gs;
-    return fmaf((float)code, __half2float(scale[g]), __half2float(zero[g]));
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(out) + i) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
   }
 }
 
-template <int NBITS>
-__global__ void __launch_bounds__(kTokens) paged_attention_kernel(const PagedArgs a) {
-  __shared__ float s_q[128], s_p[kTokens], s_red[4];
-  __shared__ int64_t s_row[kTokens];
-  const int tid = threadIdx.x, b = blockIdx.x / a.HQ, h = blockIdx.x - b * a.HQ;
-  const int hkv = h / (a.HQ / a.HKV), D = a.D;
-  const int64_t qrow = ((int64_t)b * a.HQ + h) * D;
-  if (tid < D) s_q[tid] = __half2float(load_q_half(a.q, a.q_dtype, qrow + tid)) * a.qk_scale;
-  const int len = (int)min((int64_t)max(a.seq_lens[b], 0), (int64_t)a.max_pages * a.page);
-  float M = -INFINITY, L = 0.f, acc = 0.f;
-  for (int n0 = 0; n0 < len; n0 += kTokens) {
-    __syncthreads();
-    const int n = n0 + tid;
-    int64_t row = -1;
-    float s = -INFINITY;
-    if (n < len) {
-      const int i = n / a.page, id = a.table[b * a.table_stride + i];
-      if (id >= 0 && id < a.num_pages) row = ((int64_t)id * a.HKV + hkv) * a.page + (n - i * a.page);
-    }
-    if (row >= 0) {
-      s = 0.f;
-      for (int d = 0; d < D; ++d)
-        s = fmaf(s_q[d], cache_value<NBITS>(a.kp, a.ks, a.kz, row, d, D, a.gs), s);
-    }
-    float m = s;
-    for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
-    if ((tid & 31) == 0) s_red[tid >> 5] = m;
-    s_row[tid] = row;
-    __syncthreads();
-    m = fmaxf(M, fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])));
-    if (m == -INFINITY) continue;  // nothing to attend so far
-    s_p[tid] = ex2(s - m);
-    __syncthreads();
-    const float alpha = ex2(M - m);
-    M = m;
-    L *= alpha;
-    acc *= alpha;
-    const int count = min(kTokens, len - n0);
-    for (int j = 0; j < count; ++j) {
-      if (s_row[j] < 0) continue;  // what lies there may be anything
-      L += s_p[j];
-      if (tid < D) acc = fmaf(s_p[j], cache_value<NBITS>(a.vp, a.vs, a.vz, s_row[j], tid, D, a.gs), acc);
-    }
+struct PagedSegment {
+  int b, hkv, hc, unit;
+  int lo_tok, hi;   // first token; end of the sequence
+  int ntiles, g_end;
+  int first, count; // first CTA of the unit and how many it spans
+};
+
+template <int kTok>
+__device__ __forceinline__ PagedSegment paged_segment_at(const PagedParams& pp, const int* pref, FastDiv dTC,
+                                                         int g, int g1) {
+  PagedSegment s;
+  int lo = 0, hi = pp.d.B;  // largest b with HKVc * pref[b] <= g (sequences without tiles are skipped)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pp.HKVc * (pref[mid] >> kRemBits) <= g) lo = mid; else hi = mid;
   }
-  if (tid < D) {
-    const float o = L > 0.f ? acc / L : 0.f;
-    if (a.out_dtype == TKV_DTYPE_F32) reinterpret_cast<float*>(a.out)[qrow + tid] = o;
-    else if (a.out_dtype == TKV_DTYPE_F16) reinterpret_cast<__half*>(a.out)[qrow + tid] = __float2half_rn(o);
-    else reinterpret_cast<__nv_bfloat16*>(a.out)[qrow + tid] = __float2bfloat16_rn(o);
-  }
+  const int word = pref[lo], before = word >> kRemBits;
+  const int t_b = (pref[lo + 1] >> kRemBits) - before;
+  const int r = g - pp.HKVc * before;
+  const int hk = (int)((uint32_t)r / (uint32_t)t_b);
+  const int tile = r - hk * t_b;
+  const int unit_start = g - tile, unit_end = unit_start + t_b;
+  s.b = lo;
+  s.unit = lo * pp.HKVc + hk;
+  s.hkv = fast_div(hk, pp.dHch);
+  s.hc = hk - s.hkv * pp.d.hchunks;
+  s.hi = (t_b - 1) * kTok + (word & ((1 << kRemBits) - 1)) + 1;
+  s.lo_tok = tile * kTok;
+  s.g_end = min(g1, unit_end);
+  s.ntiles = s.g_end - g;
+  s.first = fast_div(unit_start, dTC);
+  s.count = fast_div(unit_end - 1, dTC) - s.first + 1;
+  return s;
 }
 
-static int paged_check(const char* who, const PagedArgs& a, int nbits) {
-  TKV_REQUIRE(a.B > 0 && a.HQ > 0 && a.HKV > 0 && a.HQ % a.HKV == 0, TKV_ERR_INVALID,
-              "%s: bad sizes B=%d HQ=%d HKV=%d (HQ must be a multiple of HKV)", who, a.B, a.HQ, a.HKV);
-  TKV_REQUIRE(a.num_pages > 0 && a.page > 0 && a.max_pages >= 0, TKV_ERR_INVALID,
-              "%s: bad sizes num_pages=%d page_size=%d max_pages=%d", who, a.num_pages, a.page, a.max_pages);
-  TKV_REQUIRE(a.page % 16 == 0, TKV_ERR_UNSUPPORTED, "%s: unsupported page_size=%d (a multiple of 16 tokens)",
-              who, a.page);
-  TKV_REQUIRE((int64_t)a.num_pages * a.HKV * a.page < (1LL << 31), TKV_ERR_INVALID,
-              "%s: a pool of %lld token rows exceeds 2^31", who, (long long)a.num_pages * a.HKV * a.page);
-  TKV_REQUIRE((int64_t)a.max_pages * a.page < (1LL << 30), TKV_ERR_INVALID,
-              "%s: a table row of %lld tokens exceeds 2^30", who, (long long)a.max_pages * a.page);
-  TKV_REQUIRE((int64_t)a.B * a.HQ < (1LL << 31), TKV_ERR_INVALID, "%s: B*HQ exceeds 2^31", who);
-  TKV_REQUIRE(a.q_dtype >= 0 && a.q_dtype <= 2 && a.out_dtype >= 0 && a.out_dtype <= 2, TKV_ERR_INVALID,
-              "%s: bad dtype codes %d, %d", who, a.q_dtype, a.out_dtype);
-  TKV_REQUIRE(a.D == 64 || a.D == 128, TKV_ERR_UNSUPPORTED, "%s: unsupported head_dim=%d (built: 64, 128)", who, a.D);
-  if (nbits != 16) {
-    TKV_REQUIRE(nbits == 2 || nbits == 4, TKV_ERR_INVALID, "nbits must be one of (2, 4), got %d", nbits);
-    TKV_REQUIRE((a.gs == 16 || a.gs == 32 || a.gs == 64 || a.gs == 128) && a.gs <= a.D, TKV_ERR_UNSUPPORTED,
-                "%s: unsupported (nbits=%d, head_dim=%d, group_size=%d); built: group_size in {16,32,64,128} "
-                "with group_size <= head_dim", who, nbits, a.D, a.gs);
-    TKV_REQUIRE(aligned16(a.ks) && aligned16(a.kz) && aligned16(a.vs) && aligned16(a.vz), TKV_ERR_ALIGN,
-                "%s: scale and zero pointers must be 16-byte aligned", who);
+// Where a warp's copies stand: the next tile to issue, segments ahead of the one being computed.
+template <int PIECES>
+struct PagedCursor {
+  int b, hkv;
+  int tok, hi;       // first token of the next tile; end of the sequence
+  int cnt, g_end;    // tiles left in the cursor's segment; its end
+  int k;             // which lane's row the next tile takes
+  int row[PIECES];   // this lane's: pool rows of tile `lane` of the present 32, or -1
+};
+
+template <class Policy>
+__global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
+    paged_split_kernel(const __grid_constant__ typename Policy::Maps maps, const PagedParams pp) {
+  constexpr int WARPS = Policy::WARPS, STAGES = Policy::STAGES, D = Policy::D, PIECES = Policy::PIECES;
+  constexpr int kTok = Policy::TOK, STAGE_BYTES = Policy::STAGE_BYTES;
+  constexpr int kLog2D = D == 64 ? 6 : 7;
+  static_assert((1 << kLog2D) == D && Policy::PIPELINED && STAGES >= 3 && STAGE_BYTES % 1024 == 0 &&
+                    STAGE_BYTES >= kHeadsPerCta * D * 4 && STAGES * 2 <= 32,
+                "the software-pipelined ring");
+  const DecodeParams& p = pp.d;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ float s_m[WARPS][kHeadsPerCta];
+  __shared__ float s_l[WARPS][kHeadsPerCta];
+  __shared__ int s_slot[WARPS];
+  const int warp = __shfl_sync(kFullMask, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int cta = blockIdx.x;
+  pdl_launch_dependents();  // the whole grid is resident: the merge may take its place and wait
+  if (threadIdx.x == 0) Policy::prefetch_maps(maps);
+
+  uint8_t* ring = smem + (size_t)warp * STAGES * STAGE_BYTES;
+  const uint32_t ring_u32 = smem_u32(ring);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)WARPS * STAGES * STAGE_BYTES);
+  const uint32_t bar_u32 = smem_u32(bars + warp * STAGES);
+  constexpr int QB = kHeadsPerCta * D * 4;  // query rows of a segment, staged one segment ahead
+  uint64_t* qbars = bars + WARPS * STAGES;
+  const uint32_t qbar_u32 = smem_u32(qbars);
+  uint8_t* qbuf = reinterpret_cast<uint8_t*>(qbars + 2);
+  const uint32_t qbuf_u32 = smem_u32(qbuf);
+  const uint32_t qfrag_u32 = qbuf_u32 + 2 * QB;
+  int* s_pref = reinterpret_cast<int*>(qbuf + 2 * QB + ((Policy::QFRAG_BYTES + 15) & ~15));
+  if (lane == 0) {
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) mbar_init(bar_u32 + 8 * s, Policy::BAR_COUNT);
+    if (warp == 0) {
+      mbar_init(qbar_u32, WARPS * 32);
+      mbar_init(qbar_u32 + 8, WARPS * 32);
+    }
+    fence_barrier_init();
   }
-  TKV_REQUIRE(a.q && a.kp && a.vp && a.seq_lens && a.out && (a.table || a.max_pages == 0), TKV_ERR_INVALID,
-              "%s: null pointer", who);
-  TKV_REQUIRE(aligned16(a.q) && aligned16(a.kp) && aligned16(a.vp) && aligned16(a.out), TKV_ERR_ALIGN,
-              "%s: q, the pools and out must be 16-byte aligned", who);
+  const int q_esz = p.q_dtype == TKV_DTYPE_F32 ? 4 : 2;
+  auto prefetch_q = [&](int slot, const PagedSegment& s) {
+    const int row_bytes = D * q_esz, cpr = row_bytes >> 4, cpr_shift = q_esz == 4 ? kLog2D - 2 : kLog2D - 3;
+    for (int i = threadIdx.x; i < kHeadsPerCta * cpr; i += WARPS * 32) {
+      const int h = i >> cpr_shift, c = i - (h << cpr_shift);
+      const int hg = s.hc * kHeadsPerCta + h;
+      const bool ok = hg < p.group;
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
+                           (((int64_t)s.b * p.HQ + (int64_t)s.hkv * p.group + hg) * D) * q_esz + c * 16;
+      cp_async16(qbuf_u32 + slot * QB + h * row_bytes + c * 16,
+                 ok ? src : reinterpret_cast<const uint8_t*>(p.q), ok ? 16 : 0);
+    }
+    cp_async_mbar_arrive_noinc(qbar_u32 + 8 * slot);
+  };
+  typename Policy::IssueState ist;
+  Policy::issue_init(ist, p, lane);
+  typename Policy::Query qs;
+  Policy::lane_init(qs, p, lane);
+
+  // ---- the tile sequence: word b = (tiles before sequence b) << kRemBits | tokens in its last tile - 1 ----
+  pdl_wait();
+  for (int b = threadIdx.x; b < p.B; b += WARPS * 32) s_pref[b] = min(max(p.seq_lens[b], 0), p.S);
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + lane;
+      const int len = b < p.B ? s_pref[b] : 0;
+      const int t = (len + kTok - 1) / kTok;
+      int incl = t;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(kFullMask, incl, off);
+        if (lane >= off) incl += y;
+      }
+      if (b < p.B) s_pref[b] = ((carry + incl - t) << kRemBits) | (t > 0 ? len - (t - 1) * kTok - 1 : 0);
+      carry += __shfl_sync(kFullMask, incl, 31);
+    }
+    if (lane == 0) s_pref[p.B] = carry << kRemBits;
+  }
+  __syncthreads();
+  const int T = pp.HKVc * (s_pref[p.B] >> kRemBits);
+  int TC = max(1, (T + (int)gridDim.x - 1) / (int)gridDim.x);
+  if (TC <= 4 * WARPS) TC = (TC + WARPS - 1) / WARPS * WARPS;  // no warp without a tile: fewer partials, same time
+  const FastDiv dTC = make_fastdiv_device(TC);
+  // sequences without tokens are touched by no range
+  for (int u = cta; u < p.B * pp.HKVc; u += gridDim.x) {
+    const int b = fast_div(u, pp.dHKVc), hk = u - b * pp.HKVc;
+    if ((s_pref[b + 1] >> kRemBits) != (s_pref[b] >> kRemBits)) continue;
+    const int hkv = fast_div(hk, pp.dHch), hc = hk - hkv * p.hchunks;
+    for (int idx = threadIdx.x; idx < kHeadsPerCta * D / 4; idx += WARPS * 32) {
+      const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4, hg = hc * kHeadsPerCta + h;
+      if (hg < p.group)
+        store_out4(pp.out, pp.out_dtype, ((int64_t)b * p.HQ + hkv * p.group + hg) * D + d, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+    if (threadIdx.x == 0) pp.info[u] = make_int2(0, 0);
+  }
+  const int g0 = min(cta * TC, T), g1 = min(g0 + TC, T);
+  if (g0 >= g1) return;
+  PagedSegment seg = paged_segment_at<kTok>(pp, s_pref, dTC, g0, g1);
+
+  // ---- issue cursor ----
+  PagedCursor<PIECES> cur;
+  auto look_up = [&]() {  // lane i: the rows of this warp's i-th tile from the cursor on
+    cur.k = 0;
+    const int tok = cur.tok + lane * (WARPS * kTok);
+#pragma unroll
+    for (int h = 0; h < PIECES; ++h) {
+      const int n = tok + h * (kTok / PIECES);
+      int row = -1;
+      if (lane < cur.cnt && n < cur.hi) {
+        const int i = fast_div(n, pp.dpage), id = __ldcg(pp.table + cur.b * pp.table_stride + i);
+        if ((unsigned)id < (unsigned)pp.num_pages) row = (id * p.HKV + cur.hkv) * pp.page + (n - i * pp.page);
+      }
+      cur.row[h] = row;
+    }
+  };
+  auto cursor_enter = [&](const PagedSegment& s) {
+    cur.b = s.b;
+    cur.hkv = s.hkv;
+    cur.tok = s.lo_tok + warp * kTok;
+    cur.hi = s.hi;
+    cur.cnt = s.ntiles > warp ? (s.ntiles - warp + WARPS - 1) / WARPS : 0;
+    cur.g_end = s.g_end;
+    if (cur.cnt > 0) look_up();
+  };
+  auto cursor_skip_empty = [&]() {  // to the next segment in which this warp has a tile
+    while (cur.cnt == 0 && cur.g_end < g1) cursor_enter(paged_segment_at<kTok>(pp, s_pref, dTC, cur.g_end, g1));
+  };
+  cursor_enter(seg);
+  cursor_skip_empty();
+  int iss_slot = 0;          // slot the next issue fills
+  uint32_t valid = 0;        // bits [s*PIECES, (s+1)*PIECES): which pieces of slot s name a page
+  constexpr uint32_t kAll = (1u << PIECES) - 1u;
+  bool need_proxy_fence = false;
+  auto issue_next = [&]() {
+    if (cur.cnt == 0) return;
+    const int slot = iss_slot;
+    iss_slot = (slot + 1 == STAGES) ? 0 : slot + 1;
+    if (need_proxy_fence) {  // a generic-proxy epilogue touched the ring since the last issue
+      fence_proxy_async();
+      need_proxy_fence = false;
+    }
+    int rows[PIECES];
+    uint32_t ok = 0;
+#pragma unroll
+    for (int h = 0; h < PIECES; ++h) {
+      rows[h] = __shfl_sync(kFullMask, cur.row[h], cur.k);
+      ok |= (rows[h] >= 0 ? 1u : 0u) << h;
+    }
+    valid = (valid & ~(kAll << (slot * PIECES))) | (ok << (slot * PIECES));
+    Policy::issue_pieces(ist, p, maps, rows, min(kTok, cur.hi - cur.tok), ring_u32 + slot * STAGE_BYTES,
+                         bar_u32 + 8 * slot, lane);
+    cur.tok += WARPS * kTok;
+    if (--cur.cnt == 0) cursor_skip_empty();
+    else if (++cur.k == 32) look_up();
+  };
+  prefetch_q(0, seg);
+#pragma unroll 1
+  for (int s = 0; s < STAGES - 1; ++s) issue_next();
+  if (seg.g_end < g1) prefetch_q(1, paged_segment_at<kTok>(pp, s_pref, dTC, seg.g_end, g1));
+  int seg_k = 0;  // index of the current segment within this CTA
+  int c_slot = 0, c_phase = 0;  // slot and barrier phase of the next tile to consume
+  bool timed_out = false;
+  typename Policy::Accum acc;
+
+  for (;;) {
+    // ---- one segment ----
+    if (!mbar_wait_bounded(qbar_u32 + 8 * (seg_k & 1), (seg_k >> 1) & 1)) timed_out = true;
+    if (Policy::QFRAG_BYTES > 0) {
+      Policy::build_query(p, qbuf + (seg_k & 1) * QB, qfrag_u32, warp, lane);
+      __syncthreads();
+    }
+    Policy::load_query(qs, p, qbuf + (seg_k & 1) * QB, qfrag_u32, lane);
+    Policy::reset(acc);
+    const int my_tiles = seg.ntiles > warp ? (seg.ntiles - warp + WARPS - 1) / WARPS : 0;
+    int left = seg.hi - (seg.lo_tok + warp * kTok);
+    auto scores = [&](typename Policy::Scores& sc, int slot, int left_of) {
+      Policy::scores(sc, qs, ring_u32 + slot * STAGE_BYTES, ring + slot * STAGE_BYTES, left_of, p.qk_scale, lane);
+      if constexpr (PIECES > 1) {
+        const uint32_t v = valid >> (slot * PIECES) & kAll;
+        if (v != kAll) Policy::mask_pieces(sc, v);
+      }
+    };
+    // a tile of nothing but unnamed pages adds nothing (and has no maximum)
+    auto update = [&](typename Policy::Scores& sc, int slot) {
+      if (valid >> (slot * PIECES) & kAll)
+        Policy::update(acc, qs, sc, ring_u32 + slot * STAGE_BYTES, ring + slot * STAGE_BYTES, left, lane);
+    };
+    // Software pipeline: the scores of tile i+1 beside the softmax and output of tile i.
+    if (my_tiles > 0 && !timed_out) {
+      typename Policy::Scores sc_cur;
+      if (!mbar_wait_bounded(bar_u32 + 8 * c_slot, c_phase)) timed_out = true;
+      __syncwarp();
+      if (!timed_out) scores(sc_cur, c_slot, left);
+      for (int i = 1; i < my_tiles && !timed_out; ++i) {
+        int n_slot = c_slot + 1, n_phase = c_phase;
+        if (n_slot == STAGES) {
+          n_slot = 0;
+          n_phase ^= 1;
+        }
+        if (!mbar_wait_bounded(bar_u32 + 8 * n_slot, n_phase)) {
+          timed_out = true;
+          break;
+        }
+        __syncwarp();
+        issue_next();  // refills the stage whose tile was finished in the previous iteration
+        typename Policy::Scores sc_next;
+        scores(sc_next, n_slot, left - WARPS * kTok);
+        update(sc_cur, c_slot);
+        sc_cur = sc_next;
+        left -= WARPS * kTok;
+        c_slot = n_slot;
+        c_phase = n_phase;
+      }
+      if (!timed_out) {
+        __syncwarp();
+        issue_next();
+        update(sc_cur, c_slot);
+        if (++c_slot == STAGES) {
+          c_slot = 0;
+          c_phase ^= 1;
+        }
+      }
+    }
+
+    // ---- merge the warps, store the partial or the output ----
+    const int vals_slot = (c_slot == 0 ? STAGES : c_slot) - 1;  // the stage consumed last
+    SoftmaxState st{-INFINITY, -INFINITY, 0.f, 0.f};
+    if (my_tiles > 0) Policy::finalize(acc, reinterpret_cast<float*>(ring + vals_slot * STAGE_BYTES), st, lane);
+    if ((lane >> 2) == 0) {
+      const int t = lane & 3;
+      s_m[warp][2 * t] = st.m0;
+      s_m[warp][2 * t + 1] = st.m1;
+      s_l[warp][2 * t] = st.l0;
+      s_l[warp][2 * t + 1] = st.l1;
+    }
+    if (lane == 0) s_slot[warp] = vals_slot;
+    __syncthreads();
+    {
+      constexpr int D4 = D / 4, ITEMS = kHeadsPerCta * D4;
+      uint32_t voff[WARPS];
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) voff[w] = (uint32_t)((w * STAGES + s_slot[w]) * STAGE_BYTES);
+      const int64_t slot = (int64_t)(seg.unit + cta) * kHeadsPerCta;
+#pragma unroll
+      for (int it = 0; it < ITEMS / (WARPS * 32); ++it) {
+        const int idx = it * (WARPS * 32) + threadIdx.x;
+        const int h = idx / D4, d = (idx - h * D4) * 4, hg = seg.hc * kHeadsPerCta + h;
+        if (hg >= p.group) continue;
+        float mw[WARPS], M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          mw[w] = s_m[w][h];
+          M = fmaxf(M, mw[w]);
+        }
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const bool live = mw[w] != -INFINITY;  // a warp without tiles left its stage unwritten
+          const float s = live ? ex2(mw[w] - M) : 0.f;
+          const float4 v = *reinterpret_cast<const float4*>(smem + voff[w] + (h * D + d) * 4);
+          a.x = fmaf(s, live ? v.x : 0.f, a.x);
+          a.y = fmaf(s, live ? v.y : 0.f, a.y);
+          a.z = fmaf(s, live ? v.z : 0.f, a.z);
+          a.w = fmaf(s, live ? v.w : 0.f, a.w);
+          L = fmaf(s, s_l[w][h], L);
+        }
+        if (seg.count > 1) {
+          *reinterpret_cast<float4*>(pp.acc + (slot + h) * D + d) = a;
+          if (d == 0) {
+            pp.m[slot + h] = M;
+            pp.l[slot + h] = L;
+          }
+        } else {
+          const float inv = L > 0.f ? 1.f / L : 0.f;
+          store_out4(pp.out, pp.out_dtype, ((int64_t)seg.b * p.HQ + seg.hkv * p.group + hg) * D + d,
+                     make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+        }
+      }
+      if (threadIdx.x == 0 && seg.first == cta)
+        pp.info[seg.unit] = seg.count > 1 ? make_int2(seg.unit + cta, seg.count) : make_int2(0, 0);
+    }
+    __syncthreads();
+    need_proxy_fence = true;
+    const int g = seg.g_end;
+    if (g >= g1 || timed_out) break;
+    seg = paged_segment_at<kTok>(pp, s_pref, dTC, g, g1);
+    if (seg.g_end < g1)  // the query slot just released takes the segment after the next
+      prefetch_q(seg_k & 1, paged_segment_at<kTok>(pp, s_pref, dTC, seg.g_end, g1));
+    ++seg_k;
+  }
+  if (timed_out && lane == 0) Policy::report_timeout();
+}
+
+// ---------------------------------------------------------------- merge of a unit's partials
+//     out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M),   M = max_s m_s
+// GROUPS groups of D/4 threads per row (sequence, query head): a warp or half of one where there are
+// many rows of few partials each, a whole CTA where few rows have many.
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams pp, int rows) {
+  constexpr int TPR = D / 4 * GROUPS, RPC = 256 / TPR;  // threads per row, rows per CTA
+  __shared__ float4 s_a[GROUPS > 1 ? 256 : 1];
+  __shared__ float s_x[GROUPS > 1 ? 256 : 1];
+  const DecodeParams& p = pp.d;
+  const int tid = threadIdx.x, sub = tid % TPR, row = blockIdx.x * RPC + tid / TPR;
+  const int g = sub / (D / 4), d = sub % (D / 4) * 4;
+  if (GROUPS > 1) pdl_launch_dependents();
+  pdl_wait();
+  int2 at = make_int2(0, 0);
+  int h = 0;
+  if (row < rows) {
+    const int b = row / p.HQ, hq = row - b * p.HQ, hkv = hq / p.group, hg = hq - hkv * p.group;
+    at = __ldcg(pp.info + b * pp.HKVc + hkv * p.hchunks + hg / kHeadsPerCta);
+    h = hg % kHeadsPerCta;
+  }
+  const int n = at.y;
+  const int64_t r0 = (int64_t)at.x * kHeadsPerCta + h;
+  float M = -INFINITY;
+  if constexpr (GROUPS == 1) {
+    for (int s = 0; s < n; ++s) M = fmaxf(M, __ldcg(pp.m + r0 + s * kHeadsPerCta));
+  } else {
+    for (int s = sub; s < n; s += TPR) M = fmaxf(M, __ldcg(pp.m + r0 + s * kHeadsPerCta));
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(kFullMask, M, off));
+    s_x[tid] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) M = fmaxf(M, s_x[tid / TPR * TPR + w * 32]);
+    __syncthreads();
+  }
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L = 0.f;
+#pragma unroll 4
+  for (int s = g; s < n; s += GROUPS) {
+    const int64_t r = r0 + s * kHeadsPerCta;
+    const float m = __ldcg(pp.m + r), l = __ldcg(pp.l + r);
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(pp.acc + r * D + d));
+    const float w = m > -INFINITY ? ex2(m - M) : 0.f;  // a partial without tokens is zero
+    a.x = fmaf(w, x.x, a.x);
+    a.y = fmaf(w, x.y, a.y);
+    a.z = fmaf(w, x.z, a.z);
+    a.w = fmaf(w, x.w, a.w);
+    L = fmaf(w, l, L);
+  }
+  if constexpr (GROUPS > 1) {
+    s_a[tid] = a;
+    s_x[tid] = L;
+    __syncthreads();
+    if (g == 0) {
+#pragma unroll
+      for (int k = 1; k < GROUPS; ++k) {
+        const float4 x = s_a[tid + k * (D / 4)];
+        a.x += x.x;
+        a.y += x.y;
+        a.z += x.z;
+        a.w += x.w;
+        L += s_x[tid + k * (D / 4)];
+      }
+    }
+  }
+  if (n > 0 && g == 0) {
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    store_out4(pp.out, pp.out_dtype, (int64_t)row * D + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+  }
+  if (GROUPS == 1) pdl_launch_dependents();  // the balanced kernel of the next step wants its SMs free
+}
+
+// ------------------------------------------------------------------ host side
+struct PagedCall {  // one call, before it is cut into launches
+  PagedParams pp;
+  int B;
+  void* workspace;
+  int64_t workspace_bytes;
+};
+
+template <class Policy>
+struct PagedLaunch {
+  static int smem_bytes(int B) {
+    return Policy::WARPS * Policy::STAGES * Policy::STAGE_BYTES + Policy::WARPS * Policy::STAGES * 8 + 16 +
+           2 * kHeadsPerCta * Policy::D * 4 + ((Policy::QFRAG_BYTES + 15) & ~15) + (B + 1) * 4 +
+           1024;  // slack for the 1024-byte alignment of the ring
+  }
+  // CTAs resident at once with the largest prefix
+  static int wave(int* out) {
+    static int cached[64] = {};
+    int dev = 0;
+    TKV_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && cached[dev] > 0) {
+      *out = cached[dev];
+      return TKV_OK;
+    }
+    const void* fn = reinterpret_cast<const void*>(&paged_split_kernel<Policy>);
+    int n = 0, sms = 0;
+    TKV_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kMaxPagedB)));
+    TKV_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, Policy::WARPS * 32, smem_bytes(kMaxPagedB)));
+    TKV_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    TKV_REQUIRE(n > 0 && sms > 0, TKV_ERR_CUDA, "paged split kernel does not fit on this device");
+    *out = n * sms;
+    if (dev < 64) cached[dev] = *out;
+    return TKV_OK;
+  }
+  // partials, then (m, l), then the units' notes
+  static int bytes(int B, int HKVc, int64_t* out) {
+    int w = 0;
+    const int rc = wave(&w);
+    if (rc != TKV_OK) return rc;
+    const int64_t units = (int64_t)(B < kMaxPagedB ? B : kMaxPagedB) * HKVc;
+    *out = (units + w) * kHeadsPerCta * (Policy::D + 2) * 4 + units * 8;
+    return TKV_OK;
+  }
+  static int run(const typename Policy::Maps& maps, const PagedCall& c, cudaStream_t stream) {
+    int w = 0;
+    int64_t need = 0;
+    int rc = wave(&w);
+    if (rc == TKV_OK) rc = bytes(c.B, c.pp.HKVc, &need);
+    if (rc != TKV_OK) return rc;
+    TKV_REQUIRE(c.workspace && c.workspace_bytes >= need, TKV_ERR_INVALID,
+                "paged decode: a workspace of %lld bytes is needed, got %lld; size it with tkv_paged_workspace",
+                (long long)need, (long long)c.workspace_bytes);
+    const int64_t tiles = ((int64_t)c.pp.d.S + Policy::TOK - 1) / Policy::TOK;  // of one sequence, at most
+    int64_t part = kMaxPagedB;  // sequences of a launch: tile numbers fit the prefix words and 30 bits
+    if (part * tiles >= (1 << 25)) part = ((1 << 25) - 1) / tiles;
+    if (part * tiles * c.pp.HKVc >= (1 << 30)) part = ((1 << 30) - 1) / (tiles * c.pp.HKVc);
+    TKV_REQUIRE(part >= 1, TKV_ERR_INVALID, "paged decode: %lld tiles of %d head units per sequence are too many",
+                (long long)tiles, c.pp.HKVc);
+    const int64_t units = (int64_t)(c.B < kMaxPagedB ? c.B : kMaxPagedB) * c.pp.HKVc, slots = units + w;
+    for (int b0 = 0; b0 < c.B; b0 += (int)part) {
+      PagedParams pp = c.pp;
+      const int n = c.B - b0 < part ? c.B - b0 : (int)part;
+      const int64_t rows0 = (int64_t)b0 * pp.d.HQ * Policy::D;
+      pp.d.B = n;
+      pp.d.q = (const uint8_t*)pp.d.q + rows0 * (pp.d.q_dtype == TKV_DTYPE_F32 ? 4 : 2);
+      pp.out = (uint8_t*)pp.out + rows0 * (pp.out_dtype == TKV_DTYPE_F32 ? 4 : 2);
+      pp.d.seq_lens += b0;
+      pp.table += b0 * pp.table_stride;
+      pp.acc = (float*)c.workspace;
+      pp.m = pp.acc + slots * kHeadsPerCta * Policy::D;
+      pp.l = pp.m + slots * kHeadsPerCta;
+      pp.info = (int2*)(pp.l + slots * kHeadsPerCta);
+      TKV_CUDA(launch_pdl(paged_split_kernel<Policy>, dim3(w), dim3(Policy::WARPS * 32), (size_t)smem_bytes(n), stream,
+                          maps, pp));
+      const int rows = n * pp.d.HQ;
+      if (rows < kSmallCombineMinRows) {
+        constexpr int GROUPS = 256 / (Policy::D / 4);
+        TKV_CUDA(launch_pdl(paged_merge_kernel<Policy::D, GROUPS>, dim3(rows), dim3(256), 0, stream, pp, rows));
+      } else {
+        constexpr int RPC = 256 / (Policy::D / 4);
+        TKV_CUDA(launch_pdl(paged_merge_kernel<Policy::D, 1>, dim3((rows + RPC - 1) / RPC), dim3(256), 0, stream, pp,
+                            rows));
+      }
+    }
+    return TKV_OK;
+  }
+};
+
+template <class P>
+static int packed_run(const PagedCall& c, cudaStream_t stream) {
+  using C = typename P::C;
+  typename P::Maps maps;
+  const DecodeParams& p = c.pp.d;
+  // pool rows as 128-byte rows, a box is one piece of a tile
+  const int64_t rows = (int64_t)c.pp.num_pages * p.HKV * c.pp.page * C::DP / 128;
+  constexpr int box = P::PIECE_BYTES / 128;
+  int rc;
+  if (p.kv_one) {
+    const uint8_t *lo = p.k_second ? p.vp : p.kp, *hi = p.k_second ? p.kp : p.vp;
+    rc = make_pair_map(&maps.k, lo, (uint64_t)(hi - lo), rows, box);
+    maps.v = maps.k;
+  } else {
+    rc = make_row_map(&maps.k, p.kp, rows, 128, 128, box);
+    if (rc == TKV_OK) rc = make_row_map(&maps.v, p.vp, rows, 128, 128, box);
+  }
+  if (rc != TKV_OK) return rc;
+  return PagedLaunch<P>::run(maps, c, stream);
+}
+
+template <class P>
+static int f16_run(const PagedCall& c, cudaStream_t stream) {
+  typename P::Maps maps;
+  maps.unused = 0;
+  return PagedLaunch<P>::run(maps, c, stream);
+}
+
+template <int NB, int DD, int GG, int PIECES>
+using PagedPolicy = FusedPolicy<NB, DD, GG, true, 32, 4, 3, 3, true, false, PIECES>;
+
+#define TKV_PAGED_ONE(NB, DD, GG, EXPR)                        \
+  if (nbits == NB && D == DD && gs == GG) {                    \
+    if (page % 32 == 0) {                                      \
+      using P = PagedPolicy<NB, DD, GG, 1>;                    \
+      return EXPR;                                             \
+    }                                                          \
+    using P = PagedPolicy<NB, DD, GG, 2>;                      \
+    return EXPR;                                               \
+  }
+#define TKV_PAGED_ALL(EXPR)          \
+  TKV_PAGED_ONE(4, 128, 16, EXPR)    \
+  TKV_PAGED_ONE(4, 128, 32, EXPR)    \
+  TKV_PAGED_ONE(4, 128, 64, EXPR)    \
+  TKV_PAGED_ONE(4, 128, 128, EXPR)   \
+  TKV_PAGED_ONE(2, 128, 16, EXPR)    \
+  TKV_PAGED_ONE(2, 128, 32, EXPR)    \
+  TKV_PAGED_ONE(2, 128, 64, EXPR)    \
+  TKV_PAGED_ONE(2, 128, 128, EXPR)   \
+  TKV_PAGED_ONE(4, 64, 16, EXPR)     \
+  TKV_PAGED_ONE(4, 64, 32, EXPR)     \
+  TKV_PAGED_ONE(4, 64, 64, EXPR)     \
+  TKV_PAGED_ONE(2, 64, 16, EXPR)     \
+  TKV_PAGED_ONE(2, 64, 32, EXPR)     \
+  TKV_PAGED_ONE(2, 64, 64, EXPR)
+
+static int packed_unsupported(int nbits, int D, int gs) {
+  set_error("paged decode: unsupported (nbits=%d, head_dim=%d, group_size=%d); built: nbits in {2,4}, head_dim in "
+            "{64,128}, group_size in {16,32,64,128} with group_size <= head_dim", nbits, D, gs);
+  return TKV_ERR_UNSUPPORTED;
+}
+
+int paged_device_status(int* status) {
+  int a = 0, b = 0;
+  TKV_CUDA(cudaMemcpyFromSymbol(&a, g_fused_status, sizeof(int)));
+  TKV_CUDA(cudaMemcpyFromSymbol(&b, g_fp16_status, sizeof(int)));
+  *status = a | b;
+  return TKV_OK;
+}
+
+int paged_device_status_clear() {
+  const int zero = 0;
+  TKV_CUDA(cudaMemcpyToSymbol(g_fused_status, &zero, sizeof(int)));
+  TKV_CUDA(cudaMemcpyToSymbol(g_fp16_status, &zero, sizeof(int)));
+  return TKV_OK;
+}
+
+// Checks shared by the two entry points; fills everything but the pools.
+static int paged_fill(const char* who, PagedCall& c, const void* q, int q_dtype, const int32_t* table,
+                      int64_t table_stride, const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
+                      int64_t workspace_bytes, int B, int HQ, int HKV, int num_pages, int page, int max_pages, int D,
+                      float sm_scale) {
+  TKV_REQUIRE(B > 0 && HQ > 0 && HKV > 0 && HQ % HKV == 0, TKV_ERR_INVALID,
+              "%s: bad sizes B=%d HQ=%d HKV=%d (HQ must be a multiple of HKV)", who, B, HQ, HKV);
+  TKV_REQUIRE(num_pages > 0 && page > 0 && max_pages >= 0, TKV_ERR_INVALID,
+              "%s: bad sizes num_pages=%d page_size=%d max_pages=%d", who, num_pages, page, max_pages);
+  TKV_REQUIRE(page % 16 == 0, TKV_ERR_UNSUPPORTED, "%s: unsupported page_size=%d (a multiple of 16 tokens)", who, page);
+  TKV_REQUIRE((int64_t)num_pages * HKV * page < (1LL << 31), TKV_ERR_INVALID,
+              "%s: a pool of %lld token rows exceeds 2^31", who, (long long)num_pages * HKV * page);
+  TKV_REQUIRE((int64_t)max_pages * page < (1LL << 30), TKV_ERR_INVALID,
+              "%s: a table row of %lld tokens exceeds 2^30", who, (long long)max_pages * page);
+  TKV_REQUIRE((int64_t)kMaxPagedB * HQ < (1LL << 31), TKV_ERR_INVALID, "%s: HQ=%d is too large", who, HQ);
+  TKV_REQUIRE(q_dtype >= 0 && q_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, TKV_ERR_INVALID,
+              "%s: bad dtype codes %d, %d", who, q_dtype, out_dtype);
+  TKV_REQUIRE(q && seq_lens && out && (table || max_pages == 0), TKV_ERR_INVALID, "%s: null pointer", who);
+  TKV_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace), TKV_ERR_ALIGN,
+              "%s: q, out and the workspace must be 16-byte aligned", who);
+  c = PagedCall{};
+  c.B = B;
+  c.workspace = workspace;
+  c.workspace_bytes = workspace_bytes;
+  PagedParams& pp = c.pp;
+  DecodeParams& p = pp.d;
+  p.q = q;
+  p.q_dtype = q_dtype;
+  p.seq_lens = seq_lens;
+  p.HQ = HQ;
+  p.HKV = HKV;
+  p.S = max_pages * page;
+  p.group = HQ / HKV;
+  p.hchunks = (p.group + kHeadsPerCta - 1) / kHeadsPerCta;
+  p.qk_scale = sm_scale * kLog2e;
+  p.meta_aligned = 16;
+  p.wide = 1;
+  pp.table = table;
+  pp.table_stride = table_stride;
+  pp.out = out;
+  pp.out_dtype = out_dtype;
+  pp.num_pages = num_pages;
+  pp.page = page;
+  pp.max_pages = max_pages;
+  pp.HKVc = HKV * p.hchunks;
+  pp.dpage = make_fastdiv(page);
+  pp.dHch = make_fastdiv(p.hchunks);
+  pp.dHKVc = make_fastdiv(pp.HKVc);
   return TKV_OK;
 }
 
 }  // namespace tkv
 
+extern "C" int tkv_paged_workspace(int B, int HQ, int HKV, int page_size, int D, int nbits, int gs, int64_t* bytes) {
+  using namespace tkv;
+  TKV_REQUIRE(bytes && B > 0 && HQ > 0 && HKV > 0 && HQ % HKV == 0 && page_size > 0, TKV_ERR_INVALID,
+              "paged_workspace: bad sizes B=%d HQ=%d HKV=%d page_size=%d", B, HQ, HKV, page_size);
+  const int page = page_size, HKVc = HKV * ((HQ / HKV + kHeadsPerCta - 1) / kHeadsPerCta);
+  if (nbits == 16) {
+    if (D == 128) return PagedLaunch<Fp16Policy<128>>::bytes(B, HKVc, bytes);
+    if (D == 64) return PagedLaunch<Fp16Policy<64>>::bytes(B, HKVc, bytes);
+    set_error("paged fp16 decode: unsupported head_dim=%d (built: 64, 128)", D);
+    return TKV_ERR_UNSUPPORTED;
+  }
+  TKV_PAGED_ALL(PagedLaunch<P>::bytes(B, HKVc, bytes))
+  return packed_unsupported(nbits, D, gs);
+}
+
 extern "C" int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_packed, const void* k_scale,
                                 const void* k_zero, const uint8_t* v_packed, const void* v_scale,
                                 const void* v_zero, const int32_t* block_table, int64_t table_stride,
-                                const int32_t* seq_lens, void* out, int out_dtype, int B, int HQ, int HKV,
-                                int num_pages, int page_size, int max_pages, int D, int nbits, int gs,
-                                float sm_scale, void* stream) {
+                                const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
+                                int64_t workspace_bytes, int B, int HQ, int HKV, int num_pages, int page_size,
+                                int max_pages, int D, int nbits, int gs, float sm_scale, void* stream) {
   using namespace tkv;
-  const PagedArgs a{q, k_packed, v_packed, (const __half*)k_scale, (const __half*)k_zero, (const __half*)v_scale,
-                    (const __half*)v_zero, block_table, seq_lens, out, table_stride, q_dtype, out_dtype, B, HQ,
-                    HKV, D, num_pages, page_size, max_pages, gs, sm_scale * kLog2e};
-  TKV_REQUIRE(k_scale && k_zero && v_scale && v_zero, TKV_ERR_INVALID, "paged decode: null pointer");
   TKV_REQUIRE(nbits == 2 || nbits == 4, TKV_ERR_INVALID, "nbits must be one of (2, 4), got %d", nbits);
-  const int rc = paged_check("paged decode", a, nbits);
+  PagedCall c;
+  const int rc = paged_fill("paged decode", c, q, q_dtype, block_table, table_stride, seq_lens, out, out_dtype,
+                            workspace, workspace_bytes, B, HQ, HKV, num_pages, page_size, max_pages, D, sm_scale);
   if (rc != TKV_OK) return rc;
-  if (nbits == 4)
-    paged_attention_kernel<4><<<B * HQ, kTokens, 0, (cudaStream_t)stream>>>(a);
-  else
-    paged_attention_kernel<2><<<B * HQ, kTokens, 0, (cudaStream_t)stream>>>(a);
-  TKV_CUDA(cudaGetLastError());
-  return TKV_OK;
+  TKV_REQUIRE(k_packed && k_scale && k_zero && v_packed && v_scale && v_zero, TKV_ERR_INVALID, "paged decode: null pointer");
+  TKV_REQUIRE(aligned16(k_packed) && aligned16(v_packed) && aligned16(k_scale) && aligned16(k_zero) &&
+                  aligned16(v_scale) && aligned16(v_zero), TKV_ERR_ALIGN, "paged decode: the pools must be 16-byte aligned");
+  DecodeParams& p = c.pp.d;
+  p.kp = k_packed;
+  p.vp = v_packed;
+  p.ks = (const __half*)k_scale;
+  p.kz = (const __half*)k_zero;
+  p.vs = (const __half*)v_scale;
+  p.vz = (const __half*)v_zero;
+  const int page = page_size;
+  {
+    // one tensor map over both code pools, where a K and a V run land side by side in whole swizzle
+    // atoms (or the stage is laid out for it: two pieces)
+    const uint8_t *lo = k_packed < v_packed ? k_packed : v_packed, *hi = k_packed < v_packed ? v_packed : k_packed;
+    const uint64_t gap = (uint64_t)(hi - lo);
+    const int64_t pool = (int64_t)num_pages * HKV * page * (D * nbits / 8);
+    p.kv_one = (page % 32 != 0 || (32 * (D * nbits / 8)) % 1024 == 0) && gap % 16 == 0 && gap < (1ull << 40) &&
+               gap >= (uint64_t)pool;
+    p.k_second = p.kv_one && k_packed > v_packed;
+  }
+  TKV_PAGED_ALL(packed_run<P>(c, (cudaStream_t)stream))
+  return packed_unsupported(nbits, D, gs);
 }
 
 extern "C" int tkv_paged_fp16_decode(const void* q, int q_dtype, const void* k, const void* v,
                                      const int32_t* block_table, int64_t table_stride,
-                                     const int32_t* seq_lens, void* out, int out_dtype, int B, int HQ, int HKV,
-                                     int num_pages, int page_size, int max_pages, int D, float sm_scale,
-                                     void* stream) {
+                                     const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
+                                     int64_t workspace_bytes, int B, int HQ, int HKV, int num_pages, int page_size,
+                                     int max_pages, int D, float sm_scale, void* stream) {
   using namespace tkv;
-  const PagedArgs a{q, (const uint8_t*)k, (const uint8_t*)v, nullptr, nullptr, nullptr, nullptr, block_table,
-                    seq_lens, out, table_stride, q_dtype, out_dtype, B, HQ, HKV, D, num_pages, page_size,
-                    max_pages, 0, sm_scale * kLog2e};
-  const int rc = paged_check("paged fp16 decode", a, 16);
+  PagedCall c;
+  const int rc = paged_fill("paged fp16 decode", c, q, q_dtype, block_table, table_stride, seq_lens, out, out_dtype,
+                            workspace, workspace_bytes, B, HQ, HKV, num_pages, page_size, max_pages, D, sm_scale);
   if (rc != TKV_OK) return rc;
-  paged_attention_kernel<16><<<B * HQ, kTokens, 0, (cudaStream_t)stream>>>(a);
-  TKV_CUDA(cudaGetLastError());
-  return TKV_OK;
+  TKV_REQUIRE(k && v, TKV_ERR_INVALID, "paged fp16 decode: null pointer");
+  TKV_REQUIRE(aligned16(k) && aligned16(v), TKV_ERR_ALIGN, "paged fp16 decode: the pools must be 16-byte aligned");
+  c.pp.d.k = (const __half*)k;
+  c.pp.d.v = (const __half*)v;
+  if (D == 128) return f16_run<Fp16Policy<128>>(c, (cudaStream_t)stream);
+  if (D == 64) return f16_run<Fp16Policy<64>>(c, (cudaStream_t)stream);
+  set_error("paged fp16 decode: unsupported head_dim=%d (built: 64, 128)", D);
+  return TKV_ERR_UNSUPPORTED;
 }

@@ -63,7 +63,8 @@ def paged_decode_attention(
     first ``seq_lens[b]`` tokens (clamped to the table's), without those whose table entry names no
     page; with none left its output is zero.  Returns ``(B, HQ, D)`` float32, or ``out``, which may
     also be float16 or bfloat16 (rounded once, at the end).  With ``out`` and ``_workspace`` (a dict
-    that the caller keeps; one for each stream or captured graph that may run at the same time)
+    that the caller keeps, as long as a graph that was captured with it; one for each stream or
+    graph that may run at the same time)
     supplied, the call allocates nothing after its first use and can be captured."""
     if not isinstance(kq, QuantizedTensor) or not isinstance(vq, QuantizedTensor):
         raise TypeError("paged_decode_attention reads packed pools (QuantizedTensor); see paged_fp16_decode_attention")
@@ -76,10 +77,11 @@ def paged_decode_attention(
         return out
     dev = q.device
     with _cabi.on_device(dev):
+        ws = _cabi.paged_workspace(_workspace, B, HQ, HKV, page, D, kq.nbits, kq.group_size, dev)
         _cabi.check(lib.tkv_paged_decode(
             q.data_ptr(), _cabi.dtype_code(q), kt[0].data_ptr(), kt[1].data_ptr(), kt[2].data_ptr(), vt[0].data_ptr(),
             vt[1].data_ptr(), vt[2].data_ptr(), block_table.data_ptr(), stride, seq_lens.data_ptr(), out.data_ptr(),
-            _cabi.dtype_code(out), B, HQ, HKV, NP, page, W, D, kq.nbits, kq.group_size,
+            _cabi.dtype_code(out), ws.data_ptr(), ws.numel(), B, HQ, HKV, NP, page, W, D, kq.nbits, kq.group_size,
             1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _cabi.stream_ptr(dev)))
     return out
 
@@ -105,8 +107,9 @@ def paged_fp16_decode_attention(
         return out
     dev = q.device
     with _cabi.on_device(dev):
+        ws = _cabi.paged_workspace(_workspace, B, HQ, HKV, page, D, 16, 0, dev)
         _cabi.check(lib.tkv_paged_fp16_decode(
             q.data_ptr(), _cabi.dtype_code(q), kt[0].data_ptr(), vt[0].data_ptr(), block_table.data_ptr(), stride,
-            seq_lens.data_ptr(), out.data_ptr(), _cabi.dtype_code(out), B, HQ, HKV, NP, page, W, D,
+            seq_lens.data_ptr(), out.data_ptr(), _cabi.dtype_code(out), ws.data_ptr(), ws.numel(), B, HQ, HKV, NP, page, W, D,
             1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _cabi.stream_ptr(dev)))
     return out
