@@ -5,12 +5,20 @@
 // the table and table entries outside the pool drop the token.  Per group of gs dims
 //     scale = f16((max - min) / (2^nbits - 1))  (1 if that is not positive),   zero = f16(min),
 //     code  = clamp(rint((x - zero) / scale), 0, 2^nbits - 1),
-// the arithmetic of tkv_quantize_pack, so the bytes are the same.  Every float operation is one
-// IEEE operation written with an intrinsic.  With a values tensor the token's code*scale + zero
-// goes there too: what the cache now stands for, as a prompt's own attention needs it.
-#include <type_traits>
-
-#include "tkv_common.cuh"
+// with the arithmetic of tkv_quantize_pack (tkv_quant_part.cuh), so the bytes are the same.  With a
+// values tensor the token's code*scale + zero goes there too: what the cache now stands for, as a
+// prompt's own attention needs it.
+//
+// K and V go in one launch.  A thread owns E = 16 (8) consecutive elements of a row, in one row of a step and
+// four of a prompt.
+// Two ways to cut the rows (BLOCK):
+//   * prompts: a CTA takes a block of tokens of one head of one sequence, so that where it stands
+//     is known from its indexes alone and the codes and metadata it writes are consecutive;
+//   * a step (T of at most kStepTokens): a CTA takes rows of several heads and sequences.
+// The row's place (two dependent loads: position, then table entry) is looked up beside the element
+// loads and needed only by the stores.
+#include "tkv_quant_part.cuh"
+#include "tkv_splitk_driver.cuh"  // FastDiv
 
 namespace tkv {
 
@@ -26,95 +34,195 @@ struct AppendArgs {
   AppendTensor t[2];                // K, V
   const int32_t *table, *positions, *lengths;
   int64_t table_stride;
-  int pos0, B, HKV, T, D, gs, num_pages, page, max_pages;
+  int pos0, B, HKV, T, num_pages, page;
+  int limit;                        // tokens that a row of the table has room for
+  FastDiv dpage, dT, dHKV;
 };
 
+constexpr int kStepTokens = 8;
+constexpr int kRowsBlock = 4, kRowsStep = 1;  // rows of a thread
+
+__device__ __forceinline__ float elem_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float elem_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half*) { return pack_half2(a, b); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 8 consecutive values, 16 or 32 bytes
 template <typename T>
-__device__ __forceinline__ float to_f32(T x) {
-  if constexpr (sizeof(T) == 4) return x;
-  else return static_cast<float>(x);
-}
-__device__ __forceinline__ void from_f32(float* d, float x) { *d = x; }
-__device__ __forceinline__ void from_f32(__half* d, float x) { *d = __float2half_rn(x); }
-__device__ __forceinline__ void from_f32(__nv_bfloat16* d, float x) { *d = __float2bfloat16_rn(x); }
-
-// The pool row of token t of (sequence b, head h), or -1.
-__device__ __forceinline__ int64_t append_row(const AppendArgs& a, int b, int h, int t) {
-  if (a.lengths && t >= a.lengths[b]) return -1;
-  const int64_t pos = (a.positions ? (int64_t)a.positions[b] : (int64_t)a.pos0) + t;
-  if (pos < 0 || pos >= (int64_t)a.max_pages * a.page) return -1;
-  const int i = (int)(pos / a.page), id = a.table[b * a.table_stride + i];
-  if (id < 0 || id >= a.num_pages) return -1;
-  return ((int64_t)id * a.HKV + h) * a.page + (pos - (int64_t)i * a.page);
-}
-
-// One CTA of D threads per row; NBITS == 16 copies into float16 pages.
-template <typename T, int NBITS>
-__global__ void paged_append_kernel(const AppendArgs a) {
-  __shared__ float s_x[256];
-  __shared__ uint8_t s_code[256];
-  const int d = threadIdx.x, D = a.D;
-  const AppendTensor& w = a.t[blockIdx.y];
-  const int64_t r = blockIdx.x;
-  const int t = (int)(r % a.T), h = (int)(r / a.T % a.HKV), b = (int)(r / a.T / a.HKV);
-  const int64_t row = append_row(a, b, h, t);
-  if (row < 0) return;
-  const T raw = reinterpret_cast<const T*>(w.x)[b * w.sb + h * w.sh + t * w.st + d];
-  const float x = to_f32(raw);
-  float value;
-  if constexpr (NBITS == 16) {
-    __half y;
-    if constexpr (std::is_same<T, __half>::value) y = raw;  // as stored, whatever a NaN holds
-    else y = __float2half_rn(x);
-    reinterpret_cast<__half*>(w.packed)[row * D + d] = y;
-    value = __half2float(y);
+__device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
+  if constexpr (std::is_same<T, float>::value) {
+    reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
   } else {
-    constexpr float QMAX = float((1 << NBITS) - 1);
-    s_x[d] = x;
-    __syncthreads();
-    const int g0 = d / a.gs * a.gs;
-    float lo = s_x[g0], hi = lo;
-    for (int i = 1; i < a.gs; ++i) {  // a NaN stays, as it does in tkv_quantize_pack
-      const float y = s_x[g0 + i];
-      lo = (y < lo || y != y) ? y : lo;
-      hi = (y > hi || y != y) ? y : hi;
-    }
-    float s = __fdiv_rn(__fsub_rn(hi, lo), QMAX);
-    s = s > 0.f ? s : 1.f;
-    const __half s16 = __float2half_rn(s), z16 = __float2half_rn(lo);
-    const float sf = __half2float(s16), zf = __half2float(z16);
-    float c = rintf(__fdiv_rn(__fsub_rn(x, zf), sf));
-    c = fminf(fmaxf(c, 0.f), QMAX);
-    s_code[d] = (uint8_t)c;
-    if (d == g0) {
-      const int64_t g = row * (D / a.gs) + d / a.gs;
-      w.scale[g] = s16;
-      w.zero[g] = z16;
-    }
-    __syncthreads();
-    constexpr int P = 8 / NBITS;
-    const int DP = D / P;
-    if (d < DP) {
-      uint32_t byte = 0;
-      for (int p = 0; p < P; ++p) byte |= (uint32_t)s_code[d + p * DP] << (NBITS * p);
-      w.packed[row * DP + d] = (uint8_t)byte;
-    }
-    value = __fadd_rn(__fmul_rn(c, sf), zf);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack2(v[0], v[1], dst), pack2(v[2], v[3], dst),
+                                                pack2(v[4], v[5], dst), pack2(v[6], v[7], dst));
   }
-  if (w.values) from_f32(reinterpret_cast<T*>(w.values) + b * w.vb + h * w.vh + t * w.vt + d, value);
+}
+
+// The token of a row of the work.  A row that is not there names the nearest one that is, so that
+// a whole warp can load and shuffle.
+struct AppendRow {
+  int b, h, t;
+  bool live;
+};
+template <bool BLOCK>
+__device__ __forceinline__ AppendRow append_row(const AppendArgs& a, int rows_per_cta, int i) {
+  AppendRow w;
+  if constexpr (BLOCK) {
+    const int t = blockIdx.x * rows_per_cta + i;
+    w.b = blockIdx.z;
+    w.h = blockIdx.y >> 1;
+    w.live = t < a.T;
+    w.t = min(t, a.T - 1);
+  } else {
+    const int r = blockIdx.x * rows_per_cta + i, q = fast_div(r, a.dT), b = fast_div(q, a.dHKV);
+    w.live = b < a.B;
+    w.b = min(b, a.B - 1);
+    w.h = q - b * a.HKV;
+    w.t = r - q * a.T;
+  }
+  return w;
+}
+// Its pool row, or -1: nowhere.
+__device__ __forceinline__ int append_place(const AppendArgs& a, const AppendRow& w) {
+  const int len = a.lengths ? __ldg(a.lengths + w.b) : a.T;
+  const int64_t pos = (int64_t)(a.positions ? __ldg(a.positions + w.b) : a.pos0) + w.t;
+  if (!w.live || w.t >= len || (uint64_t)pos >= (uint32_t)a.limit) return -1;
+  const int k = fast_div((int)pos, a.dpage), id = __ldg(a.table + w.b * a.table_stride + k);
+  return (unsigned)id < (unsigned)a.num_pages ? (id * a.HKV + w.h) * a.page + ((int)pos - k * a.page) : -1;
+}
+
+// `tpr_shift` = log2(D/E) (threads of a row), `lpg_shift` = log2(gs/E) (lanes of a group).
+template <typename T, int NBITS, int E, bool BLOCK>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int tpr_shift, int lpg_shift) {
+  constexpr int LOG2P = NBITS == 4 ? 1 : 2, ROWS = BLOCK ? kRowsBlock : kRowsStep;
+  const AppendTensor& w = a.t[blockIdx.y & 1];
+  const int tpr = 1 << tpr_shift, c = threadIdx.x & (tpr - 1), rstep = 256 >> tpr_shift;
+  const int tps_shift = tpr_shift - LOG2P, p = c >> tps_shift, D = E << tpr_shift;
+  if (BLOCK && a.lengths && (int)blockIdx.x * ROWS * rstep >= __ldg(a.lengths + blockIdx.z)) return;  // padding
+  const AppendRow row0 = append_row<BLOCK>(a, ROWS * rstep, threadIdx.x >> tpr_shift);
+  const T* src0 = reinterpret_cast<const T*>(w.x) + row0.b * w.sb + row0.h * w.sh + E * c;
+  T* val0 = reinterpret_cast<T*>(w.values) + row0.b * w.vb + row0.h * w.vh + E * c;
+#pragma unroll
+  for (int it = 0; it < ROWS; ++it) {
+    AppendRow row = row0;
+    if (BLOCK && it > 0) row = append_row<BLOCK>(a, ROWS * rstep, it * rstep + (threadIdx.x >> tpr_shift));
+    const int at = append_place(a, row);
+    uint32_t code[E / 4];
+    __half sc16, ze16;
+    float m[E];
+    quantize_part<T, NBITS, E>(src0 + row.t * w.st, 1 << lpg_shift, code, sc16, ze16, m);
+    if (w.values && at >= 0) {
+      T* dst = val0 + row.t * w.vt;
+      const float s = __half2float(sc16), z = __half2float(ze16);
+#pragma unroll
+      for (int i = 0; i < E / 8; ++i) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(__fsub_rn(m[8 * i + k], kMagic), s, z);  // (the product is exact)
+        store8(dst + 8 * i, v);
+      }
+    }
+    pack_slices<NBITS, E>(code, p, tps_shift, tpr);
+    if (at >= 0) {
+      if (p == 0) {
+        uint8_t* dst = w.packed + (int64_t)at * (D >> LOG2P) + E * c;
+        if constexpr (E == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(code[0], code[1], code[2], code[3]);
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[1]);
+      }
+      if ((c & ((1 << lpg_shift) - 1)) == 0) {
+        const int64_t g = ((int64_t)at << (tpr_shift - lpg_shift)) + (c >> lpg_shift);
+        w.scale[g] = sc16;
+        w.zero[g] = ze16;
+      }
+    }
+  }
+}
+
+// Float16 pages: 8 elements of a thread; float16 rows are copied as stored, whatever a NaN holds.
+template <typename T, bool BLOCK>
+__global__ void __launch_bounds__(256) paged_append_f16_kernel(const AppendArgs a, int tpr_shift) {
+  constexpr int ROWS = BLOCK ? kRowsBlock : kRowsStep;
+  const AppendTensor& w = a.t[blockIdx.y & 1];
+  const int c = threadIdx.x & ((1 << tpr_shift) - 1), rstep = 256 >> tpr_shift, D = 8 << tpr_shift;
+#pragma unroll
+  for (int it = 0; it < ROWS; ++it) {
+    const AppendRow row = append_row<BLOCK>(a, ROWS * rstep, it * rstep + (threadIdx.x >> tpr_shift));
+    const int at = append_place(a, row);
+    if (at < 0) continue;
+    const T* src = reinterpret_cast<const T*>(w.x) + row.b * w.sb + row.h * w.sh + row.t * w.st + 8 * c;
+    uint4 y;
+    if constexpr (std::is_same<T, float>::value) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(src)), v = __ldg(reinterpret_cast<const float4*>(src) + 1);
+      y = make_uint4(pack_half2(u.x, u.y), pack_half2(u.z, u.w), pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+    } else {
+      y = __ldg(reinterpret_cast<const uint4*>(src));
+      if constexpr (!std::is_same<T, __half>::value) {
+        const T* e = reinterpret_cast<const T*>(&y);
+        const uint4 x = make_uint4(pack_half2(elem_f32(e[0]), elem_f32(e[1])), pack_half2(elem_f32(e[2]), elem_f32(e[3])),
+                                   pack_half2(elem_f32(e[4]), elem_f32(e[5])), pack_half2(elem_f32(e[6]), elem_f32(e[7])));
+        y = x;
+      }
+    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(w.packed) + (int64_t)at * D + 8 * c) = y;
+    if (w.values) {
+      T* dst = reinterpret_cast<T*>(w.values) + row.b * w.vb + row.h * w.vh + row.t * w.vt + 8 * c;
+      if constexpr (std::is_same<T, __half>::value) {
+        *reinterpret_cast<uint4*>(dst) = y;
+      } else {
+        const __half* e = reinterpret_cast<const __half*>(&y);
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = __half2float(e[k]);
+        store8(dst, v);
+      }
+    }
+  }
+}
+
+static inline bool is_pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
+static inline int log2i(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+template <typename T, bool BLOCK>
+static void launch_append_as(const AppendArgs& a, dim3 grid, int D, int nbits, int gs, bool wide, cudaStream_t stream) {
+  const int E = wide ? 16 : 8, tpr = log2i(D / E), lpg = nbits == 16 ? 0 : log2i(gs / E);
+  if (nbits == 16) {
+    paged_append_f16_kernel<T, BLOCK><<<grid, 256, 0, stream>>>(a, tpr);
+  } else if (wide) {
+    if constexpr (!std::is_same<T, float>::value) {
+      if (nbits == 4) paged_append_kernel<T, 4, 16, BLOCK><<<grid, 256, 0, stream>>>(a, tpr, lpg);
+      else paged_append_kernel<T, 2, 16, BLOCK><<<grid, 256, 0, stream>>>(a, tpr, lpg);
+    }
+  } else if (nbits == 4) {
+    paged_append_kernel<T, 4, 8, BLOCK><<<grid, 256, 0, stream>>>(a, tpr, lpg);
+  } else {
+    paged_append_kernel<T, 2, 8, BLOCK><<<grid, 256, 0, stream>>>(a, tpr, lpg);
+  }
 }
 
 template <typename T>
-static int launch_append(const AppendArgs& a, int nbits, int tensors, cudaStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)a.B * a.HKV * a.T), tensors);
-  if (nbits == 16) paged_append_kernel<T, 16><<<grid, a.D, 0, stream>>>(a);
-  else if (nbits == 4) paged_append_kernel<T, 4><<<grid, a.D, 0, stream>>>(a);
-  else paged_append_kernel<T, 2><<<grid, a.D, 0, stream>>>(a);
+static int launch_append(const AppendArgs& a, int D, int nbits, int gs, cudaStream_t stream) {
+  // 16 elements of a thread where a 16-bit row gives every bit slice and every group a whole thread
+  const bool wide = !std::is_same<T, float>::value && nbits != 16 && gs >= 16 && D / 16 >= 8 / nbits;
+  const int per_pass = 256 >> log2i(D / (wide ? 16 : 8));
+  // (65535: the limit of the grid's y and z)
+  if (a.T > kStepTokens && a.HKV <= 65535 / 2 && a.B <= 65535) {
+    const int per_cta = kRowsBlock * per_pass;
+    launch_append_as<T, true>(a, dim3((a.T + per_cta - 1) / per_cta, 2 * a.HKV, a.B), D, nbits, gs, wide, stream);
+  } else {
+    const int64_t rows = (int64_t)a.B * a.HKV * a.T, per_cta = kRowsStep * per_pass;
+    launch_append_as<T, false>(a, dim3((unsigned)((rows + per_cta - 1) / per_cta), 2), D, nbits, gs, wide, stream);
+  }
   TKV_CUDA(cudaGetLastError());
   return TKV_OK;
 }
-
-static inline bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
 
 }  // namespace tkv
 
@@ -132,10 +240,10 @@ extern "C" int tkv_paged_append(const void* k, const void* v, int in_dtype, cons
               "paged append: bad sizes B=%d HKV=%d T=%d num_pages=%d page_size=%d max_pages=%d", B, HKV, T,
               num_pages, page_size, max_pages);
   TKV_REQUIRE(in_dtype >= 0 && in_dtype <= 2, TKV_ERR_INVALID, "paged append: bad dtype %d", in_dtype);
-  TKV_REQUIRE(pow2(D) && D >= 16 && D <= 256, TKV_ERR_UNSUPPORTED,
+  TKV_REQUIRE(is_pow2(D) && D >= 16 && D <= 256, TKV_ERR_UNSUPPORTED,
               "paged append: unsupported head_dim=%d (a power of two from 16 to 256)", D);
   if (nbits != 16) {
-    TKV_REQUIRE(pow2(gs) && gs >= 8 && gs <= D, TKV_ERR_UNSUPPORTED,
+    TKV_REQUIRE(is_pow2(gs) && gs >= 8 && gs <= D, TKV_ERR_UNSUPPORTED,
                 "paged append: unsupported group_size=%d (a power of two from 8 to head_dim)", gs);
     TKV_REQUIRE((D * nbits / 8) % 8 == 0, TKV_ERR_UNSUPPORTED,
                 "paged append: packed row of %d bytes is not a multiple of 8", D * nbits / 8);
@@ -153,7 +261,12 @@ extern "C" int tkv_paged_append(const void* k, const void* v, int in_dtype, cons
                 TKV_ERR_ALIGN, "paged append: rows of the new tokens must start on 16-byte boundaries");
   TKV_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_packed) && aligned16(v_packed) && aligned16(k_values) &&
                   aligned16(v_values), TKV_ERR_ALIGN, "paged append: pointers must be 16-byte aligned");
-  TKV_REQUIRE((int64_t)B * HKV * T < (1LL << 31), TKV_ERR_INVALID, "paged append: B*HKV*T exceeds 2^31");
+  TKV_REQUIRE((int64_t)max_pages * page_size < (1LL << 30), TKV_ERR_INVALID,
+              "paged append: a table row of %lld tokens exceeds 2^30", (long long)max_pages * page_size);
+  TKV_REQUIRE((int64_t)B * HKV * T < (1LL << 31) - 4096, TKV_ERR_INVALID, "paged append: %lld token rows exceed 2^31",
+              (long long)B * HKV * T);
+  TKV_REQUIRE((int64_t)num_pages * HKV * page_size < (1LL << 31), TKV_ERR_INVALID,
+              "paged append: a pool of %lld token rows exceeds 2^31", (long long)num_pages * HKV * page_size);
   AppendArgs a{};
   a.t[0] = {k, k_packed, (__half*)k_scale, (__half*)k_zero, k_values, strides[0], strides[1], strides[2], 0, 0, 0};
   a.t[1] = {v, v_packed, (__half*)v_scale, (__half*)v_zero, v_values, strides[3], strides[4], strides[5], 0, 0, 0};
@@ -167,13 +280,14 @@ extern "C" int tkv_paged_append(const void* k, const void* v, int in_dtype, cons
   a.B = B;
   a.HKV = HKV;
   a.T = T;
-  a.D = D;
-  a.gs = nbits == 16 ? D : gs;
+  a.dpage = make_fastdiv(page_size);
+  a.dT = make_fastdiv(T);
+  a.dHKV = make_fastdiv(HKV);
   a.num_pages = num_pages;
   a.page = page_size;
-  a.max_pages = max_pages;
+  a.limit = max_pages * page_size;
   cudaStream_t s = (cudaStream_t)stream;
-  if (in_dtype == TKV_DTYPE_F16) return launch_append<__half>(a, nbits, 2, s);
-  if (in_dtype == TKV_DTYPE_BF16) return launch_append<__nv_bfloat16>(a, nbits, 2, s);
-  return launch_append<float>(a, nbits, 2, s);
+  if (in_dtype == TKV_DTYPE_F16) return launch_append<__half>(a, D, nbits, gs, s);
+  if (in_dtype == TKV_DTYPE_BF16) return launch_append<__nv_bfloat16>(a, D, nbits, gs, s);
+  return launch_append<float>(a, D, nbits, gs, s);
 }

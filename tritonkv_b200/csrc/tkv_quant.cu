@@ -6,87 +6,13 @@
 // every float operation below is a single IEEE round-to-nearest operation written
 // with an explicit intrinsic so that neither FMA contraction nor a fast-math flag
 // can change it.
-#include <type_traits>
-
-#include "tkv_common.cuh"
+#include "tkv_quant_part.cuh"
 
 namespace tkv {
 
 // ---------------------------------------------------------------- quantize + pack
-// Each thread owns E consecutive elements of a row (E = 16 for f16/bf16 rows: two 16-byte loads;
-// E = 8 otherwise), in kRowsPerThread rows.  A quantisation group spans GS/E adjacent lanes; min
-// and max are butterfly-reduced inside it as the pair (min, -max) with a NaN-propagating
-// minimum -- for 16-bit inputs as ONE packed half2 per shuffle.  The codes of a thread are E/4
-// 32-bit words (one code per byte); split-P packing ORs the words of the P lanes that hold
-// dims j, j+DP, ... shifted by their bit-slice position.  Every size is a power of two, so all
-// index arithmetic is shifts.
-//
-// Codes.  The reference computes round((x - zero) / scale) with an IEEE division.  Here the
-// quotient is a * (1/scale): within 1e-5 of the IEEE quotient wherever the clamp does not
-// decide the code (|q| <= 17), so it rounds to the same integer unless it lies within 1e-4 of
-// a half-integer -- those elements (about one in 1500 for f16 data, whose quotients hit exact
-// ties) are redone with the IEEE division.  Bit-exact, at a fifth of the instructions.
-// The scale's division by 2^nbits - 1 is q0 = d*R, q1 = fma(fma(-q0, QMAX, d), R, q0) with R the
-// rounded reciprocal: the correctly rounded quotient for every finite d (checked against the
-// IEEE division over 160 M values of d, all fp16 values among them).
+// The arithmetic of a thread's elements is in tkv_quant_part.cuh.
 constexpr int kRowsPerThread = 2;
-
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float d;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float rcp_approx(float a) {
-  float d;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(a));
-  return d;
-}
-
-// A thread's E elements as f32 plus their (min, -max); NaN propagates to both (torch's
-// amin/amax do; fminf/fmaxf would drop it).  For 16-bit types the pair stays a packed half2.
-template <typename T>
-struct Pair16;
-template <>
-struct Pair16<__half> { using type = __half2; };
-template <>
-struct Pair16<__nv_bfloat16> { using type = __nv_bfloat162; };
-
-template <typename H2>
-__device__ __forceinline__ float2 widen2(H2 h);
-template <>
-__device__ __forceinline__ float2 widen2<__half2>(__half2 h) { return __half22float2(h); }
-template <>
-__device__ __forceinline__ float2 widen2<__nv_bfloat162>(__nv_bfloat162 h) { return __bfloat1622float2(h); }
-
-// (min over both halves of a, -max over both halves of b) as one packed pair
-template <typename H2>
-__device__ __forceinline__ H2 fold_minmax(H2 a, H2 b) {
-  b = __hneg2(b);
-  const uint32_t au = *reinterpret_cast<const uint32_t*>(&a), bu = *reinterpret_cast<const uint32_t*>(&b);
-  const uint32_t lo = __byte_perm(au, bu, 0x5410), hi = __byte_perm(au, bu, 0x7632);  // (a.x, b.x), (a.y, b.y)
-  return __hmin2_nan(*reinterpret_cast<const H2*>(&lo), *reinterpret_cast<const H2*>(&hi));
-}
-
-// (x.lo - z, x.hi - z) in f32 from a packed pair of 16-bit values: the mixed-precision subtract of
-// sm_100 widens the 16-bit operand itself, so no conversion instruction is spent per element.
-template <typename H2>
-__device__ __forceinline__ float2 sub_widen(H2 x, float z);
-template <>
-__device__ __forceinline__ float2 sub_widen<__half2>(__half2 x, float z) {
-  float2 r;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %3;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "r"(*reinterpret_cast<const uint32_t*>(&x)), "f"(z));
-  return r;
-}
-template <>
-__device__ __forceinline__ float2 sub_widen<__nv_bfloat162>(__nv_bfloat162 x, float z) {
-  float2 r;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.bf16 %0, l, %3;\n\tsub.rn.f32.bf16 %1, h, %3;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "r"(*reinterpret_cast<const uint32_t*>(&x)), "f"(z));
-  return r;
-}
 
 // Where the rows go when new tokens are appended to a preallocated cache (cap == 0: in place).
 struct AppendMap {
@@ -106,10 +32,6 @@ __global__ void __launch_bounds__(256)
                          __half* __restrict__ scale, __half* __restrict__ zero, int64_t rows,
                          int tpr_shift, int lpg_shift, const AppendMap am) {
   constexpr int LOG2P = NBITS == 4 ? 1 : 2;  // P = 8 / NBITS codes per packed byte
-  constexpr float QMAX = float((1 << NBITS) - 1);
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: x + kMagic holds rint(x) in its low mantissa bits
-  constexpr bool k16 = !std::is_same<T, float>::value;
-  static_assert(E == 8 || (E == 16 && k16), "16 elements per thread are two 16-byte loads of a 16-bit type");
   const int tpr = 1 << tpr_shift;
   const int c = threadIdx.x & (tpr - 1);            // E-element column block
   const int rstep = 256 >> tpr_shift;               // rows of one pass of the block
@@ -124,116 +46,11 @@ __global__ void __launch_bounds__(256)
     const bool live = row < rows;
     // Lanes past the end mirror the last row so the shuffles below stay full-warp.
     const int64_t r = live ? row : rows - 1;
-    const T* src = x + r * D + E * c;
-    float a[E], mn, nmx;  // a: the elements (f32 rows) and then x - zero
-    [[maybe_unused]] uint32_t raw[k16 ? E / 2 : 1];  // 16-bit rows: the elements as loaded
-    if constexpr (k16) {
-      using H2 = typename Pair16<T>::type;
-      H2 h[E / 2];
-#pragma unroll
-      for (int i = 0; i < E / 8; ++i)
-        *reinterpret_cast<uint4*>(&h[4 * i]) = __ldg(reinterpret_cast<const uint4*>(src) + i);
-      H2 lo = h[0], hi = h[0];
-#pragma unroll
-      for (int i = 1; i < E / 2; ++i) {
-        lo = __hmin2_nan(lo, h[i]);
-        hi = __hmax2_nan(hi, h[i]);
-      }
-      H2 pm = fold_minmax<H2>(lo, hi);
-      for (int off = 1; off < lanes_per_group; off <<= 1) {
-        const uint32_t o = __shfl_xor_sync(kFullMask, *reinterpret_cast<const uint32_t*>(&pm), off);
-        pm = __hmin2_nan(pm, *reinterpret_cast<const H2*>(&o));
-      }
-      const float2 f = widen2<H2>(pm);
-      mn = f.x;
-      nmx = f.y;
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) raw[i] = *reinterpret_cast<const uint32_t*>(&h[i]);
-    } else {
-      const float4 lo4 = __ldg(reinterpret_cast<const float4*>(src));
-      const float4 hi4 = __ldg(reinterpret_cast<const float4*>(src) + 1);
-      a[0] = lo4.x; a[1] = lo4.y; a[2] = lo4.z; a[3] = lo4.w;
-      a[4] = hi4.x; a[5] = hi4.y; a[6] = hi4.z; a[7] = hi4.w;
-      mn = a[0];
-      nmx = -a[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) {
-        mn = min_nan(mn, a[i]);
-        nmx = min_nan(nmx, -a[i]);
-      }
-      for (int off = 1; off < lanes_per_group; off <<= 1) {
-        mn = min_nan(mn, __shfl_xor_sync(kFullMask, mn, off));
-        nmx = min_nan(nmx, __shfl_xor_sync(kFullMask, nmx, off));
-      }
-    }
-    // A group that holds a NaN gets zero = NaN, scale = 1 and all codes 0, as the reference produces.
-    const float range = __fsub_rn(-nmx, mn);
-    const float q0 = __fmul_rn(range, 1.f / QMAX);
-    const float q1 = __fmaf_rn(__fmaf_rn(-q0, QMAX, range), 1.f / QMAX, q0);
-    float sc = range == INFINITY ? range : q1;  // = __fdiv_rn(range, QMAX)
-    sc = (sc > 0.f) ? sc : 1.f;
-    const __half sc16 = __float2half_rn(sc);
-    const __half ze16 = __float2half_rn(mn);
-    const float scf = __half2float(sc16), zef = __half2float(ze16);
-    const float rs = __fmul_rn(rcp_approx(scf), 1.f / QMAX);  // a * rs = quotient / QMAX, saturated to [0, 1]
-
-    if constexpr (k16) {
-      using H2 = typename Pair16<T>::type;
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const float2 d = sub_widen<H2>(*reinterpret_cast<const H2*>(&raw[i]), zef);
-        a[2 * i] = d.x;
-        a[2 * i + 1] = d.y;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) a[i] = __fsub_rn(a[i], zef);
-    }
+    uint32_t w[E / 4];
+    __half sc16, ze16;
     float m[E];
-    uint32_t near_tie = 0;  // bit i: element i lies next to a tie
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float u = __saturatef(__fmul_rn(a[i], rs));                  // NaN -> 0, as the clamp gives
-      m[i] = __fmaf_rn(u, QMAX, kMagic);
-      const float d = __fmaf_rn(u, QMAX, -__fsub_rn(m[i], kMagic));      // distance to the integer taken
-      if (fabsf(d) > 0.4999f) near_tie |= 1u << i;
-    }
-    uint32_t w[E / 4];  // codes, one per byte
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i) {
-      const uint32_t lo2 = __byte_perm(__float_as_uint(m[4 * i]), __float_as_uint(m[4 * i + 1]), 0x0040);
-      const uint32_t hi2 = __byte_perm(__float_as_uint(m[4 * i + 2]), __float_as_uint(m[4 * i + 3]), 0x0040);
-      w[i] = __byte_perm(lo2, hi2, 0x5410);
-    }
-    // About one thread in a hundred has such an element (a third of the warps): those codes are
-    // redone with the IEEE division from the element as stored and put into their byte.
-    while (near_tie) {
-      const int i = __ffs(near_tie) - 1;
-      near_tie &= near_tie - 1;
-      float xi;
-      if constexpr (std::is_same<T, float>::value) {
-        xi = src[i];
-      } else if constexpr (std::is_same<T, __half>::value) {
-        xi = __half2float(src[i]);
-      } else {
-        xi = __bfloat162float(src[i]);
-      }
-      float t = rintf(__fdiv_rn(__fsub_rn(xi, zef), scf));
-      t = fminf(fmaxf(t, 0.f), QMAX);
-      const uint32_t sh = (i & 3) * 8, code = (uint32_t)(int)t << sh, byte = 0xffu << sh;
-#pragma unroll
-      for (int k = 0; k < E / 4; ++k) {  // masks, not an indexed store: w stays in registers
-        const uint32_t sel = (k == (i >> 2)) ? byte : 0u;
-        w[k] = (w[k] & ~sel) | (code & sel);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i) w[i] <<= (NBITS * p);
-    // split-P: lane c = p*TPS + c' contributes bit slice p of bytes [E*c', E*c' + E)
-    for (int off = 1 << tps_shift; off < tpr; off <<= 1) {
-#pragma unroll
-      for (int i = 0; i < E / 4; ++i) w[i] |= __shfl_xor_sync(kFullMask, w[i], off);
-    }
+    quantize_part<T, NBITS, E>(x + r * D + E * c, lanes_per_group, w, sc16, ze16, m);
+    pack_slices<NBITS, E>(w, p, tps_shift, tpr);
     // Output row: the input row itself, or (append) slot pos[b] + t of sequence (b, head)
     // in a cache of `cap` token rows per sequence; tokens that fall outside are dropped.
     int64_t orow = row;
@@ -324,7 +141,6 @@ __global__ void __launch_bounds__(256)
                                  int64_t S, int64_t S_q, int D, int64_t n_blocks) {
   constexpr int P = 8 / NBITS;
   constexpr float QMAX = float((1 << NBITS) - 1);
-  constexpr float kMagic = 12582912.f;
   constexpr bool k16 = !std::is_same<T, float>::value;
   __shared__ __align__(16) uint8_t codes[512 * kChanTok];  // [local block][token][dim]
   const int tpb = D >> 1;                                   // threads per token block
