@@ -9,14 +9,13 @@
 // values tensor the token's code*scale + zero goes there too: what the cache now stands for, as a
 // prompt's own attention needs it.
 //
-// K and V go in one launch.  A thread owns E = 16 (8) consecutive elements of a row, in one row of a step and
-// four of a prompt.
-// Two ways to cut the rows (BLOCK):
-//   * prompts: a CTA takes a block of tokens of one head of one sequence, so that where it stands
-//     is known from its indexes alone and the codes and metadata it writes are consecutive;
-//   * a step (T of at most kStepTokens): a CTA takes rows of several heads and sequences.
-// The row's place (two dependent loads: position, then table entry) is looked up beside the element
-// loads and needed only by the stores.
+// K and V go in one launch.  A thread owns E = 16 (8) consecutive elements of a row.  Two ways to cut
+// the rows:
+//   * prompts: a warp takes 32 tokens of one head of one sequence; each lane looks up the place of one
+//     of them (two dependent loads: position, then table entry), and the warp walks over them,
+//     32 * E / D rows at a time, with the places in a shuffle's reach;
+//   * a step (T of at most kStepTokens): a CTA takes rows of several heads and sequences, one a
+//     thread, and every thread looks up its own.
 #include "tkv_quant_part.cuh"
 #include "tkv_splitk_driver.cuh"  // FastDiv
 
@@ -28,6 +27,7 @@ struct AppendTensor {
   __half *scale, *zero;             // (num_pages, HKV, page, D/gs)
   void* values;                     // (B, HKV, T, D) of x's type with its own strides, or null
   int64_t sb, sh, st, vb, vh, vt;
+  int values32;                     // every row of the values starts on a 32-byte boundary
 };
 
 struct AppendArgs {
@@ -40,7 +40,7 @@ struct AppendArgs {
 };
 
 constexpr int kStepTokens = 8;
-constexpr int kRowsBlock = 4, kRowsStep = 1;  // rows of a thread
+constexpr int kBlockThreads = 128;  // of a CTA of prompt rows: 128 tokens
 
 __device__ __forceinline__ float elem_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float elem_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -52,7 +52,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
 
 // 8 consecutive values, 16 or 32 bytes
 template <typename T>
-__device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
+__device__ __forceinline__ void store8(T* dst, const float* v) {
   if constexpr (std::is_same<T, float>::value) {
     reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -62,124 +62,129 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
   }
 }
 
-// The token of a row of the work.  A row that is not there names the nearest one that is, so that
-// a whole warp can load and shuffle.
-struct AppendRow {
-  int b, h, t;
-  bool live;
-};
-template <bool BLOCK>
-__device__ __forceinline__ AppendRow append_row(const AppendArgs& a, int rows_per_cta, int i) {
-  AppendRow w;
-  if constexpr (BLOCK) {
-    const int t = blockIdx.x * rows_per_cta + i;
-    w.b = blockIdx.z;
-    w.h = blockIdx.y >> 1;
-    w.live = t < a.T;
-    w.t = min(t, a.T - 1);
-  } else {
-    const int r = blockIdx.x * rows_per_cta + i, q = fast_div(r, a.dT), b = fast_div(q, a.dHKV);
-    w.live = b < a.B;
-    w.b = min(b, a.B - 1);
-    w.h = q - b * a.HKV;
-    w.t = r - q * a.T;
+// E consecutive values; 16 of a 16-bit type as one 32-byte store where they start on such a boundary
+// (two halves of a sector would travel to L2 apart).
+template <typename T, int E>
+__device__ __forceinline__ void store_row_part(T* dst, const float (&v)[E], bool aligned32) {
+  if constexpr (E == 16) {
+    if (aligned32) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = pack2(v[2 * i], v[2 * i + 1], dst);
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                   "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+      return;
+    }
   }
-  return w;
-}
-// Its pool row, or -1: nowhere.
-__device__ __forceinline__ int append_place(const AppendArgs& a, const AppendRow& w) {
-  const int len = a.lengths ? __ldg(a.lengths + w.b) : a.T;
-  const int64_t pos = (int64_t)(a.positions ? __ldg(a.positions + w.b) : a.pos0) + w.t;
-  if (!w.live || w.t >= len || (uint64_t)pos >= (uint32_t)a.limit) return -1;
-  const int k = fast_div((int)pos, a.dpage), id = __ldg(a.table + w.b * a.table_stride + k);
-  return (unsigned)id < (unsigned)a.num_pages ? (id * a.HKV + w.h) * a.page + ((int)pos - k * a.page) : -1;
+#pragma unroll
+  for (int i = 0; i < E / 8; ++i) store8(dst + 8 * i, v + 8 * i);
 }
 
-// `tpr_shift` = log2(D/E) (threads of a row), `lpg_shift` = log2(gs/E) (lanes of a group).
-template <typename T, int NBITS, int E, bool BLOCK>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int tpr_shift, int lpg_shift) {
-  constexpr int LOG2P = NBITS == 4 ? 1 : 2, ROWS = BLOCK ? kRowsBlock : kRowsStep;
-  const AppendTensor& w = a.t[blockIdx.y & 1];
-  const int tpr = 1 << tpr_shift, c = threadIdx.x & (tpr - 1), rstep = 256 >> tpr_shift;
+// The pool row of token t of (sequence b, head h), or -1: nowhere.
+__device__ __forceinline__ int append_place(const AppendArgs& a, int b, int h, int t) {
+  const int len = a.lengths ? __ldg(a.lengths + b) : a.T;
+  const int64_t pos = (int64_t)(a.positions ? __ldg(a.positions + b) : a.pos0) + t;
+  if (t >= min(len, a.T) || (uint64_t)pos >= (uint32_t)a.limit) return -1;
+  const int k = fast_div((int)pos, a.dpage), id = __ldg(a.table + b * a.table_stride + k);
+  return (unsigned)id < (unsigned)a.num_pages ? (id * a.HKV + h) * a.page + ((int)pos - k * a.page) : -1;
+}
+
+// Codes, scale and zero point of a thread's part of a row into pool row `at` (-1: nowhere), and what
+// they stand for to `val`.
+template <typename T, int NBITS, int E>
+__device__ __forceinline__ void append_part(const AppendTensor& w, const T* src, T* val, int at, int c, int tpr_shift,
+                                            int lpg_shift) {
+  constexpr int LOG2P = NBITS == 4 ? 1 : 2;
   const int tps_shift = tpr_shift - LOG2P, p = c >> tps_shift, D = E << tpr_shift;
-  if (BLOCK && a.lengths && (int)blockIdx.x * ROWS * rstep >= __ldg(a.lengths + blockIdx.z)) return;  // padding
-  const AppendRow row0 = append_row<BLOCK>(a, ROWS * rstep, threadIdx.x >> tpr_shift);
-  const T* src0 = reinterpret_cast<const T*>(w.x) + row0.b * w.sb + row0.h * w.sh + E * c;
-  T* val0 = reinterpret_cast<T*>(w.values) + row0.b * w.vb + row0.h * w.vh + E * c;
+  uint32_t code[E / 4];
+  __half sc16, ze16;
+  float m[E];
+  quantize_part<T, NBITS, E>(src, 1 << lpg_shift, code, sc16, ze16, m);
+  if (w.values && at >= 0) {
+    const float s = __half2float(sc16), z = __half2float(ze16);
 #pragma unroll
-  for (int it = 0; it < ROWS; ++it) {
-    AppendRow row = row0;
-    if (BLOCK && it > 0) row = append_row<BLOCK>(a, ROWS * rstep, it * rstep + (threadIdx.x >> tpr_shift));
-    const int at = append_place(a, row);
-    uint32_t code[E / 4];
-    __half sc16, ze16;
-    float m[E];
-    quantize_part<T, NBITS, E>(src0 + row.t * w.st, 1 << lpg_shift, code, sc16, ze16, m);
-    if (w.values && at >= 0) {
-      T* dst = val0 + row.t * w.vt;
-      const float s = __half2float(sc16), z = __half2float(ze16);
-#pragma unroll
-      for (int i = 0; i < E / 8; ++i) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = fmaf(__fsub_rn(m[8 * i + k], kMagic), s, z);  // (the product is exact)
-        store8(dst + 8 * i, v);
-      }
+    for (int i = 0; i < E; ++i) m[i] = fmaf(__fsub_rn(m[i], kMagic), s, z);  // (the product is exact)
+    store_row_part<T, E>(val, m, w.values32);
+  }
+  pack_slices<NBITS, E>(code, p, tps_shift, 1 << tpr_shift);
+  if (at >= 0) {
+    if (p == 0) {
+      uint8_t* dst = w.packed + (int64_t)at * (D >> LOG2P) + E * c;
+      if constexpr (E == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(code[0], code[1], code[2], code[3]);
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[1]);
     }
-    pack_slices<NBITS, E>(code, p, tps_shift, tpr);
-    if (at >= 0) {
-      if (p == 0) {
-        uint8_t* dst = w.packed + (int64_t)at * (D >> LOG2P) + E * c;
-        if constexpr (E == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(code[0], code[1], code[2], code[3]);
-        else *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[1]);
-      }
-      if ((c & ((1 << lpg_shift) - 1)) == 0) {
-        const int64_t g = ((int64_t)at << (tpr_shift - lpg_shift)) + (c >> lpg_shift);
-        w.scale[g] = sc16;
-        w.zero[g] = ze16;
-      }
+    if ((c & ((1 << lpg_shift) - 1)) == 0) {
+      const int64_t g = ((int64_t)at << (tpr_shift - lpg_shift)) + (c >> lpg_shift);
+      w.scale[g] = sc16;
+      w.zero[g] = ze16;
     }
   }
 }
 
 // Float16 pages: 8 elements of a thread; float16 rows are copied as stored, whatever a NaN holds.
-template <typename T, bool BLOCK>
-__global__ void __launch_bounds__(256) paged_append_f16_kernel(const AppendArgs a, int tpr_shift) {
-  constexpr int ROWS = BLOCK ? kRowsBlock : kRowsStep;
-  const AppendTensor& w = a.t[blockIdx.y & 1];
-  const int c = threadIdx.x & ((1 << tpr_shift) - 1), rstep = 256 >> tpr_shift, D = 8 << tpr_shift;
-#pragma unroll
-  for (int it = 0; it < ROWS; ++it) {
-    const AppendRow row = append_row<BLOCK>(a, ROWS * rstep, it * rstep + (threadIdx.x >> tpr_shift));
-    const int at = append_place(a, row);
-    if (at < 0) continue;
-    const T* src = reinterpret_cast<const T*>(w.x) + row.b * w.sb + row.h * w.sh + row.t * w.st + 8 * c;
-    uint4 y;
-    if constexpr (std::is_same<T, float>::value) {
-      const float4 u = __ldg(reinterpret_cast<const float4*>(src)), v = __ldg(reinterpret_cast<const float4*>(src) + 1);
-      y = make_uint4(pack_half2(u.x, u.y), pack_half2(u.z, u.w), pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+template <typename T>
+__device__ __forceinline__ void append_part_f16(const AppendTensor& w, const T* src, T* val, int at, int c, int D) {
+  if (at < 0) return;
+  uint4 y;
+  if constexpr (std::is_same<T, float>::value) {
+    const float4 u = __ldg(reinterpret_cast<const float4*>(src)), v = __ldg(reinterpret_cast<const float4*>(src) + 1);
+    y = make_uint4(pack_half2(u.x, u.y), pack_half2(u.z, u.w), pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+  } else {
+    y = __ldg(reinterpret_cast<const uint4*>(src));
+    if constexpr (!std::is_same<T, __half>::value) {
+      const T* e = reinterpret_cast<const T*>(&y);
+      const uint4 x = make_uint4(pack_half2(elem_f32(e[0]), elem_f32(e[1])), pack_half2(elem_f32(e[2]), elem_f32(e[3])),
+                                 pack_half2(elem_f32(e[4]), elem_f32(e[5])), pack_half2(elem_f32(e[6]), elem_f32(e[7])));
+      y = x;
+    }
+  }
+  *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(w.packed) + (int64_t)at * D + 8 * c) = y;
+  if (w.values) {
+    if constexpr (std::is_same<T, __half>::value) {
+      *reinterpret_cast<uint4*>(val) = y;
     } else {
-      y = __ldg(reinterpret_cast<const uint4*>(src));
-      if constexpr (!std::is_same<T, __half>::value) {
-        const T* e = reinterpret_cast<const T*>(&y);
-        const uint4 x = make_uint4(pack_half2(elem_f32(e[0]), elem_f32(e[1])), pack_half2(elem_f32(e[2]), elem_f32(e[3])),
-                                   pack_half2(elem_f32(e[4]), elem_f32(e[5])), pack_half2(elem_f32(e[6]), elem_f32(e[7])));
-        y = x;
-      }
-    }
-    *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(w.packed) + (int64_t)at * D + 8 * c) = y;
-    if (w.values) {
-      T* dst = reinterpret_cast<T*>(w.values) + row.b * w.vb + row.h * w.vh + row.t * w.vt + 8 * c;
-      if constexpr (std::is_same<T, __half>::value) {
-        *reinterpret_cast<uint4*>(dst) = y;
-      } else {
-        const __half* e = reinterpret_cast<const __half*>(&y);
-        float v[8];
+      const __half* e = reinterpret_cast<const __half*>(&y);
+      float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = __half2float(e[k]);
-        store8(dst, v);
-      }
+      for (int k = 0; k < 8; ++k) v[k] = __half2float(e[k]);
+      store8(val, v);
     }
+  }
+}
+
+// `tpr_shift` = log2(D/E) (threads of a row), `lpg_shift` = log2(gs/E) (lanes of a group); NBITS 16: float16
+// pages.
+template <typename T, int NBITS, int E, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? kBlockThreads : 256)
+    paged_append_kernel(const AppendArgs a, int tpr_shift, int lpg_shift) {
+  const AppendTensor& w = a.t[blockIdx.y & 1];
+  const int tpr = 1 << tpr_shift, c = threadIdx.x & (tpr - 1);
+  const T* x = reinterpret_cast<const T*>(w.x) + E * c;
+  T* values = reinterpret_cast<T*>(w.values) + E * c;
+  auto part = [&](int b, int h, int t, int at) {
+    const T* src = x + b * w.sb + h * w.sh + t * w.st;
+    T* val = values + b * w.vb + h * w.vh + t * w.vt;
+    if constexpr (NBITS == 16) append_part_f16<T>(w, src, val, at, c, E << tpr_shift);
+    else append_part<T, NBITS, E>(w, src, val, at, c, tpr_shift, lpg_shift);
+  };
+  if constexpr (BLOCK) {
+    const int lane = threadIdx.x & 31, b = blockIdx.z, h = blockIdx.y >> 1;
+    const int t0 = (blockIdx.x * (kBlockThreads / 32) + (threadIdx.x >> 5)) * 32;
+    const int len = min(a.T, a.lengths ? __ldg(a.lengths + b) : a.T);
+    if (t0 >= len) return;  // padding
+    const int place = append_place(a, b, h, t0 + lane);
+    const int per_pass = 32 >> tpr_shift, n = min(32, len - t0);
+    for (int r0 = 0; r0 < n; r0 += per_pass) {
+      const int r = r0 + (lane >> tpr_shift);
+      // (a row past the end has place -1 and mirrors the last one: the shuffles stay full-warp)
+      part(b, h, t0 + min(r, n - 1), __shfl_sync(kFullMask, place, r));
+    }
+  } else {
+    const int r = blockIdx.x * (256 >> tpr_shift) + (threadIdx.x >> tpr_shift);
+    const int q = fast_div(r, a.dT), b = fast_div(q, a.dHKV), h = q - b * a.HKV, t = r - q * a.T;
+    const bool live = b < a.B;
+    part(min(b, a.B - 1), h, t, live ? append_place(a, b, h, t) : -1);
   }
 }
 
@@ -193,17 +198,18 @@ static inline int log2i(int v) {
 template <typename T, bool BLOCK>
 static void launch_append_as(const AppendArgs& a, dim3 grid, int D, int nbits, int gs, bool wide, cudaStream_t stream) {
   const int E = wide ? 16 : 8, tpr = log2i(D / E), lpg = nbits == 16 ? 0 : log2i(gs / E);
+  constexpr int threads = BLOCK ? kBlockThreads : 256;
   if (nbits == 16) {
-    paged_append_f16_kernel<T, BLOCK><<<grid, 256, 0, stream>>>(a, tpr);
+    paged_append_kernel<T, 16, 8, BLOCK><<<grid, threads, 0, stream>>>(a, tpr, lpg);
   } else if (wide) {
     if constexpr (!std::is_same<T, float>::value) {
-      if (nbits == 4) paged_append_kernel<T, 4, 16, BLOCK><<<grid, 256, 0, stream>>>(a, tpr, lpg);
-      else paged_append_kernel<T, 2, 16, BLOCK><<<grid, 256, 0, stream>>>(a, tpr, lpg);
+      if (nbits == 4) paged_append_kernel<T, 4, 16, BLOCK><<<grid, threads, 0, stream>>>(a, tpr, lpg);
+      else paged_append_kernel<T, 2, 16, BLOCK><<<grid, threads, 0, stream>>>(a, tpr, lpg);
     }
   } else if (nbits == 4) {
-    paged_append_kernel<T, 4, 8, BLOCK><<<grid, 256, 0, stream>>>(a, tpr, lpg);
+    paged_append_kernel<T, 4, 8, BLOCK><<<grid, threads, 0, stream>>>(a, tpr, lpg);
   } else {
-    paged_append_kernel<T, 2, 8, BLOCK><<<grid, 256, 0, stream>>>(a, tpr, lpg);
+    paged_append_kernel<T, 2, 8, BLOCK><<<grid, threads, 0, stream>>>(a, tpr, lpg);
   }
 }
 
@@ -211,13 +217,11 @@ template <typename T>
 static int launch_append(const AppendArgs& a, int D, int nbits, int gs, cudaStream_t stream) {
   // 16 elements of a thread where a 16-bit row gives every bit slice and every group a whole thread
   const bool wide = !std::is_same<T, float>::value && nbits != 16 && gs >= 16 && D / 16 >= 8 / nbits;
-  const int per_pass = 256 >> log2i(D / (wide ? 16 : 8));
   // (65535: the limit of the grid's y and z)
   if (a.T > kStepTokens && a.HKV <= 65535 / 2 && a.B <= 65535) {
-    const int per_cta = kRowsBlock * per_pass;
-    launch_append_as<T, true>(a, dim3((a.T + per_cta - 1) / per_cta, 2 * a.HKV, a.B), D, nbits, gs, wide, stream);
+    launch_append_as<T, true>(a, dim3((a.T + kBlockThreads - 1) / kBlockThreads, 2 * a.HKV, a.B), D, nbits, gs, wide, stream);
   } else {
-    const int64_t rows = (int64_t)a.B * a.HKV * a.T, per_cta = kRowsStep * per_pass;
+    const int64_t rows = (int64_t)a.B * a.HKV * a.T, per_cta = 256 >> log2i(D / (wide ? 16 : 8));
     launch_append_as<T, false>(a, dim3((unsigned)((rows + per_cta - 1) / per_cta), 2), D, nbits, gs, wide, stream);
   }
   TKV_CUDA(cudaGetLastError());
@@ -268,10 +272,15 @@ extern "C" int tkv_paged_append(const void* k, const void* v, int in_dtype, cons
   TKV_REQUIRE((int64_t)num_pages * HKV * page_size < (1LL << 31), TKV_ERR_INVALID,
               "paged append: a pool of %lld token rows exceeds 2^31", (long long)num_pages * HKV * page_size);
   AppendArgs a{};
-  a.t[0] = {k, k_packed, (__half*)k_scale, (__half*)k_zero, k_values, strides[0], strides[1], strides[2], 0, 0, 0};
-  a.t[1] = {v, v_packed, (__half*)v_scale, (__half*)v_zero, v_values, strides[3], strides[4], strides[5], 0, 0, 0};
+  a.t[0] = {k, k_packed, (__half*)k_scale, (__half*)k_zero, k_values, strides[0], strides[1], strides[2], 0, 0, 0, 0};
+  a.t[1] = {v, v_packed, (__half*)v_scale, (__half*)v_zero, v_values, strides[3], strides[4], strides[5], 0, 0, 0, 0};
   if (k_values) a.t[0].vb = value_strides[0], a.t[0].vh = value_strides[1], a.t[0].vt = value_strides[2];
   if (v_values) a.t[1].vb = value_strides[3], a.t[1].vh = value_strides[4], a.t[1].vt = value_strides[5];
+  for (int i = 0; i < 2; ++i) {
+    const AppendTensor& t = a.t[i];
+    a.t[i].values32 = in_dtype != TKV_DTYPE_F32 && ((uintptr_t)t.values & 31) == 0 && t.vb % 16 == 0 && t.vh % 16 == 0 &&
+                      t.vt % 16 == 0;
+  }
   a.table = block_table;
   a.positions = positions;
   a.lengths = lengths;
