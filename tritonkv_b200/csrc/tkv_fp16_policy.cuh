@@ -40,6 +40,10 @@ struct Fp16Policy {
     float acc[NCH][4];
   };
 
+  struct Scores {
+    float s[4];  // (token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
+  };
+
   __device__ static void report_timeout() { atomicExch(&g_fp16_status, 1); }
   __device__ static __forceinline__ void prefetch_maps(const Maps&) {}
 
@@ -83,6 +87,13 @@ struct Fp16Policy {
     issue(is, p, maps, max(rows[0], 0), rows[0] < 0 ? 0 : nvalid, st, nullptr, bar, lane);
   }
 
+  // Scores of tokens from `left` on, or of all where the tile lies in no page (`valid` 0)
+  __device__ static __forceinline__ void mask_tokens(Scores& sc, int left, uint32_t valid, int lane) {
+    const int n = valid ? left - (lane >> 2) : 0;
+    if (n <= 0) sc.s[0] = sc.s[1] = -INFINITY;
+    if (n <= 8) sc.s[2] = sc.s[3] = -INFINITY;
+  }
+
   // query fragments: B operand, k-slots (2t,2t+1) <-> dims 16c+2t, 16c+2t+1 and
   // (2t+8, 2t+9) <-> dims 16c+8+2t, 16c+9+2t, column g = head g.
   static constexpr int QFRAG_BYTES = 0;  // every warp reads the query rows itself
@@ -114,10 +125,6 @@ struct Fp16Policy {
 #pragma unroll
       for (int i = 0; i < 4; ++i) ac.acc[ch][i] = 0.f;
   }
-
-  struct Scores {
-    float s[4];  // (token g, head 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
-  };
 
   // Scores of one 16-token tile (scaled, tokens past the unit end set to -inf).
   __device__ static __forceinline__ void scores(Scores& out, const Query& qq, uint32_t st,

@@ -278,15 +278,14 @@ struct FusedPolicy {
     cp_async_mbar_arrive_noinc(bar);
   }
 
-  // Scores of pieces that name no page (bit h of `valid` clear)
-  __device__ static __forceinline__ void mask_pieces(Scores& sc, uint32_t valid) {
+  // Scores of tokens from `left` on, and of pieces that name no page (bit h of `valid` clear)
+  __device__ static __forceinline__ void mask_tokens(Scores& sc, int left, uint32_t valid, int lane) {
 #pragma unroll
-    for (int h = 0; h < PIECES; ++h)
-      if (!((valid >> h) & 1u)) {
-#pragma unroll
-        for (int mt = h * MT / PIECES; mt < (h + 1) * MT / PIECES; ++mt)
-          sc.s[mt][0] = sc.s[mt][1] = sc.s[mt][2] = sc.s[mt][3] = -INFINITY;
-      }
+    for (int mt = 0; mt < MT; ++mt) {
+      const int n = ((valid >> (mt * PIECES / MT)) & 1u) ? left - mt * 16 - (lane >> 2) : 0;
+      if (n <= 0) sc.s[mt][0] = sc.s[mt][1] = -INFINITY;
+      if (n <= 8) sc.s[mt][2] = sc.s[mt][3] = -INFINITY;
+    }
   }
 
   // Scale/zero of a tile in CS-byte copies: rows that only start on 8- or 4-byte boundaries

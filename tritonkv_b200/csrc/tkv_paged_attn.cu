@@ -26,6 +26,7 @@
 
 namespace tkv {
 
+constexpr float kNoReference = -1e30f;  // below every score: the softmax reference before the first token
 constexpr int kMaxPagedB = 512;  // sequences whose tile prefix a CTA holds; larger batches go in parts
 
 struct PagedParams {
@@ -35,7 +36,7 @@ struct PagedParams {
   void* out;
   int out_dtype;
   int num_pages, page, max_pages, HKVc;
-  FastDiv dpage, dHch, dHKVc;
+  FastDiv dpage, dHch, dHKVc, dHQ, dgroup;
   float *acc, *m, *l;     // (slots, 8, D), (slots, 8), (slots, 8)
   int2* info;             // (units): first slot and number of partials; none: the output is there
 };
@@ -52,47 +53,59 @@ __device__ __forceinline__ void store_out4(void* out, int dtype, int64_t i, floa
   }
 }
 
+// The part of a unit that a CTA processes.  `pref` is the prefix of tiles per sequence, see the kernel.
 struct PagedSegment {
-  int b, hkv, hc, unit;
-  int lo_tok, hi;   // first token; end of the sequence
+  int b, hk;        // sequence; KV head and head chunk
+  int hi, t_b;      // length of the sequence, tiles of the unit
+  int lo_tile;      // first tile, within the unit
   int ntiles, g_end;
-  int first, count; // first CTA of the unit and how many it spans
 };
 
 template <int kTok>
-__device__ __forceinline__ PagedSegment paged_segment_at(const PagedParams& pp, const int* pref, FastDiv dTC,
-                                                         int g, int g1) {
+__device__ __forceinline__ void paged_segment_of(PagedSegment& s, const int* pref, int g, int g1) {
+  const int word = pref[s.b];
+  s.t_b = (pref[s.b + 1] >> kRemBits) - (word >> kRemBits);
+  s.hi = (s.t_b - 1) * kTok + (word & ((1 << kRemBits) - 1)) + 1;
+  s.ntiles = min(g1 - g, s.t_b - s.lo_tile);
+  s.g_end = g + s.ntiles;
+}
+// The segment at tile g of the tile sequence
+template <int kTok>
+__device__ __forceinline__ PagedSegment paged_segment_at(const int* pref, int B, int HKVc, int g, int g1) {
   PagedSegment s;
-  int lo = 0, hi = pp.d.B;  // largest b with HKVc * pref[b] <= g (sequences without tiles are skipped)
+  int lo = 0, hi = B;  // largest b with HKVc * pref[b] <= g (sequences without tiles are skipped)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (pp.HKVc * (pref[mid] >> kRemBits) <= g) lo = mid; else hi = mid;
+    if (HKVc * (pref[mid] >> kRemBits) <= g) lo = mid; else hi = mid;
   }
-  const int word = pref[lo], before = word >> kRemBits;
-  const int t_b = (pref[lo + 1] >> kRemBits) - before;
-  const int r = g - pp.HKVc * before;
-  const int hk = (int)((uint32_t)r / (uint32_t)t_b);
-  const int tile = r - hk * t_b;
-  const int unit_start = g - tile, unit_end = unit_start + t_b;
+  const int before = pref[lo] >> kRemBits, t_b = (pref[lo + 1] >> kRemBits) - before, r = g - HKVc * before;
   s.b = lo;
-  s.unit = lo * pp.HKVc + hk;
-  s.hkv = fast_div(hk, pp.dHch);
-  s.hc = hk - s.hkv * pp.d.hchunks;
-  s.hi = (t_b - 1) * kTok + (word & ((1 << kRemBits) - 1)) + 1;
-  s.lo_tok = tile * kTok;
-  s.g_end = min(g1, unit_end);
-  s.ntiles = s.g_end - g;
-  s.first = fast_div(unit_start, dTC);
-  s.count = fast_div(unit_end - 1, dTC) - s.first + 1;
+  s.hk = (int)((uint32_t)r / (uint32_t)t_b);
+  s.lo_tile = r - s.hk * t_b;
+  paged_segment_of<kTok>(s, pref, g, g1);
   return s;
+}
+// The one behind it (there is one: s.g_end < g1): the next unit from its start
+template <int kTok>
+__device__ __forceinline__ void paged_segment_next(PagedSegment& s, const int* pref, int HKVc, int g1) {
+  s.lo_tile = 0;
+  if (++s.hk == HKVc) {
+    s.hk = 0;
+    do ++s.b;
+    while ((pref[s.b + 1] >> kRemBits) == (pref[s.b] >> kRemBits));
+    paged_segment_of<kTok>(s, pref, s.g_end, g1);
+  } else {
+    s.ntiles = min(g1 - s.g_end, s.t_b);
+    s.g_end += s.ntiles;
+  }
 }
 
 // Where a warp's copies stand: the next tile to issue, segments ahead of the one being computed.
 template <int PIECES>
 struct PagedCursor {
-  int b, hkv;
-  int tok, hi;       // first token of the next tile; end of the sequence
-  int cnt, g_end;    // tiles left in the cursor's segment; its end
+  PagedSegment seg;
+  int tok;           // first token of the next tile
+  int cnt;           // tiles left in the cursor's segment
   int k;             // which lane's row the next tile takes
   int row[PIECES];   // this lane's: pool rows of tile `lane` of the present 32, or -1
 };
@@ -140,13 +153,14 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   }
   const int q_esz = p.q_dtype == TKV_DTYPE_F32 ? 4 : 2;
   auto prefetch_q = [&](int slot, const PagedSegment& s) {
+    const int s_hkv = fast_div(s.hk, pp.dHch), s_hc = s.hk - s_hkv * p.hchunks;
     const int row_bytes = D * q_esz, cpr = row_bytes >> 4, cpr_shift = q_esz == 4 ? kLog2D - 2 : kLog2D - 3;
     for (int i = threadIdx.x; i < kHeadsPerCta * cpr; i += WARPS * 32) {
       const int h = i >> cpr_shift, c = i - (h << cpr_shift);
-      const int hg = s.hc * kHeadsPerCta + h;
+      const int hg = s_hc * kHeadsPerCta + h;
       const bool ok = hg < p.group;
       const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
-                           (((int64_t)s.b * p.HQ + (int64_t)s.hkv * p.group + hg) * D) * q_esz + c * 16;
+                           (((int64_t)s.b * p.HQ + (int64_t)s_hkv * p.group + hg) * D) * q_esz + c * 16;
       cp_async16(qbuf_u32 + slot * QB + h * row_bytes + c * 16,
                  ok ? src : reinterpret_cast<const uint8_t*>(p.q), ok ? 16 : 0);
     }
@@ -182,52 +196,56 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   const int T = pp.HKVc * (s_pref[p.B] >> kRemBits);
   int TC = max(1, (T + (int)gridDim.x - 1) / (int)gridDim.x);
   if (TC <= 4 * WARPS) TC = (TC + WARPS - 1) / WARPS * WARPS;  // no warp without a tile: fewer partials, same time
-  const FastDiv dTC = make_fastdiv_device(TC);
-  // sequences without tokens are touched by no range
-  for (int u = cta; u < p.B * pp.HKVc; u += gridDim.x) {
-    const int b = fast_div(u, pp.dHKVc), hk = u - b * pp.HKVc;
-    if ((s_pref[b + 1] >> kRemBits) != (s_pref[b] >> kRemBits)) continue;
-    const int hkv = fast_div(hk, pp.dHch), hc = hk - hkv * p.hchunks;
-    for (int idx = threadIdx.x; idx < kHeadsPerCta * D / 4; idx += WARPS * 32) {
-      const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4, hg = hc * kHeadsPerCta + h;
-      if (hg < p.group)
-        store_out4(pp.out, pp.out_dtype, ((int64_t)b * p.HQ + hkv * p.group + hg) * D + d, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
-    if (threadIdx.x == 0) pp.info[u] = make_int2(0, 0);
-  }
   const int g0 = min(cta * TC, T), g1 = min(g0 + TC, T);
-  if (g0 >= g1) return;
-  PagedSegment seg = paged_segment_at<kTok>(pp, s_pref, dTC, g0, g1);
+  // sequences without tokens are touched by no range
+  auto empty_units = [&]() {
+    for (int u = cta; u < p.B * pp.HKVc; u += gridDim.x) {
+      const int b = fast_div(u, pp.dHKVc), hk = u - b * pp.HKVc;
+      if ((s_pref[b + 1] >> kRemBits) != (s_pref[b] >> kRemBits)) continue;
+      const int hkv = fast_div(hk, pp.dHch), hc = hk - hkv * p.hchunks;
+      for (int idx = threadIdx.x; idx < kHeadsPerCta * D / 4; idx += WARPS * 32) {
+        const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4, hg = hc * kHeadsPerCta + h;
+        if (hg < p.group)
+          store_out4(pp.out, pp.out_dtype, ((int64_t)b * p.HQ + hkv * p.group + hg) * D + d, make_float4(0.f, 0.f, 0.f, 0.f));
+      }
+      if (threadIdx.x == 0) pp.info[u] = make_int2(0, 0);
+    }
+  };
+  if (g0 >= g1) {
+    empty_units();
+    return;
+  }
+  PagedSegment seg = paged_segment_at<kTok>(s_pref, p.B, pp.HKVc, g0, g1);
 
   // ---- issue cursor ----
   PagedCursor<PIECES> cur;
+  cur.seg = seg;
   auto look_up = [&]() {  // lane i: the rows of this warp's i-th tile from the cursor on
     cur.k = 0;
-    const int tok = cur.tok + lane * (WARPS * kTok);
+    const int tok = cur.tok + lane * (WARPS * kTok), hkv = fast_div(cur.seg.hk, pp.dHch);
 #pragma unroll
     for (int h = 0; h < PIECES; ++h) {
       const int n = tok + h * (kTok / PIECES);
       int row = -1;
-      if (lane < cur.cnt && n < cur.hi) {
-        const int i = fast_div(n, pp.dpage), id = __ldcg(pp.table + cur.b * pp.table_stride + i);
-        if ((unsigned)id < (unsigned)pp.num_pages) row = (id * p.HKV + cur.hkv) * pp.page + (n - i * pp.page);
+      if (lane < cur.cnt && n < cur.seg.hi) {
+        const int i = fast_div(n, pp.dpage), id = __ldcg(pp.table + cur.seg.b * pp.table_stride + i);
+        if ((unsigned)id < (unsigned)pp.num_pages) row = (id * p.HKV + hkv) * pp.page + (n - i * pp.page);
       }
       cur.row[h] = row;
     }
   };
-  auto cursor_enter = [&](const PagedSegment& s) {
-    cur.b = s.b;
-    cur.hkv = s.hkv;
-    cur.tok = s.lo_tok + warp * kTok;
-    cur.hi = s.hi;
-    cur.cnt = s.ntiles > warp ? (s.ntiles - warp + WARPS - 1) / WARPS : 0;
-    cur.g_end = s.g_end;
+  auto cursor_enter = [&]() {
+    cur.tok = (cur.seg.lo_tile + warp) * kTok;
+    cur.cnt = cur.seg.ntiles > warp ? (cur.seg.ntiles - warp + WARPS - 1) / WARPS : 0;
     if (cur.cnt > 0) look_up();
   };
   auto cursor_skip_empty = [&]() {  // to the next segment in which this warp has a tile
-    while (cur.cnt == 0 && cur.g_end < g1) cursor_enter(paged_segment_at<kTok>(pp, s_pref, dTC, cur.g_end, g1));
+    while (cur.cnt == 0 && cur.seg.g_end < g1) {
+      paged_segment_next<kTok>(cur.seg, s_pref, pp.HKVc, g1);
+      cursor_enter();
+    }
   };
-  cursor_enter(seg);
+  cursor_enter();
   cursor_skip_empty();
   int iss_slot = 0;          // slot the next issue fills
   uint32_t valid = 0;        // bits [s*PIECES, (s+1)*PIECES): which pieces of slot s name a page
@@ -249,7 +267,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       ok |= (rows[h] >= 0 ? 1u : 0u) << h;
     }
     valid = (valid & ~(kAll << (slot * PIECES))) | (ok << (slot * PIECES));
-    Policy::issue_pieces(ist, p, maps, rows, min(kTok, cur.hi - cur.tok), ring_u32 + slot * STAGE_BYTES,
+    Policy::issue_pieces(ist, p, maps, rows, min(kTok, cur.seg.hi - cur.tok), ring_u32 + slot * STAGE_BYTES,
                          bar_u32 + 8 * slot, lane);
     cur.tok += WARPS * kTok;
     if (--cur.cnt == 0) cursor_skip_empty();
@@ -258,7 +276,12 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   prefetch_q(0, seg);
 #pragma unroll 1
   for (int s = 0; s < STAGES - 1; ++s) issue_next();
-  if (seg.g_end < g1) prefetch_q(1, paged_segment_at<kTok>(pp, s_pref, dTC, seg.g_end, g1));
+  empty_units();
+  if (seg.g_end < g1) {
+    PagedSegment s = seg;
+    paged_segment_next<kTok>(s, s_pref, pp.HKVc, g1);
+    prefetch_q(1, s);
+  }
   int seg_k = 0;  // index of the current segment within this CTA
   int c_slot = 0, c_phase = 0;  // slot and barrier phase of the next tile to consume
   bool timed_out = false;
@@ -273,19 +296,17 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     }
     Policy::load_query(qs, p, qbuf + (seg_k & 1) * QB, qfrag_u32, lane);
     Policy::reset(acc);
+    // (finite, so that a first tile without any token is exp2(-inf) = 0 like any other masked one)
+    acc.m_ref0 = acc.m_ref1 = kNoReference;
     const int my_tiles = seg.ntiles > warp ? (seg.ntiles - warp + WARPS - 1) / WARPS : 0;
-    int left = seg.hi - (seg.lo_tok + warp * kTok);
+    int left = seg.hi - (seg.lo_tile + warp) * kTok;
     auto scores = [&](typename Policy::Scores& sc, int slot, int left_of) {
-      Policy::scores(sc, qs, ring_u32 + slot * STAGE_BYTES, ring + slot * STAGE_BYTES, left_of, p.qk_scale, lane);
-      if constexpr (PIECES > 1) {
-        const uint32_t v = valid >> (slot * PIECES) & kAll;
-        if (v != kAll) Policy::mask_pieces(sc, v);
-      }
+      Policy::scores(sc, qs, ring_u32 + slot * STAGE_BYTES, ring + slot * STAGE_BYTES, kTok, p.qk_scale, lane);
+      const uint32_t v = valid >> (slot * PIECES) & kAll;
+      if (left_of < kTok || v != kAll) Policy::mask_tokens(sc, left_of, v, lane);
     };
-    // a tile of nothing but unnamed pages adds nothing (and has no maximum)
     auto update = [&](typename Policy::Scores& sc, int slot) {
-      if (valid >> (slot * PIECES) & kAll)
-        Policy::update(acc, qs, sc, ring_u32 + slot * STAGE_BYTES, ring + slot * STAGE_BYTES, left, lane);
+      Policy::update(acc, qs, sc, ring_u32 + slot * STAGE_BYTES, ring + slot * STAGE_BYTES, left, lane);
     };
     // Software pipeline: the scores of tile i+1 beside the softmax and output of tile i.
     if (my_tiles > 0 && !timed_out) {
@@ -342,11 +363,17 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       uint32_t voff[WARPS];
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) voff[w] = (uint32_t)((w * STAGES + s_slot[w]) * STAGE_BYTES);
-      const int64_t slot = (int64_t)(seg.unit + cta) * kHeadsPerCta;
+      const int hkv = fast_div(seg.hk, pp.dHch), hc = seg.hk - hkv * p.hchunks;
+      const int unit = seg.b * pp.HKVc + seg.hk;
+      // the CTAs of the unit: only a unit that crosses a border of this one's range takes a division
+      const int u0 = seg.g_end - seg.ntiles - seg.lo_tile, u1 = u0 + seg.t_b;  // its tiles in the sequence
+      const int first = seg.lo_tile == 0 ? cta : (int)((uint32_t)u0 / (uint32_t)TC);
+      const int count = (u1 <= g1 ? cta : (int)((uint32_t)(u1 - 1) / (uint32_t)TC)) - first + 1;
+      const int64_t slot = (int64_t)(unit + cta) * kHeadsPerCta;
 #pragma unroll
       for (int it = 0; it < ITEMS / (WARPS * 32); ++it) {
         const int idx = it * (WARPS * 32) + threadIdx.x;
-        const int h = idx / D4, d = (idx - h * D4) * 4, hg = seg.hc * kHeadsPerCta + h;
+        const int h = idx / D4, d = (idx - h * D4) * 4, hg = hc * kHeadsPerCta + h;
         if (hg >= p.group) continue;
         float mw[WARPS], M = -INFINITY;
 #pragma unroll
@@ -367,7 +394,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
           a.w = fmaf(s, live ? v.w : 0.f, a.w);
           L = fmaf(s, s_l[w][h], L);
         }
-        if (seg.count > 1) {
+        if (count > 1) {
           *reinterpret_cast<float4*>(pp.acc + (slot + h) * D + d) = a;
           if (d == 0) {
             pp.m[slot + h] = M;
@@ -375,20 +402,21 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
           }
         } else {
           const float inv = L > 0.f ? 1.f / L : 0.f;
-          store_out4(pp.out, pp.out_dtype, ((int64_t)seg.b * p.HQ + seg.hkv * p.group + hg) * D + d,
+          store_out4(pp.out, pp.out_dtype, ((int64_t)seg.b * p.HQ + hkv * p.group + hg) * D + d,
                      make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
         }
       }
-      if (threadIdx.x == 0 && seg.first == cta)
-        pp.info[seg.unit] = seg.count > 1 ? make_int2(seg.unit + cta, seg.count) : make_int2(0, 0);
+      if (threadIdx.x == 0 && first == cta) pp.info[unit] = count > 1 ? make_int2(unit + cta, count) : make_int2(0, 0);
     }
     __syncthreads();
     need_proxy_fence = true;
-    const int g = seg.g_end;
-    if (g >= g1 || timed_out) break;
-    seg = paged_segment_at<kTok>(pp, s_pref, dTC, g, g1);
-    if (seg.g_end < g1)  // the query slot just released takes the segment after the next
-      prefetch_q(seg_k & 1, paged_segment_at<kTok>(pp, s_pref, dTC, seg.g_end, g1));
+    if (seg.g_end >= g1 || timed_out) break;
+    paged_segment_next<kTok>(seg, s_pref, pp.HKVc, g1);
+    if (seg.g_end < g1) {  // the query slot just released takes the segment after the next
+      PagedSegment s = seg;
+      paged_segment_next<kTok>(s, s_pref, pp.HKVc, g1);
+      prefetch_q(seg_k & 1, s);
+    }
     ++seg_k;
   }
   if (timed_out && lane == 0) Policy::report_timeout();
@@ -396,75 +424,153 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
 
 // ---------------------------------------------------------------- merge of a unit's partials
 //     out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M),   M = max_s m_s
-// GROUPS groups of D/4 threads per row (sequence, query head): a warp or half of one where there are
-// many rows of few partials each, a whole CTA where few rows have many.
-template <int D, int GROUPS>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams pp, int rows) {
-  constexpr int TPR = D / 4 * GROUPS, RPC = 256 / TPR;  // threads per row, rows per CTA
-  __shared__ float4 s_a[GROUPS > 1 ? 256 : 1];
-  __shared__ float s_x[GROUPS > 1 ? 256 : 1];
+// Bound by latency: where the partials are (one load), then maxima, sums and the first partials in one
+// go.  A partial without tokens has m = -inf, weighs 0 and holds zeros.
+
+// Where the partials of row (sequence, query head) are: first slot row and how many; 0: nothing to do.
+__device__ __forceinline__ int2 paged_partials(const PagedParams& pp, int row) {
   const DecodeParams& p = pp.d;
-  const int tid = threadIdx.x, sub = tid % TPR, row = blockIdx.x * RPC + tid / TPR;
-  const int g = sub / (D / 4), d = sub % (D / 4) * 4;
-  if (GROUPS > 1) pdl_launch_dependents();
+  const int b = fast_div(row, pp.dHQ), hq = row - b * p.HQ, hkv = fast_div(hq, pp.dgroup), hg = hq - hkv * p.group;
+  const int2 at = __ldcg(pp.info + b * pp.HKVc + hkv * p.hchunks + hg / kHeadsPerCta);
+  return make_int2(at.x * kHeadsPerCta + hg % kHeadsPerCta, at.y);
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor_sync(kFullMask, x, off));
+  return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) x += __shfl_xor_sync(kFullMask, x, off);
+  return x;
+}
+__device__ __forceinline__ void fma4(float4& a, float w, const float4& x) {
+  a.x = fmaf(w, x.x, a.x);
+  a.y = fmaf(w, x.y, a.y);
+  a.z = fmaf(w, x.z, a.z);
+  a.w = fmaf(w, x.w, a.w);
+}
+
+// Many rows of few partials each: a warp per row, 128 / D partials at a time.
+template <int D>
+__global__ void __launch_bounds__(256) paged_merge_rows_kernel(const PagedParams pp, int rows) {
+  constexpr int PAR = 128 / D, AHEAD = 4;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int sub = lane / (32 / PAR), d = lane % (32 / PAR) * 4;
   pdl_wait();
-  int2 at = make_int2(0, 0);
-  int h = 0;
   if (row < rows) {
-    const int b = row / p.HQ, hq = row - b * p.HQ, hkv = hq / p.group, hg = hq - hkv * p.group;
-    at = __ldcg(pp.info + b * pp.HKVc + hkv * p.hchunks + hg / kHeadsPerCta);
-    h = hg % kHeadsPerCta;
-  }
-  const int n = at.y;
-  const int64_t r0 = (int64_t)at.x * kHeadsPerCta + h;
-  float M = -INFINITY;
-  if constexpr (GROUPS == 1) {
-    for (int s = 0; s < n; ++s) M = fmaxf(M, __ldcg(pp.m + r0 + s * kHeadsPerCta));
-  } else {
-    for (int s = sub; s < n; s += TPR) M = fmaxf(M, __ldcg(pp.m + r0 + s * kHeadsPerCta));
+    const int2 at = paged_partials(pp, row);
+    const int n = at.y;
+    if (n > 0) {
+      const float* acc = pp.acc + (int64_t)at.x * D + d;
+      float4 x[AHEAD], a = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto fetch = [&](int s0) {
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(kFullMask, M, off));
-    s_x[tid] = M;
-    __syncthreads();
+        for (int i = 0; i < AHEAD; ++i) {
+          const int s = s0 + i * PAR + sub;
+          x[i] = s < n ? __ldcg(reinterpret_cast<const float4*>(acc + (int64_t)s * (kHeadsPerCta * D))) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      };
+      fetch(0);
+      float m = lane < n ? __ldcg(pp.m + at.x + lane * kHeadsPerCta) : -INFINITY;
+      float l = lane < n ? __ldcg(pp.l + at.x + lane * kHeadsPerCta) : 0.f;
+      float M = m;
+      for (int s = 32 + lane; s < n; s += 32) M = fmaxf(M, __ldcg(pp.m + at.x + s * kHeadsPerCta));
+      M = warp_max(M);
+      float L = 0.f;
+      for (int s0 = 0; s0 < n; s0 += 32) {  // weights of 32 partials, a lane each
+        if (s0 > 0) {
+          m = s0 + lane < n ? __ldcg(pp.m + at.x + (s0 + lane) * kHeadsPerCta) : -INFINITY;
+          l = s0 + lane < n ? __ldcg(pp.l + at.x + (s0 + lane) * kHeadsPerCta) : 0.f;
+        }
+        const float w = m > -INFINITY ? ex2(m - M) : 0.f;
+        L = fmaf(w, l, L);
+        for (int s1 = s0; s1 < min(n, s0 + 32); s1 += AHEAD * PAR) {
+          if (s1 > 0) fetch(s1);
 #pragma unroll
-    for (int w = 0; w < TPR / 32; ++w) M = fmaxf(M, s_x[tid / TPR * TPR + w * 32]);
-    __syncthreads();
-  }
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float L = 0.f;
-#pragma unroll 4
-  for (int s = g; s < n; s += GROUPS) {
-    const int64_t r = r0 + s * kHeadsPerCta;
-    const float m = __ldcg(pp.m + r), l = __ldcg(pp.l + r);
-    const float4 x = __ldcg(reinterpret_cast<const float4*>(pp.acc + r * D + d));
-    const float w = m > -INFINITY ? ex2(m - M) : 0.f;  // a partial without tokens is zero
-    a.x = fmaf(w, x.x, a.x);
-    a.y = fmaf(w, x.y, a.y);
-    a.z = fmaf(w, x.z, a.z);
-    a.w = fmaf(w, x.w, a.w);
-    L = fmaf(w, l, L);
-  }
-  if constexpr (GROUPS > 1) {
-    s_a[tid] = a;
-    s_x[tid] = L;
-    __syncthreads();
-    if (g == 0) {
-#pragma unroll
-      for (int k = 1; k < GROUPS; ++k) {
-        const float4 x = s_a[tid + k * (D / 4)];
-        a.x += x.x;
-        a.y += x.y;
-        a.z += x.z;
-        a.w += x.w;
-        L += s_x[tid + k * (D / 4)];
+          for (int i = 0; i < AHEAD; ++i) fma4(a, __shfl_sync(kFullMask, w, (s1 - s0 + i * PAR + sub) & 31), x[i]);
+        }
       }
+      L = warp_sum(L);
+      if constexpr (PAR == 2) {
+        a.x += __shfl_xor_sync(kFullMask, a.x, 16);
+        a.y += __shfl_xor_sync(kFullMask, a.y, 16);
+        a.z += __shfl_xor_sync(kFullMask, a.z, 16);
+        a.w += __shfl_xor_sync(kFullMask, a.w, 16);
+      }
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      if (sub == 0)
+        store_out4(pp.out, pp.out_dtype, (int64_t)row * D + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
     }
   }
-  if (n > 0 && g == 0) {
+  pdl_launch_dependents();  // the balanced kernel of the next step wants its SMs free: only now
+}
+
+// Few rows of many partials: a CTA per 32 dims of a row, 32 groups of 8 threads over the partials.
+template <int D>
+__global__ void __launch_bounds__(256) paged_merge_long_kernel(const PagedParams pp) {
+  constexpr int kAtOnce = 256, PER = kAtOnce / 32;  // partials in flight, of a thread
+  __shared__ float s_w[kAtOnce], s_red[8], s_sum[8];
+  __shared__ float4 s_acc[8][8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x;
+  const int g = tid >> 3, d = blockIdx.y * 32 + (tid & 7) * 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int2 at = paged_partials(pp, row);
+  const int n = at.y;
+  if (n == 0) return;
+  const float* acc = pp.acc + (int64_t)at.x * D + d;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L = 0.f, M = -INFINITY;
+  for (int s0 = 0; s0 < n; s0 += kAtOnce) {
+    float4 x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int s = s0 + i * 32 + g;
+      x[i] = s < n ? __ldcg(reinterpret_cast<const float4*>(acc + (int64_t)s * (kHeadsPerCta * D))) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const float m = s0 + tid < n ? __ldcg(pp.m + at.x + (s0 + tid) * kHeadsPerCta) : -INFINITY;
+    const float l = s0 + tid < n ? __ldcg(pp.l + at.x + (s0 + tid) * kHeadsPerCta) : 0.f;
+    const float mw = warp_max(m);
+    if (lane == 0) s_red[warp] = mw;
+    __syncthreads();
+    float top = M;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_red[w]);
+    const float w = m > -INFINITY ? ex2(m - top) : 0.f;
+    s_w[tid] = w;
+    const float old = M > -INFINITY ? ex2(M - top) : 0.f;  // (more than kAtOnce partials: a running maximum)
+    L = fmaf(L, old, w * l);
+    a.x *= old;
+    a.y *= old;
+    a.z *= old;
+    a.w *= old;
+    M = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) fma4(a, s_w[i * 32 + g], x[i]);
+  }
+  L = warp_sum(L);
+#pragma unroll
+  for (int off = 8; off <= 16; off <<= 1) {  // the 4 groups of a warp
+    a.x += __shfl_xor_sync(kFullMask, a.x, off);
+    a.y += __shfl_xor_sync(kFullMask, a.y, off);
+    a.z += __shfl_xor_sync(kFullMask, a.z, off);
+    a.w += __shfl_xor_sync(kFullMask, a.w, off);
+  }
+  if (lane < 8) s_acc[warp][lane] = a;
+  if (lane == 0) s_sum[warp] = L;
+  __syncthreads();
+  if (tid < 8) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      fma4(a, 1.f, s_acc[w][tid]);
+      L += s_sum[w];
+    }
+    L = __shfl_sync(0xffu, L, 0);
     const float inv = L > 0.f ? 1.f / L : 0.f;
     store_out4(pp.out, pp.out_dtype, (int64_t)row * D + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
   }
-  if (GROUPS == 1) pdl_launch_dependents();  // the balanced kernel of the next step wants its SMs free
 }
 
 // ------------------------------------------------------------------ host side
@@ -542,14 +648,10 @@ struct PagedLaunch {
       TKV_CUDA(launch_pdl(paged_split_kernel<Policy>, dim3(w), dim3(Policy::WARPS * 32), (size_t)smem_bytes(n), stream,
                           maps, pp));
       const int rows = n * pp.d.HQ;
-      if (rows < kSmallCombineMinRows) {
-        constexpr int GROUPS = 256 / (Policy::D / 4);
-        TKV_CUDA(launch_pdl(paged_merge_kernel<Policy::D, GROUPS>, dim3(rows), dim3(256), 0, stream, pp, rows));
-      } else {
-        constexpr int RPC = 256 / (Policy::D / 4);
-        TKV_CUDA(launch_pdl(paged_merge_kernel<Policy::D, 1>, dim3((rows + RPC - 1) / RPC), dim3(256), 0, stream, pp,
-                            rows));
-      }
+      if (rows < kSmallCombineMinRows)
+        TKV_CUDA(launch_pdl(paged_merge_long_kernel<Policy::D>, dim3(rows, Policy::D / 32), dim3(256), 0, stream, pp));
+      else
+        TKV_CUDA(launch_pdl(paged_merge_rows_kernel<Policy::D>, dim3((rows + 7) / 8), dim3(256), 0, stream, pp, rows));
     }
     return TKV_OK;
   }
@@ -680,6 +782,8 @@ static int paged_fill(const char* who, PagedCall& c, const void* q, int q_dtype,
   pp.dpage = make_fastdiv(page);
   pp.dHch = make_fastdiv(p.hchunks);
   pp.dHKVc = make_fastdiv(pp.HKVc);
+  pp.dHQ = make_fastdiv(HQ);
+  pp.dgroup = make_fastdiv(p.group);
   return TKV_OK;
 }
 
