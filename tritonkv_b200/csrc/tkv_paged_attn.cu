@@ -53,6 +53,10 @@ __device__ __forceinline__ void store_out4(void* out, int dtype, int64_t i, floa
   }
 }
 
+// What all lanes of a warp hold, said so that the compiler sees it: ring slots, cursor and barrier
+// arithmetic that hangs off it can then go to the uniform datapath.
+__device__ __forceinline__ int warp_uniform(int x) { return __shfl_sync(kFullMask, x, 0); }
+
 // The part of a unit that a CTA processes.  `pref` is the prefix of tiles per sequence, see the kernel.
 struct PagedSegment {
   int b, hk;        // sequence; KV head and head chunk
@@ -63,8 +67,8 @@ struct PagedSegment {
 
 template <int kTok>
 __device__ __forceinline__ void paged_segment_of(PagedSegment& s, const int* pref, int g, int g1) {
-  const int word = pref[s.b];
-  s.t_b = (pref[s.b + 1] >> kRemBits) - (word >> kRemBits);
+  const int word = warp_uniform(pref[s.b]);
+  s.t_b = warp_uniform(pref[s.b + 1] >> kRemBits) - (word >> kRemBits);
   s.hi = (s.t_b - 1) * kTok + (word & ((1 << kRemBits) - 1)) + 1;
   s.ntiles = min(g1 - g, s.t_b - s.lo_tile);
   s.g_end = g + s.ntiles;
@@ -78,7 +82,9 @@ __device__ __forceinline__ PagedSegment paged_segment_at(const int* pref, int B,
     const int mid = (lo + hi) >> 1;
     if (HKVc * (pref[mid] >> kRemBits) <= g) lo = mid; else hi = mid;
   }
-  const int before = pref[lo] >> kRemBits, t_b = (pref[lo + 1] >> kRemBits) - before, r = g - HKVc * before;
+  lo = warp_uniform(lo);
+  const int before = warp_uniform(pref[lo] >> kRemBits), t_b = warp_uniform(pref[lo + 1] >> kRemBits) - before;
+  const int r = g - HKVc * before;
   s.b = lo;
   s.hk = (int)((uint32_t)r / (uint32_t)t_b);
   s.lo_tile = r - s.hk * t_b;
@@ -92,7 +98,7 @@ __device__ __forceinline__ void paged_segment_next(PagedSegment& s, const int* p
   if (++s.hk == HKVc) {
     s.hk = 0;
     do ++s.b;
-    while ((pref[s.b + 1] >> kRemBits) == (pref[s.b] >> kRemBits));
+    while (warp_uniform(pref[s.b + 1] >> kRemBits) == warp_uniform(pref[s.b] >> kRemBits));
     paged_segment_of<kTok>(s, pref, s.g_end, g1);
   } else {
     s.ntiles = min(g1 - s.g_end, s.t_b);
@@ -100,15 +106,17 @@ __device__ __forceinline__ void paged_segment_next(PagedSegment& s, const int* p
   }
 }
 
-// Where a warp's copies stand: the next tile to issue, segments ahead of the one being computed.
-template <int PIECES>
+// Where a warp's copies stand, segments ahead of the one being computed.  Kept in shared memory: only
+// the look-up of the next 32 tiles needs it.
 struct PagedCursor {
   PagedSegment seg;
-  int tok;           // first token of the next tile
-  int cnt;           // tiles left in the cursor's segment
-  int k;             // which lane's row the next tile takes
-  int row[PIECES];   // this lane's: pool rows of tile `lane` of the present 32, or -1
+  int tile;  // the warp's next tile, within the segment
 };
+// A tile's place as one word: (pool row / 16) << 5 | tokens - 1, or all ones where it has none.
+constexpr uint32_t kNoPlace = 0xffffffffu;
+__device__ __forceinline__ uint32_t place_word(int row, int tokens) {
+  return ((uint32_t)row >> 4) << 5 | (uint32_t)(tokens - 1);
+}
 
 template <class Policy>
 __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
@@ -126,6 +134,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   __shared__ float s_m[WARPS][kHeadsPerCta];
   __shared__ float s_l[WARPS][kHeadsPerCta];
   __shared__ int s_slot[WARPS];
+  __shared__ PagedCursor s_cursor[WARPS];
   const int warp = __shfl_sync(kFullMask, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
   pdl_launch_dependents();  // the whole grid is resident: the merge may take its place and wait
@@ -193,7 +202,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     if (lane == 0) s_pref[p.B] = carry << kRemBits;
   }
   __syncthreads();
-  const int T = pp.HKVc * (s_pref[p.B] >> kRemBits);
+  const int T = pp.HKVc * warp_uniform(s_pref[p.B] >> kRemBits);
   int TC = max(1, (T + (int)gridDim.x - 1) / (int)gridDim.x);
   if (TC <= 4 * WARPS) TC = (TC + WARPS - 1) / WARPS * WARPS;  // no warp without a tile: fewer partials, same time
   const int g0 = min(cta * TC, T), g1 = min(g0 + TC, T);
@@ -217,61 +226,67 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   }
   PagedSegment seg = paged_segment_at<kTok>(s_pref, p.B, pp.HKVc, g0, g1);
 
-  // ---- issue cursor ----
-  PagedCursor<PIECES> cur;
-  cur.seg = seg;
-  auto look_up = [&]() {  // lane i: the rows of this warp's i-th tile from the cursor on
-    cur.k = 0;
-    const int tok = cur.tok + lane * (WARPS * kTok), hkv = fast_div(cur.seg.hk, pp.dHch);
+  // ---- the warp's next 32 tiles, across segments: lane i has the place of the i-th ----
+  PagedCursor* my_cursor = &s_cursor[warp];
+  if (lane == 0) *my_cursor = PagedCursor{seg, warp};
+  uint32_t place[PIECES];
+  int k_next = 0, n_listed = 0;  // the tile to issue next, and how many there are
+  auto look_up = [&]() {
+    __syncwarp();
+    PagedCursor cur = *my_cursor;
+    k_next = n_listed = 0;
 #pragma unroll
-    for (int h = 0; h < PIECES; ++h) {
-      const int n = tok + h * (kTok / PIECES);
-      int row = -1;
-      if (lane < cur.cnt && n < cur.seg.hi) {
-        const int i = fast_div(n, pp.dpage), id = __ldcg(pp.table + cur.seg.b * pp.table_stride + i);
-        if ((unsigned)id < (unsigned)pp.num_pages) row = (id * p.HKV + hkv) * pp.page + (n - i * pp.page);
+    for (int h = 0; h < PIECES; ++h) place[h] = kNoPlace;
+    for (;;) {
+      const int cnt = cur.seg.ntiles > cur.tile ? (cur.seg.ntiles - cur.tile + WARPS - 1) / WARPS : 0;
+      const int take = min(cnt, 32 - n_listed), i = lane - n_listed;
+      if (i >= 0 && i < take) {
+        const int tok = (cur.seg.lo_tile + cur.tile + i * WARPS) * kTok, hkv = fast_div(cur.seg.hk, pp.dHch);
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h) {
+          const int n = tok + h * (kTok / PIECES);
+          if (n < cur.seg.hi) {
+            const int e = fast_div(n, pp.dpage), id = __ldcg(pp.table + cur.seg.b * pp.table_stride + e);
+            if ((unsigned)id < (unsigned)pp.num_pages)
+              place[h] = place_word((id * p.HKV + hkv) * pp.page + (n - e * pp.page), min(kTok, cur.seg.hi - tok));
+          }
+        }
       }
-      cur.row[h] = row;
-    }
-  };
-  auto cursor_enter = [&]() {
-    cur.tok = (cur.seg.lo_tile + warp) * kTok;
-    cur.cnt = cur.seg.ntiles > warp ? (cur.seg.ntiles - warp + WARPS - 1) / WARPS : 0;
-    if (cur.cnt > 0) look_up();
-  };
-  auto cursor_skip_empty = [&]() {  // to the next segment in which this warp has a tile
-    while (cur.cnt == 0 && cur.seg.g_end < g1) {
+      n_listed += take;
+      cur.tile += take * WARPS;
+      if (n_listed == 32 || cur.seg.g_end >= g1) break;
       paged_segment_next<kTok>(cur.seg, s_pref, pp.HKVc, g1);
-      cursor_enter();
+      cur.tile = warp;
     }
+    __syncwarp();
+    if (lane == 0) *my_cursor = cur;
   };
-  cursor_enter();
-  cursor_skip_empty();
+  look_up();
   int iss_slot = 0;          // slot the next issue fills
   uint32_t valid = 0;        // bits [s*PIECES, (s+1)*PIECES): which pieces of slot s name a page
   constexpr uint32_t kAll = (1u << PIECES) - 1u;
   bool need_proxy_fence = false;
   auto issue_next = [&]() {
-    if (cur.cnt == 0) return;
+    if (k_next >= n_listed) return;
     const int slot = iss_slot;
     iss_slot = (slot + 1 == STAGES) ? 0 : slot + 1;
     if (need_proxy_fence) {  // a generic-proxy epilogue touched the ring since the last issue
       fence_proxy_async();
       need_proxy_fence = false;
     }
-    int rows[PIECES];
+    int rows[PIECES], tokens = kTok;
     uint32_t ok = 0;
 #pragma unroll
     for (int h = 0; h < PIECES; ++h) {
-      rows[h] = __shfl_sync(kFullMask, cur.row[h], cur.k);
-      ok |= (rows[h] >= 0 ? 1u : 0u) << h;
+      const uint32_t w = __shfl_sync(kFullMask, place[h], k_next);
+      const bool there = w != kNoPlace;
+      rows[h] = there ? (int)(w >> 5 << 4) : -1;
+      if (there) tokens = (int)(w & 31u) + 1;
+      ok |= (there ? 1u : 0u) << h;
     }
     valid = (valid & ~(kAll << (slot * PIECES))) | (ok << (slot * PIECES));
-    Policy::issue_pieces(ist, p, maps, rows, min(kTok, cur.seg.hi - cur.tok), ring_u32 + slot * STAGE_BYTES,
-                         bar_u32 + 8 * slot, lane);
-    cur.tok += WARPS * kTok;
-    if (--cur.cnt == 0) cursor_skip_empty();
-    else if (++cur.k == 32) look_up();
+    Policy::issue_pieces(ist, p, maps, rows, tokens, ring_u32 + slot * STAGE_BYTES, bar_u32 + 8 * slot, lane);
+    if (++k_next == 32) look_up();
   };
   prefetch_q(0, seg);
 #pragma unroll 1
