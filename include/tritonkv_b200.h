@@ -264,7 +264,8 @@ int tkv_paged_append(const void* k, const void* v, int in_dtype, const int64_t* 
                      void* stream);
 
 /* 32-bit words of device workspace that tkv_pages_fork (B rows of the new table) and
- * tkv_pages_compact need.  Calls that may run at the same time need workspaces of their own. */
+ * tkv_pages_compact need.  It is zero before its first use, serves one num_pages (its first words
+ * are left zero by every call), and calls that may run at the same time need one each. */
 int tkv_pages_workspace(int B, int num_pages, int64_t* words);
 
 /* New table (B, max_pages) and lengths (B,) whose row b continues row parents[b] of the old ones

@@ -339,6 +339,21 @@ def test_compact_into_given_tensors_and_empty():
     assert t.shape == (3, 0) and n.tolist() == [0]
 
 
+def test_one_workspace_for_many_calls():
+    """Forks and compactions of different sizes and pools in turn with one workspace."""
+    ws = {}
+    for i in range(12):
+        NP, B, W, page = [(70, 9, 6, 16), (500, 40, 9, 32), (33, 3, 4, 16)][i % 3]
+        pools = [random_pool(NP, 1, page, 64, 4, 32, i)]
+        table, lens = random_table(B, W, NP, page, i)
+        parents = [(j * 5 + i) % (B + 1) - 1 for j in range(B)]
+        want = walk_fork(table, lens, parents, [3] * B, NP, page)
+        t, n, miss = fork_pages(pools, ints(table), ints(lens), ints(parents), reserve=3, _workspace=ws)
+        assert (t.tolist(), n.tolist(), miss.tolist()) == (want[0], want[1], [want[2]])
+        c, live = compact_pages(pools, t, _workspace=ws)
+        assert (c.tolist(), live.tolist()) == (walk_compact(t.tolist(), NP)[0], [walk_compact(t.tolist(), NP)[1]])
+
+
 # ------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("nbits", [2, 4, 16])
 @pytest.mark.parametrize("captured", [False, True])

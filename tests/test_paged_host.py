@@ -169,5 +169,5 @@ def test_c_entries_refuse():
     def compact(B=2, W=4, NP=8, live=P, n=1):
         return lib.tkv_pages_compact(P, W, B, W, NP, P, live, P, ptrs, sizes, n, None)
 
-    for kw in (dict(B=1 << 16), dict(NP=0), dict(live=None), dict(W=1 << 29), dict(n=-1)):
+    for kw in (dict(B=-1), dict(NP=0), dict(live=None), dict(W=1 << 29), dict(n=-1)):
         assert compact(**kw) == I, (kw, _cabi.last_error())

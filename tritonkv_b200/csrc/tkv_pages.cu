@@ -12,77 +12,74 @@
 //
 // Compaction.  With n pages in use, the k-th used page at or above n moves to the k-th unused page
 // below n.  Pages are only read above n and only written below, so the old table stays valid.
+//
+// Each is two launches.  The first reads the table -- a bit per used page -- and its last CTA to finish
+// (a ticket) ranks and lists what has to be done: everything in order of rows or pages, so the outcome does
+// not depend on which CTA that is.  The second, a programmatic dependent, does it: table entries, and
+// the copies cut into slices of 16 KB.  The bitmap and the ticket are left zero for the next call.
 #include "tkv_common.cuh"
 
 namespace tkv {
 
-constexpr int kMaxPoolTensors = 24;
+constexpr int kMaxPoolTensors = 24;  // of one launch
+constexpr int kSlice = 16384;        // bytes that a CTA copies at a time
+constexpr int kPlanThreads = 1024;
 
 struct PoolTensors {
   uint8_t* base[kMaxPoolTensors];
   int64_t page_bytes[kMaxPoolTensors];
-  int n;
+  int first[kMaxPoolTensors];  // slices of the tensors before
+  int n, slices;               // tensors; slices of one page of all of them
+  int wide;                    // every page is 16-byte aligned in all of them
 };
 
-struct ForkArgs {
-  const int32_t *table, *lens, *parents, *reserve;
-  int32_t *new_table, *new_lens, *missing;
-  uint32_t* used;        // bit i of word w: page 32 w + i is named by a kept entry
-  int32_t *src, *dst;    // (B) page copies, -1 for none
-  int32_t* start;        // (B) fresh pages of the rows before
-  int32_t* fresh;        // (num_pages) unused pages, lowest first
-  int64_t table_stride;
-  int reserve0, B_old, B, num_pages, page, W;
-};
+// One CTA: copy slice `slice` of page `s` to page `d`.
+__device__ __forceinline__ void copy_slice(const PoolTensors& t, int slice, int s, int d) {
+  int i = 0;
+  while (i + 1 < t.n && slice >= t.first[i + 1]) ++i;
+  const int64_t at = (int64_t)(slice - t.first[i]) * kSlice, bytes = t.page_bytes[i];
+  const int len = (int)min((int64_t)kSlice, bytes - at);
+  const uint8_t* from = t.base[i] + s * bytes + at;
+  uint8_t* to = t.base[i] + d * bytes + at;
+  if (t.wide) {
+    constexpr int PER = kSlice / (256 * 16);
+    uint4 v[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int o = (k * 256 + threadIdx.x) * 16;
+      if (o < len) v[k] = __ldcs(reinterpret_cast<const uint4*>(from + o));
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int o = (k * 256 + threadIdx.x) * 16;
+      if (o < len) *reinterpret_cast<uint4*>(to + o) = v[k];
+    }
+  } else {
+    for (int o = threadIdx.x; o < len; o += 256) to[o] = from[o];
+  }
+}
 
 __device__ __forceinline__ bool page_ok(int id, int num_pages) { return (unsigned)id < (unsigned)num_pages; }
 
-struct ForkRow {
-  int n, full, held, want;  // tokens; pages filled, touched, and touched with the reserve
-};
-__device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int b, int n) {
-  ForkRow r;
-  r.n = n;
-  r.full = n / a.page;
-  r.held = (int)(((int64_t)n + a.page - 1) / a.page);
-  const int64_t more = max(a.reserve ? a.reserve[b] : a.reserve0, 0);
-  r.want = (int)min((int64_t)a.W, (n + more + a.page - 1) / a.page);
-  return r;
+__device__ __forceinline__ uint32_t word_mask(int w, int num_pages) {  // bits of word w that are pages
+  const int left = num_pages - w * 32;
+  return left >= 32 ? 0xffffffffu : (1u << left) - 1u;
 }
 
-// One CTA per new row: entries that stay, and what the row needs besides.
-__global__ void __launch_bounds__(128) fork_mark_kernel(const ForkArgs a) {
-  const int b = blockIdx.x, tid = threadIdx.x, par = a.parents[b];
-  int32_t* row = a.new_table + (int64_t)b * a.W;
-  const bool live = par >= 0 && par < a.B_old;
-  bool elder = false;
-  if (live)
-    for (int i = tid; i < b; i += 128) elder |= a.parents[i] == par;
-  const bool first = !__syncthreads_or(elder);
-  const int n = live ? (int)min((int64_t)max(a.lens[par], 0), (int64_t)a.W * a.page) : 0;
-  const ForkRow r = fork_row(a, b, n);
-  const int32_t* old = a.table + (live ? par : 0) * a.table_stride;
-  const int keep = live ? (first ? r.held : r.full) : 0;
-  for (int i = tid; i < a.W; i += 128) {
-    int id = -1;
-    if (i < keep) {
-      id = old[i];
-      if (!page_ok(id, a.num_pages)) id = -1;
-      else atomicOr(a.used + (id >> 5), 1u << (id & 31));
-    }
-    row[i] = id;
-  }
-  if (tid == 0) {
-    const bool copy = live && r.held > r.full && !first && page_ok(old[r.full], a.num_pages);
-    a.src[b] = copy ? old[r.full] : -1;
-    a.dst[b] = -1;
-    a.new_lens[b] = n;
-    a.start[b] = live ? (copy ? 1 : 0) + max(0, r.want - r.held) : 0;
-  }
+// Whether this CTA is the last of the grid to come here; what the others wrote before is then visible.
+__device__ __forceinline__ bool last_cta(uint32_t* ticket) {
+  __shared__ bool s_last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (s_last) __threadfence();
+  return s_last;
 }
 
-// Exclusive prefix sum over the CTA's 1024 threads; `total` is the sum.
-__device__ __forceinline__ int block_scan(int x, int* s_warp, int& total) {
+// Exclusive prefix sum over the CTA's kPlanThreads threads; `total` is the sum.
+__device__ __forceinline__ int block_scan(int x, int& total) {
+  __shared__ int s_warp[kPlanThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int incl = x;
 #pragma unroll
@@ -103,83 +100,142 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int& total) {
     s_warp[lane] = w;
   }
   __syncthreads();
-  total = s_warp[31];
+  total = s_warp[kPlanThreads / 32 - 1];
   return incl - x + (warp > 0 ? s_warp[warp - 1] : 0);
 }
 
-__device__ __forceinline__ uint32_t word_mask(int w, int num_pages) {  // bits of word w that are pages
-  const int left = num_pages - w * 32;
-  return left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+// ------------------------------------------------------------------ fork
+struct ForkArgs {
+  const int32_t *table, *lens, *parents, *reserve;
+  int32_t *new_table, *new_lens, *missing;
+  uint32_t *ticket, *used;  // bit i of used[w]: page 32 w + i is named by a kept entry
+  int32_t* listed;       // fresh pages that are there
+  int32_t* src;          // (B) page that the row copies, or -1
+  int32_t* start;        // (B) fresh pages of the rows before
+  int32_t* fresh;        // (num_pages) unused pages, lowest first
+  int64_t table_stride;
+  int reserve0, B_old, B, num_pages, page, W;
+};
+
+struct ForkRow {
+  int full, held, want;  // pages that are filled, touched, and touched with the reserve
+};
+__device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int b, int n) {
+  ForkRow r;
+  r.full = n / a.page;
+  r.held = r.full + (n - r.full * a.page > 0 ? 1 : 0);
+  const int64_t more = max(a.reserve ? a.reserve[b] : a.reserve0, 0);
+  r.want = (int)min((int64_t)a.W, (n + more + a.page - 1) / a.page);
+  return r;
 }
 
-// One CTA: rank the rows' needs, list the lowest unused pages, hand them out.
-__global__ void __launch_bounds__(1024) fork_assign_kernel(const ForkArgs a) {
-  __shared__ int s_warp[32];
-  const int tid = threadIdx.x, words = (a.num_pages + 31) / 32;
-  int need = 0, total;
-  for (int b0 = 0; b0 < a.B; b0 += 1024) {
-    const int b = b0 + tid, x = b < a.B ? a.start[b] : 0;
-    const int before = block_scan(x, s_warp, total);
+// A warp per new row: entries that stay, and what the row needs besides.  Then, in the last CTA: rank the
+// rows' needs and list the lowest unused pages.
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkArgs a) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  pdl_launch_dependents();
+  for (int b = blockIdx.x * (kPlanThreads / 32) + (tid >> 5); b < a.B; b += gridDim.x * (kPlanThreads / 32)) {
+    const int par = a.parents[b];
+    int32_t* row = a.new_table + (int64_t)b * a.W;
+    const bool live = par >= 0 && par < a.B_old;
+    bool elder = false;
+    if (live)
+      for (int i = lane; i < b; i += 32) elder |= a.parents[i] == par;
+    const bool first = !__any_sync(kFullMask, elder);
+    const int n = live ? (int)min((int64_t)max(a.lens[par], 0), (int64_t)a.W * a.page) : 0;
+    const ForkRow r = fork_row(a, b, n);
+    const int32_t* old = a.table + (live ? par : 0) * a.table_stride;
+    const int keep = live ? (first ? r.held : r.full) : 0;
+    for (int i = lane; i < a.W; i += 32) {
+      int id = -1;
+      if (i < keep) {
+        id = old[i];
+        if (!page_ok(id, a.num_pages)) id = -1;
+        else atomicOr(a.used + (id >> 5), 1u << (id & 31));
+      }
+      row[i] = id;
+    }
+    if (lane == 0) {
+      const bool copy = live && r.held > r.full && !first && page_ok(old[r.full], a.num_pages);
+      a.src[b] = copy ? old[r.full] : -1;
+      a.new_lens[b] = n;
+      a.start[b] = live ? (copy ? 1 : 0) + max(0, r.want - r.held) : 0;
+    }
+  }
+  if (!last_cta(a.ticket)) return;
+  int need = 0, have = 0, total;
+  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+    const int b = b0 + tid, x = b < a.B ? __ldcg(a.start + b) : 0;
+    const int before = block_scan(x, total);
     if (b < a.B) a.start[b] = need + before;
     need += total;
   }
-  int have = 0;
-  for (int w0 = 0; w0 < words && have < need; w0 += 1024) {
+  const int words = (a.num_pages + 31) / 32;
+  for (int w0 = 0; w0 < words; w0 += kPlanThreads) {
     const int w = w0 + tid;
-    uint32_t free = w < words ? ~a.used[w] & word_mask(w, a.num_pages) : 0u;
-    int rank = have + block_scan(__popc(free), s_warp, total);
+    uint32_t free = 0;
+    if (w < words) {
+      free = ~__ldcg(a.used + w) & word_mask(w, a.num_pages);
+      a.used[w] = 0;
+    }
+    if (have >= need) continue;  // (the same for all threads) enough: the rest is only wiped
+    int rank = have + block_scan(__popc(free), total);
     for (; free && rank < need; free &= free - 1, ++rank) a.fresh[rank] = w * 32 + __ffs(free) - 1;
     have += total;
   }
-  if (tid == 0) *a.missing = max(0, need - have);
-  __syncthreads();
-  for (int b = tid >> 5; b < a.B; b += 32) {
-    const int par = a.parents[b];
-    if (par < 0 || par >= a.B_old) continue;
-    const ForkRow r = fork_row(a, b, a.new_lens[b]);
-    int32_t* row = a.new_table + (int64_t)b * a.W;
-    const int copy = a.src[b] >= 0 ? 1 : 0, count = copy + max(0, r.want - r.held), start = a.start[b];
-    for (int j = tid & 31; j < count; j += 32) {
-      const int id = start + j < have ? a.fresh[start + j] : -1;
-      if (j < copy) {
-        row[r.full] = id;
-        a.dst[b] = id;
-      } else {
-        row[r.held + j - copy] = id;
-      }
-    }
+  if (tid == 0) {
+    *a.listed = min(need, have);
+    *a.missing = max(0, need - have);
+    *a.ticket = 0;
   }
 }
 
+// CTA (row, part): fresh pages into the row's entries (part 0 of the first launch), and its slices of the copy.
+__global__ void __launch_bounds__(256) fork_apply_kernel(const ForkArgs a, const PoolTensors t, int entries) {
+  const int b = blockIdx.x;
+  pdl_wait();
+  const int src = __ldcg(a.src + b), start = __ldcg(a.start + b), listed = __ldcg(a.listed), par = a.parents[b];
+  if (entries && blockIdx.y == 0 && par >= 0 && par < a.B_old) {
+    const ForkRow r = fork_row(a, b, __ldcg(a.new_lens + b));
+    int32_t* row = a.new_table + (int64_t)b * a.W;
+    const int copy = src >= 0 ? 1 : 0, count = copy + max(0, r.want - r.held);
+    for (int j = threadIdx.x; j < count; j += 256)
+      row[j < copy ? r.full : r.held + j - copy] = start + j < listed ? __ldcg(a.fresh + start + j) : -1;
+  }
+  if (src < 0 || start >= listed) return;
+  const int dst = __ldcg(a.fresh + start);
+  for (int slice = blockIdx.y; slice < t.slices; slice += gridDim.y) copy_slice(t, slice, src, dst);
+}
+
+// ------------------------------------------------------------------ compact
 struct CompactArgs {
   const int32_t* table;
   int32_t *new_table, *live;
-  uint32_t* used;
+  uint32_t *ticket, *used;
+  int32_t* n_moves;
   int32_t* before;        // (words) used pages in the words before
   int32_t *src, *dst;     // moves
-  int32_t* n_moves;
+  int32_t* to;            // (num_pages) where page p >= live goes
   int64_t table_stride;
   int B, W, num_pages;
 };
 
-__global__ void __launch_bounds__(256) compact_mark_kernel(const CompactArgs a) {
-  const int b = blockIdx.y;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < a.W; i += gridDim.x * 256) {
-    const int id = a.table[b * a.table_stride + i];
-    if (page_ok(id, a.num_pages)) atomicOr(a.used + (id >> 5), 1u << (id & 31));
-  }
-}
-
-// One CTA: count the used pages, then list the moves.
-__global__ void __launch_bounds__(1024) compact_plan_kernel(const CompactArgs a) {
-  __shared__ int s_warp[32];
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const CompactArgs a) {
   __shared__ int s_below;
-  const int tid = threadIdx.x, words = (a.num_pages + 31) / 32;
+  const int tid = threadIdx.x, lane = tid & 31;
+  pdl_launch_dependents();
+  for (int b = blockIdx.x * (kPlanThreads / 32) + (tid >> 5); b < a.B; b += gridDim.x * (kPlanThreads / 32))
+    for (int i = lane; i < a.W; i += 32) {
+      const int id = a.table[b * a.table_stride + i];
+      if (page_ok(id, a.num_pages)) atomicOr(a.used + (id >> 5), 1u << (id & 31));
+    }
+  if (!last_cta(a.ticket)) return;
+  const int words = (a.num_pages + 31) / 32;
   int live = 0, total;
-  for (int w0 = 0; w0 < words; w0 += 1024) {
+  for (int w0 = 0; w0 < words; w0 += kPlanThreads) {
     const int w = w0 + tid;
-    const int x = w < words ? __popc(a.used[w]) : 0;
-    const int before = block_scan(x, s_warp, total);
+    const int x = w < words ? __popc(__ldcg(a.used + w)) : 0;
+    const int before = block_scan(x, total);
     if (w < words) a.before[w] = live + before;
     live += total;
   }
@@ -188,83 +244,77 @@ __global__ void __launch_bounds__(1024) compact_plan_kernel(const CompactArgs a)
     int below = live;
     if (live < a.num_pages) {
       const int w = live >> 5;
-      below = a.before[w] + __popc(a.used[w] & ((1u << (live & 31)) - 1u));
+      below = a.before[w] + __popc(__ldcg(a.used + w) & ((1u << (live & 31)) - 1u));
     }
     s_below = below;
     *a.live = live;
     *a.n_moves = live - below;
+    *a.ticket = 0;
   }
   __syncthreads();
   const int below = s_below;
-  for (int w = tid; w < words; w += 1024) {
-    const uint32_t used = a.used[w], mask = word_mask(w, a.num_pages);
-    const int p0 = w * 32, before = a.before[w];
-    for (uint32_t m = mask; m; m &= m - 1) {
-      const int i = __ffs(m) - 1, p = p0 + i, u = before + __popc(used & ((1u << i) - 1u));
-      if ((used >> i) & 1u) {
-        if (p >= live) a.src[u - below] = p;
-      } else if (p < live) {
-        a.dst[p - u] = p;
-      }
+  for (int w = tid >> 5; w < words; w += kPlanThreads / 32) {  // a lane per page: its rank says where it goes
+    const uint32_t used = __ldcg(a.used + w);
+    const int p = w * 32 + lane, u = a.before[w] + __popc(used & ((1u << lane) - 1u));
+    if ((used >> lane) & 1u) {
+      if (p >= live) a.src[u - below] = p;
+    } else if (p < live) {
+      a.dst[p - u] = p;
     }
+    __syncwarp();
+    if (lane == 0) a.used[w] = 0;
+  }
+  __syncthreads();
+  const int moves = live - below;
+  for (int i = tid; i < moves; i += kPlanThreads) a.to[a.src[i]] = a.dst[i];
+}
+
+__global__ void __launch_bounds__(256) compact_apply_kernel(const CompactArgs a, const PoolTensors t, int entries) {
+  pdl_wait();
+  const int live = __ldcg(a.live), moves = __ldcg(a.n_moves);
+  if (entries) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)a.B * a.W; i += (int64_t)gridDim.x * 256) {
+      const int b = (int)(i / a.W);
+      int id = a.table[b * a.table_stride + (i - (int64_t)b * a.W)];
+      if (!page_ok(id, a.num_pages)) id = -1;
+      else if (id >= live) id = __ldcg(a.to + id);
+      a.new_table[i] = id;
+    }
+  }
+  const int64_t items = (int64_t)moves * t.slices;
+  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const int m = (int)(i / t.slices);
+    copy_slice(t, (int)(i - (int64_t)m * t.slices), __ldcg(a.src + m), __ldcg(a.dst + m));
   }
 }
 
-__global__ void __launch_bounds__(256) compact_table_kernel(const CompactArgs a) {
-  const int b = blockIdx.y, live = *a.live, below = live - *a.n_moves;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < a.W; i += gridDim.x * 256) {
-    int id = a.table[b * a.table_stride + i];
-    if (!page_ok(id, a.num_pages)) id = -1;
-    else if (id >= live) {
-      const int w = id >> 5;
-      id = a.dst[a.before[w] + __popc(a.used[w] & ((1u << (id & 31)) - 1u)) - below];
-    }
-    a.new_table[(int64_t)b * a.W + i] = id;
-  }
-}
-
-// Copy page src[i] to dst[i] in every tensor, i < (count ? *count : n); a negative entry is none.
-__global__ void __launch_bounds__(256)
-    copy_pages_kernel(const PoolTensors t, const int32_t* __restrict__ src, const int32_t* __restrict__ dst,
-                      const int32_t* __restrict__ count, int n) {
-  const int pairs = count ? *count : n;
-  for (int i = blockIdx.x; i < pairs; i += gridDim.x) {
-    const int s = src[i], d = dst[i];
-    if (s < 0 || d < 0) continue;
-    const int64_t bytes = t.page_bytes[blockIdx.y];
-    const uint8_t* from = t.base[blockIdx.y] + s * bytes;
-    uint8_t* to = t.base[blockIdx.y] + d * bytes;
-    if (((bytes | reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to)) & 15) == 0) {
-      for (int64_t k = threadIdx.x * 16; k < bytes; k += 256 * 16)
-        *reinterpret_cast<uint4*>(to + k) = *reinterpret_cast<const uint4*>(from + k);
-    } else {
-      for (int64_t k = threadIdx.x; k < bytes; k += 256) to[k] = from[k];
-    }
-  }
-}
-
+// ------------------------------------------------------------------ host side
 static int check_pools(const char* who, void* const* pools, const int64_t* page_bytes, int n) {
   TKV_REQUIRE(n >= 0 && (n == 0 || (pools && page_bytes)), TKV_ERR_INVALID, "%s: bad list of %d pools", who, n);
   for (int i = 0; i < n; ++i)
-    TKV_REQUIRE(pools[i] && page_bytes[i] > 0, TKV_ERR_INVALID, "%s: bad pool tensor %d", who, i);
+    TKV_REQUIRE(pools[i] && page_bytes[i] > 0 && page_bytes[i] < (1LL << 40), TKV_ERR_INVALID, "%s: bad pool tensor %d",
+                who, i);
   return TKV_OK;
 }
 
-// The copies of all tensors, kMaxPoolTensors in a launch.
-static int launch_copy(void* const* pools, const int64_t* page_bytes, int n_pools, const int32_t* src,
-                       const int32_t* dst, const int32_t* count, int n, cudaStream_t stream) {
-  if (n == 0) return TKV_OK;
-  for (int i0 = 0; i0 < n_pools; i0 += kMaxPoolTensors) {
-    PoolTensors t{};
-    t.n = n_pools - i0 < kMaxPoolTensors ? n_pools - i0 : kMaxPoolTensors;
-    for (int i = 0; i < t.n; ++i) {
-      t.base[i] = static_cast<uint8_t*>(pools[i0 + i]);
-      t.page_bytes[i] = page_bytes[i0 + i];
-    }
-    copy_pages_kernel<<<dim3(n < 2048 ? n : 2048, t.n), 256, 0, stream>>>(t, src, dst, count, n);
-    TKV_CUDA(cudaGetLastError());
+// Tensors [i0, i0 + kMaxPoolTensors) of the list.
+static PoolTensors some_pools(void* const* pools, const int64_t* page_bytes, int n, int i0) {
+  PoolTensors t{};
+  t.n = n - i0 < kMaxPoolTensors ? n - i0 : kMaxPoolTensors;
+  t.wide = 1;
+  for (int i = 0; i < t.n; ++i) {
+    t.base[i] = static_cast<uint8_t*>(pools[i0 + i]);
+    t.page_bytes[i] = page_bytes[i0 + i];
+    t.first[i] = t.slices;
+    t.slices += (int)((t.page_bytes[i] + kSlice - 1) / kSlice);
+    if ((reinterpret_cast<uintptr_t>(t.base[i]) | (uintptr_t)t.page_bytes[i]) & 15) t.wide = 0;
   }
-  return TKV_OK;
+  return t;
+}
+
+static int plan_grid(int rows) {  // a warp per row, few CTAs: the last one waits for all
+  const int n = (rows + kPlanThreads / 32 - 1) / (kPlanThreads / 32);
+  return n < 1 ? 1 : n < 148 ? n : 148;
 }
 
 }  // namespace tkv
@@ -272,7 +322,7 @@ static int launch_copy(void* const* pools, const int64_t* page_bytes, int n_pool
 extern "C" int tkv_pages_workspace(int B, int num_pages, int64_t* words) {
   TKV_REQUIRE(words && B >= 0 && num_pages > 0, TKV_ERR_INVALID, "pages_workspace: bad sizes B=%d num_pages=%d", B,
               num_pages);
-  *words = 2LL * ((num_pages + 31) / 32) + 2LL * num_pages + 3LL * B + 4;
+  *words = 4 + 2LL * ((num_pages + 31) / 32) + 3LL * num_pages + 2LL * B;
   return TKV_OK;
 }
 
@@ -303,11 +353,12 @@ extern "C" int tkv_pages_fork(const int32_t* block_table, int64_t table_stride, 
   a.new_table = new_table;
   a.new_lens = new_lens;
   a.missing = missing;
-  a.used = (uint32_t*)workspace;
-  a.fresh = workspace + words;
+  a.ticket = (uint32_t*)workspace;  // [ticket, listed, -, -][bitmap][fresh][src][start]
+  a.listed = workspace + 1;
+  a.used = (uint32_t*)workspace + 4;
+  a.fresh = workspace + 4 + words;
   a.src = a.fresh + num_pages;
-  a.dst = a.src + B;
-  a.start = a.dst + B;
+  a.start = a.src + B;
   a.table_stride = table_stride;
   a.reserve0 = reserve0;
   a.B_old = B_old;
@@ -315,22 +366,25 @@ extern "C" int tkv_pages_fork(const int32_t* block_table, int64_t table_stride, 
   a.num_pages = num_pages;
   a.page = page_size;
   a.W = max_pages;
-  TKV_CUDA(cudaMemsetAsync(a.used, 0, (size_t)words * 4, s));
-  if (B > 0) {
-    fork_mark_kernel<<<B, 128, 0, s>>>(a);
-    TKV_CUDA(cudaGetLastError());
-  }
-  fork_assign_kernel<<<1, 1024, 0, s>>>(a);
+  fork_plan_kernel<<<plan_grid(B), kPlanThreads, 0, s>>>(a);
   TKV_CUDA(cudaGetLastError());
-  return launch_copy(pools, page_bytes, n_pools, a.src, a.dst, nullptr, B, s);
+  if (B == 0) return TKV_OK;
+  for (int i0 = 0; i0 == 0 || i0 < n_pools; i0 += kMaxPoolTensors) {
+    const PoolTensors t = some_pools(pools, page_bytes, n_pools, i0);
+    // CTAs of a row: about four waves in all where every row copies
+    int parts = (148 * 32 + B - 1) / B;
+    parts = parts < 1 ? 1 : parts > t.slices ? (t.slices > 0 ? t.slices : 1) : parts;
+    TKV_CUDA(launch_pdl(fork_apply_kernel, dim3(B, parts), dim3(256), 0, s, a, t, i0 == 0 ? 1 : 0));
+  }
+  return TKV_OK;
 }
 
 extern "C" int tkv_pages_compact(const int32_t* block_table, int64_t table_stride, int B, int max_pages,
                                  int num_pages, int32_t* new_table, int32_t* live, int32_t* workspace,
                                  void* const* pools, const int64_t* page_bytes, int n_pools, void* stream) {
   using namespace tkv;
-  TKV_REQUIRE(B >= 0 && B < 65536 && max_pages >= 0 && num_pages > 0, TKV_ERR_INVALID,
-              "compact: bad sizes B=%d (below 65536) max_pages=%d num_pages=%d", B, max_pages, num_pages);
+  TKV_REQUIRE(B >= 0 && max_pages >= 0 && num_pages > 0, TKV_ERR_INVALID,
+              "compact: bad sizes B=%d max_pages=%d num_pages=%d", B, max_pages, num_pages);
   TKV_REQUIRE((int64_t)B * max_pages < (1LL << 30), TKV_ERR_INVALID, "compact: a table of %d x %d entries is too large",
               B, max_pages);
   TKV_REQUIRE(live && workspace, TKV_ERR_INVALID, "compact: null pointer");
@@ -343,26 +397,22 @@ extern "C" int tkv_pages_compact(const int32_t* block_table, int64_t table_strid
   a.table = block_table;
   a.new_table = new_table;
   a.live = live;
-  a.used = (uint32_t*)workspace;
-  a.before = workspace + words;
+  a.ticket = (uint32_t*)workspace;  // [ticket, moves, -, -][bitmap][before][src][dst][to]
+  a.n_moves = workspace + 1;
+  a.used = (uint32_t*)workspace + 4;
+  a.before = workspace + 4 + words;
   a.src = a.before + words;
   a.dst = a.src + num_pages;
-  a.n_moves = a.dst + num_pages;
+  a.to = a.dst + num_pages;
   a.table_stride = table_stride;
   a.B = B;
   a.W = max_pages;
   a.num_pages = num_pages;
-  TKV_CUDA(cudaMemsetAsync(a.used, 0, (size_t)words * 4, s));
-  const dim3 grid((max_pages + 255) / 256, B);
-  if (B > 0 && max_pages > 0) {
-    compact_mark_kernel<<<grid, 256, 0, s>>>(a);
-    TKV_CUDA(cudaGetLastError());
-  }
-  compact_plan_kernel<<<1, 1024, 0, s>>>(a);
+  compact_plan_kernel<<<plan_grid(B), kPlanThreads, 0, s>>>(a);
   TKV_CUDA(cudaGetLastError());
-  if (B > 0 && max_pages > 0) {
-    compact_table_kernel<<<grid, 256, 0, s>>>(a);
-    TKV_CUDA(cudaGetLastError());
+  for (int i0 = 0; i0 == 0 || i0 < n_pools; i0 += kMaxPoolTensors) {
+    const PoolTensors t = some_pools(pools, page_bytes, n_pools, i0);
+    TKV_CUDA(launch_pdl(compact_apply_kernel, dim3(148 * 8), dim3(256), 0, s, a, t, i0 == 0 ? 1 : 0));
   }
-  return launch_copy(pools, page_bytes, n_pools, a.src, a.dst, a.n_moves, num_pages, s);
+  return TKV_OK;
 }

@@ -177,14 +177,23 @@ def _pool_list(pools) -> tuple[list[torch.Tensor], int, int, torch.device]:
     return ts, NP, page, ts[0].device
 
 
+_pages_words: dict = {}
+
+
 def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
-    n = ctypes.c_int64(0)
-    _cabi.check(_cabi.load().tkv_pages_workspace(B, NP, ctypes.byref(n)))
-    t = None if ws is None else ws.get("pages")
-    if t is None or t.numel() < n.value or t.device != dev:
-        t = torch.empty(n.value, dtype=torch.int32, device=dev)
+    """The plan's scratch, zero at first and kept in the caller's dict ``ws`` for one number of pages."""
+    need = _pages_words.get((B, NP))
+    if need is None:
+        n = ctypes.c_int64(0)
+        _cabi.check(_cabi.load().tkv_pages_workspace(B, NP, ctypes.byref(n)))
+        need = n.value
+        if len(_pages_words) < 4096:
+            _pages_words[(B, NP)] = need
+    kept, t = (None, None) if ws is None else ws.get("pages", (None, None))
+    if kept != NP or t.numel() < need or t.device != dev:
+        t = torch.zeros(need, dtype=torch.int32, device=dev)
         if ws is not None:
-            ws["pages"] = t
+            ws["pages"] = (NP, t)
     return t
 
 
