@@ -84,16 +84,16 @@ SIGNATURES = {
                                       c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int,
                                       c_int, c_int, c_int, c_float, c_void_p]),
     "tkv_paged_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
-    "tkv_paged_append": (c_int, [c_void_p, c_void_p, c_int, POINTER(c_int64), c_void_p, c_void_p, c_void_p,
-                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, POINTER(c_int64),
+    "tkv_paged_append": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                  c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
                                  c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "tkv_pages_workspace": (c_int, [c_int, c_int, POINTER(c_int64)]),
     "tkv_pages_fork": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
-                               c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, POINTER(c_void_p),
-                               POINTER(c_int64), c_int, c_void_p]),
+                               c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_int, c_void_p]),
     "tkv_pages_compact": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
-                                  POINTER(c_void_p), POINTER(c_int64), c_int, c_void_p]),
+                                  c_void_p, c_void_p, c_int, c_void_p]),
 }
 
 _lib = None

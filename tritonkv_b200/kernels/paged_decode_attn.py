@@ -19,17 +19,21 @@ from ._launch import q_for_kernel
 __all__ = ["paged_decode_attention", "paged_fp16_decode_attention"]
 
 
+_OUT = {torch.float32, torch.float16, torch.bfloat16}
+
+
 def _check(q, k, v, block_table, seq_lens, out):
     """Checked arguments shared by the two forms: (k tensors, v tensors, q, seq_lens, out, sizes)."""
     kt, vt = pool_tensors(k, "k"), pool_tensors(v, "v")
-    if len(kt) != len(vt) or any(a.shape != b.shape for a, b in zip(kt, vt)):
+    shape = kt[0].shape
+    if len(kt) != len(vt) or vt[0].shape != shape:
         raise ValueError("K and V pools must have the same shape")
     if q.dim() != 3:
         raise ValueError(f"q must be (B, HQ, head_dim), got {tuple(q.shape)}")
     B, HQ, D = q.shape
-    NP, HKV, page, _ = kt[0].shape
-    if D != (k.head_dim if len(kt) == 3 else kt[0].shape[3]):
-        raise ValueError(f"q {tuple(q.shape)} is incompatible with pools of {tuple(kt[0].shape)}")
+    NP, HKV, page, row = shape
+    if D != (k.head_dim if len(kt) == 3 else row):
+        raise ValueError(f"q {tuple(q.shape)} is incompatible with pools of {tuple(shape)}")
     if HKV == 0 or HQ == 0 or HQ % HKV != 0:
         raise ValueError(f"HQ={HQ} must be a multiple of HKV={HKV}")
     dev = q.device
@@ -39,8 +43,7 @@ def _check(q, k, v, block_table, seq_lens, out):
     seq_lens = check_lens(seq_lens, B, dev, "seq_lens")
     if out is None:
         out = torch.empty((B, HQ, D), device=dev, dtype=torch.float32)
-    elif (out.shape != (B, HQ, D) or out.device != dev or not out.is_contiguous()
-          or out.dtype not in (torch.float32, torch.float16, torch.bfloat16)):
+    elif out.shape != q.shape or out.dtype not in _OUT or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous float32, float16 or bfloat16 tensor of shape {(B, HQ, D)} on {dev}")
     return kt, vt, q_for_kernel(q), seq_lens, out, (B, HQ, HKV, NP, page, W, D), stride
 

@@ -21,69 +21,79 @@ whose caches are contiguous.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from . import _cabi
 from .quantize import QuantizedTensor, check_cache_tensors
 
-Pool = "QuantizedTensor | torch.Tensor"
+_U8, _F16, _I32 = torch.uint8, torch.float16, torch.int32
 
 
 def pool_tensors(pool, what: str) -> tuple[torch.Tensor, ...]:
     """The contiguous 4-D tensors of a pool; the kernels use them in place."""
     if isinstance(pool, QuantizedTensor):
-        t = (pool.packed, pool.scale, pool.zero)
-        check_cache_tensors(pool, what, pool.packed.device)
-        if pool.packed.dim() != 4 or t[1].shape[:3] != t[0].shape[:3] or t[2].shape != t[1].shape:
+        p, s, z = pool.packed, pool.scale, pool.zero
+        a, b = p.shape, s.shape
+        # a well-formed pool passes here; a decode step is a few microseconds, so no more is spent on it
+        if (len(a) == 4 and len(b) == 4 and p.dtype is _U8 and s.dtype is _F16 and z.dtype is _F16 and z.shape == b
+                and a[0] == b[0] and a[1] == b[1] and a[2] == b[2] and a[3] * 8 == pool.head_dim * pool.nbits
+                and b[3] * pool.group_size == pool.head_dim and p.is_contiguous() and s.is_contiguous()
+                and z.is_contiguous() and p.get_device() == s.get_device() == z.get_device()):
+            return p, s, z
+        check_cache_tensors(pool, what, p.device)
+        if len(a) != 4 or len(b) != 4 or b[:3] != a[:3] or z.shape != b:
             raise ValueError(f"{what}: a packed pool has packed (num_pages, HKV, page_size, bytes) and scale, zero "
-                             f"(num_pages, HKV, page_size, groups); got {[tuple(x.shape) for x in t]}")
-        if t[0].shape[3] * 8 != pool.head_dim * pool.nbits or t[1].shape[3] * pool.group_size != pool.head_dim:
-            raise ValueError(f"{what}: rows of {t[0].shape[3]} bytes and {t[1].shape[3]} groups are not those of "
-                             f"head_dim {pool.head_dim} at {pool.nbits} bits in groups of {pool.group_size}")
+                             f"(num_pages, HKV, page_size, groups); got {[tuple(x.shape) for x in (p, s, z)]}")
+        if a[3] * 8 != pool.head_dim * pool.nbits or b[3] * pool.group_size != pool.head_dim:
+            raise ValueError(f"{what}: rows of {a[3]} bytes and {b[3]} groups are not those of head_dim {pool.head_dim} "
+                             f"at {pool.nbits} bits in groups of {pool.group_size}")
     elif isinstance(pool, torch.Tensor):
-        t = (pool,)
-        if pool.dtype != torch.float16:
+        if pool.dtype is not _F16:
             raise TypeError(f"{what} must be a QuantizedTensor or a float16 tensor, got {pool.dtype}")
         if pool.dim() != 4:
             raise ValueError(f"{what}: a float16 pool is (num_pages, HKV, page_size, head_dim), got {tuple(pool.shape)}")
+        if pool.is_contiguous():
+            return (pool,)
     else:
         raise TypeError(f"{what} must be a QuantizedTensor or a float16 tensor, got {type(pool).__name__}")
-    for x in t:
-        if not x.is_contiguous():
-            raise ValueError(f"{what} must be contiguous: a pool is used in place")
-    return t
+    raise ValueError(f"{what} must be contiguous: a pool is used in place")
 
 
 def check_table(block_table: torch.Tensor, B: int | None, device) -> tuple[int, int]:
     """(entries per row, row stride) of an int32 table (B, max_pages) whose rows are contiguous."""
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != device:
+    shape = block_table.shape
+    if len(shape) != 2 or block_table.dtype is not _I32 or block_table.device != device:
         raise ValueError(f"block_table must be an int32 tensor (B, max_pages) on {device}")
-    if B is not None and block_table.shape[0] != B:
-        raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} sequences")
-    n = block_table.shape[1]
-    if n > 1 and block_table.stride(1) != 1:
+    if B is not None and shape[0] != B:
+        raise ValueError(f"block_table has {shape[0]} rows for {B} sequences")
+    stride = block_table.stride()
+    if shape[1] > 1 and stride[1] != 1:
         raise ValueError("block_table rows must be contiguous")
-    return n, block_table.stride(0)
+    return shape[1], stride[0]
 
 
 def check_lens(lens: torch.Tensor, B: int, device, what: str) -> torch.Tensor:
-    if lens.shape != (B,) or lens.dtype != torch.int32 or lens.device != device:
+    shape = lens.shape
+    if len(shape) != 1 or shape[0] != B or lens.dtype is not _I32 or lens.device != device:
         raise ValueError(f"{what} must be an int32 tensor of shape ({B},) on {device}")
-    return lens.contiguous()
+    return lens if lens.is_contiguous() else lens.contiguous()
 
 
-def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """x itself where its rows are contiguous and start on 16-byte boundaries, else a copy."""
-    al = 16 // x.element_size()
-    ok = x.stride(3) == 1 and x.data_ptr() % 16 == 0
-    for size, stride in zip(x.shape[:3], x.stride()[:3]):
-        ok = ok and (size == 1 or stride % al == 0)
-    return x if ok else x.clone(memory_format=torch.contiguous_format)
+def _row_strides(x: torch.Tensor) -> tuple | None:
+    """Strides of (B, HKV, T) of a 4-D tensor whose rows are contiguous and start on 16-byte boundaries."""
+    b, h, t, d = x.stride()
+    al = 16 // x.element_size() - 1
+    if not (b | h | t) & al and d == 1 and not x.data_ptr() & 15:
+        return b, h, t
+    if x.shape[3] > 1 and d != 1 or x.data_ptr() & 15:
+        return None
+    kept = tuple(s if n > 1 else 0 for n, s in zip(x.shape, (b, h, t)))  # (an axis of one has no stride)
+    return None if (kept[0] | kept[1] | kept[2]) & al else kept
 
 
-def _strides(x: torch.Tensor) -> list[int]:
-    return [s if n > 1 else 0 for n, s in zip(x.shape[:3], x.stride()[:3])]
+_PACK6 = struct.Struct("6q").pack
 
 
 def append_kv_paged(kq, vq, k_new: torch.Tensor, v_new: torch.Tensor, block_table: torch.Tensor, positions,
@@ -106,25 +116,27 @@ def append_kv_paged(kq, vq, k_new: torch.Tensor, v_new: torch.Tensor, block_tabl
     Two tokens that go to one place in the same call leave either of them there.
     Returns ``(kq, vq)``."""
     kt, vt = pool_tensors(kq, "kq"), pool_tensors(vq, "vq")
-    packed = isinstance(kq, QuantizedTensor)
-    if len(kt) != len(vt) or any(a.shape != b.shape for a, b in zip(kt, vt)):
+    packed = len(kt) == 3
+    if len(vt) != len(kt) or kt[0].shape != vt[0].shape:
         raise ValueError("K and V pools must have the same format and shape")
-    if packed and (kq.nbits, kq.group_size) != (vq.nbits, vq.group_size):
+    if packed and (kq.nbits != vq.nbits or kq.group_size != vq.group_size):
         raise ValueError("K and V must use the same nbits/group_size")
-    NP, HKV, page, _ = kt[0].shape
-    D = kq.head_dim if packed else kt[0].shape[3]
+    NP, HKV, page, D = kt[0].shape
+    if packed:
+        D = kq.head_dim
     dev = kt[0].device
-    if k_new.dim() != 4 or k_new.shape != v_new.shape:
-        raise ValueError(f"k_new and v_new must both be (B, HKV, T, head_dim), got {tuple(k_new.shape)} and {tuple(v_new.shape)}")
-    B, H, T, Dn = k_new.shape
-    if (H, Dn) != (HKV, D):
-        raise ValueError(f"k_new {tuple(k_new.shape)} does not match pools of {HKV} heads of {D}")
-    if k_new.dtype != v_new.dtype:
-        raise ValueError(f"k_new and v_new must have the same dtype, got {k_new.dtype} and {v_new.dtype}")
+    shape, dtype = k_new.shape, k_new.dtype
+    if len(shape) != 4 or shape != v_new.shape:
+        raise ValueError(f"k_new and v_new must both be (B, HKV, T, head_dim), got {tuple(shape)} and {tuple(v_new.shape)}")
+    B, H, T, Dn = shape
+    if H != HKV or Dn != D:
+        raise ValueError(f"k_new {tuple(shape)} does not match pools of {HKV} heads of {D}")
+    if dtype != v_new.dtype:
+        raise ValueError(f"k_new and v_new must have the same dtype, got {dtype} and {v_new.dtype}")
     if k_new.device != dev or v_new.device != dev or vt[0].device != dev:
         raise ValueError(f"the pools and the new tokens must be on one device, got {dev}, {vt[0].device}, {k_new.device}")
     W, stride = check_table(block_table, B, dev)
-    pos_ptr, pos0 = None, 0
+    pos_ptr, pos0, len_ptr = None, 0, None
     if isinstance(positions, torch.Tensor):
         positions = check_lens(positions, B, dev, "positions")
         pos_ptr = positions.data_ptr()
@@ -134,30 +146,36 @@ def append_kv_paged(kq, vq, k_new: torch.Tensor, v_new: torch.Tensor, block_tabl
             raise ValueError(f"tokens [{pos0}, {pos0 + T}) do not fit a table of {W} pages of {page}")
     if lengths is not None:
         lengths = check_lens(lengths, B, dev, "lengths")
-    vstrides = [0] * 6
-    for i, (val, new, what) in enumerate(((k_values, k_new, "k_values"), (v_values, v_new, "v_values"))):
+        len_ptr = lengths.data_ptr()
+    places, vstrides = [None, None], [(0, 0, 0), (0, 0, 0)]
+    for i, (val, what) in enumerate(((k_values, "k_values"), (v_values, "v_values"))):
         if val is None:
             continue
-        if val.shape != new.shape or val.dtype != new.dtype or val.device != dev:
-            raise ValueError(f"{what} must be a {new.dtype} tensor of shape {tuple(new.shape)} on {dev}")
-        if _rows16(val) is not val:
+        if val.shape != shape or val.dtype != dtype or val.device != dev:
+            raise ValueError(f"{what} must be a {dtype} tensor of shape {tuple(shape)} on {dev}")
+        vstrides[i] = _row_strides(val)
+        if vstrides[i] is None:
             raise ValueError(f"{what} must have contiguous rows that start on 16-byte boundaries: it is written in place")
-        vstrides[3 * i:3 * i + 3] = _strides(val)
+        places[i] = val.data_ptr()
     code = _cabi.dtype_code(k_new)
     _cabi.require_cuda(kt[0], "kq")
     lib = _cabi.load()
     if B == 0 or T == 0 or W == 0:
         return kq, vq
-    k_new, v_new = _rows16(k_new), _rows16(v_new)
-    ks, kz, vs, vz = (kt[1], kt[2], vt[1], vt[2]) if packed else (None,) * 4
-    i6 = ctypes.c_int64 * 6
+    k_strides, v_strides = _row_strides(k_new), _row_strides(v_new)
+    if k_strides is None:
+        k_new = k_new.clone(memory_format=torch.contiguous_format)
+        k_strides = _row_strides(k_new)
+    if v_strides is None:
+        v_new = v_new.clone(memory_format=torch.contiguous_format)
+        v_strides = _row_strides(v_new)
+    meta = [t.data_ptr() for t in (*kt[1:], *vt[1:])] if packed else (None,) * 4
     with _cabi.on_device(dev):
         _cabi.check(lib.tkv_paged_append(
-            k_new.data_ptr(), v_new.data_ptr(), code, i6(*_strides(k_new), *_strides(v_new)), kt[0].data_ptr(),
-            _cabi.ptr(ks), _cabi.ptr(kz), vt[0].data_ptr(), _cabi.ptr(vs), _cabi.ptr(vz), _cabi.ptr(k_values),
-            _cabi.ptr(v_values), i6(*vstrides), block_table.data_ptr(), stride, pos_ptr, pos0, _cabi.ptr(lengths), B,
-            HKV, T, NP, page, W, D, kq.nbits if packed else 16, kq.group_size if packed else 0,
-            _cabi.stream_ptr(dev)))
+            k_new.data_ptr(), v_new.data_ptr(), code, _PACK6(*k_strides, *v_strides), kt[0].data_ptr(), meta[0], meta[1],
+            vt[0].data_ptr(), meta[2], meta[3], places[0], places[1], _PACK6(*vstrides[0], *vstrides[1]),
+            block_table.data_ptr(), stride, pos_ptr, pos0, len_ptr, B, HKV, T, NP, page, W, D,
+            kq.nbits if packed else 16, kq.group_size if packed else 0, _cabi.stream_ptr(dev)))
     return kq, vq
 
 
@@ -169,10 +187,12 @@ def _pool_list(pools) -> tuple[list[torch.Tensor], int, int, torch.device]:
     if not ts:
         raise ValueError("pools must name at least one pool")
     NP, _, page, _ = ts[0].shape
+    where = ts[0].get_device()
     for t in ts:
-        if (t.shape[0], t.shape[2]) != (NP, page) or t.device != ts[0].device:
+        shape = t.shape
+        if shape[0] != NP or shape[2] != page or t.get_device() != where:
             raise ValueError("pools that share a block table must have the same number and size of pages and one device")
-    if NP == 0 or page == 0:
+    if NP == 0 or page == 0 or ts[0].numel() == 0:
         raise ValueError("pools must have at least one page of at least one token")
     return ts, NP, page, ts[0].device
 
@@ -198,15 +218,16 @@ def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
 
 
 def _pool_args(ts):
-    ptrs = (ctypes.c_void_p * len(ts))(*(t.data_ptr() for t in ts))
-    sizes = (ctypes.c_int64 * len(ts))(*(t.numel() // t.shape[0] * t.element_size() for t in ts))
-    return ptrs, sizes, len(ts)
+    """Addresses and bytes per page (of contiguous tensors: stride 0) as the C arrays of 64-bit words."""
+    form = f"{len(ts)}q"
+    return (struct.pack(form, *[t.data_ptr() for t in ts]),
+            struct.pack(form, *[t.stride(0) * t.element_size() for t in ts]), len(ts))
 
 
 def _new_like(x, shape, dev, what):
     if x is None:
-        return torch.empty(shape, dtype=torch.int32, device=dev)
-    if x.shape != shape or x.dtype != torch.int32 or x.device != dev or not x.is_contiguous():
+        return torch.empty(shape, dtype=_I32, device=dev)
+    if x.shape != shape or x.dtype is not _I32 or x.device != dev or not x.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)} on {dev}")
     return x
 
