@@ -234,17 +234,21 @@ int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_packed, const 
                      const void* k_zero, const uint8_t* v_packed, const void* v_scale,
                      const void* v_zero, const int32_t* block_table, int64_t table_stride,
                      const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
-                     int64_t workspace_bytes, int B, int HQ, int HKV, int num_pages, int page_size,
-                     int max_pages, int D, int nbits, int gs, float sm_scale, void* stream);
+                     int64_t workspace_bytes, uint32_t* tickets, int B, int HQ, int HKV, int num_pages,
+                     int page_size, int max_pages, int D, int nbits, int gs, float sm_scale, void* stream);
 int tkv_paged_fp16_decode(const void* q, int q_dtype, const void* k, const void* v,
                           const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
-                          void* out, int out_dtype, void* workspace, int64_t workspace_bytes, int B,
-                          int HQ, int HKV, int num_pages, int page_size, int max_pages, int D,
+                          void* out, int out_dtype, void* workspace, int64_t workspace_bytes,
+                          uint32_t* tickets, int B, int HQ, int HKV, int num_pages, int page_size, int max_pages, int D,
                           float sm_scale, void* stream);
 
 /* Bytes of device workspace (partials of the split history) that the two calls above need on the
- * current device; nbits = 16 for the f16 form.  Calls that may run at the same time need
- * workspaces of their own. */
+ * current device; nbits = 16 for the f16 form.  tickets: null, or TKV_PAGED_TICKETS words of the
+ * caller's that are zero before their first use and that every call leaves zero (unless it ends
+ * with a nonzero tkv_device_status): with them, units of few partials are merged by the split
+ * kernel itself, a launch less.  Calls that may run at the same time need workspaces and tickets
+ * of their own. */
+#define TKV_PAGED_TICKETS 8192
 int tkv_paged_workspace(int B, int HQ, int HKV, int page_size, int D, int nbits, int gs,
                         int64_t* bytes);
 

@@ -138,14 +138,14 @@ def test_c_entries_refuse():
     lib, P = _cabi.load(), 4096  # a pointer that nothing follows: every call fails before that
 
     def decode(q=P, out=P, B=1, HQ=4, HKV=2, NP=8, page=16, W=4, D=64, nbits=4, gs=32, dt=0, scale=P):
-        return lib.tkv_paged_decode(q, dt, P, scale, P, P, P, P, P, W, P, out, 0, P, 1 << 30, B, HQ, HKV, NP, page, W, D, nbits, gs, 1.0, None)
+        return lib.tkv_paged_decode(q, dt, P, scale, P, P, P, P, P, W, P, out, 0, P, 1 << 30, None, B, HQ, HKV, NP, page, W, D, nbits, gs, 1.0, None)
 
     I, U, A = _cabi.TKV_ERR_INVALID, _cabi.TKV_ERR_UNSUPPORTED, _cabi.TKV_ERR_ALIGN
     for rc, kw in ((I, dict(q=None)), (I, dict(B=0)), (I, dict(HQ=5)), (I, dict(NP=0)), (I, dict(nbits=3)), (I, dict(dt=7)),
                    (I, dict(NP=1 << 27)), (I, dict(W=1 << 27)), (U, dict(page=24)), (U, dict(D=96)), (U, dict(gs=8)),
                    (U, dict(gs=128)), (A, dict(q=P + 8)), (A, dict(scale=P + 2)), (A, dict(out=P + 4))):
         assert decode(**kw) == rc, (kw, _cabi.last_error())
-    assert lib.tkv_paged_fp16_decode(P, 0, P, None, P, 4, P, P, 0, P, 1 << 30, 1, 4, 2, 8, 16, 4, 64, 1.0, None) == I
+    assert lib.tkv_paged_fp16_decode(P, 0, P, None, P, 4, P, P, 0, P, 1 << 30, None, 1, 4, 2, 8, 16, 4, 64, 1.0, None) == I
     i6 = (ctypes.c_int64 * 6)(*[64] * 6)
 
     def append(k=P, st=i6, B=1, T=1, D=64, nbits=4, gs=32, dt=0, val=None, vs=None, scale=P):

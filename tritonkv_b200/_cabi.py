@@ -78,10 +78,10 @@ SIGNATURES = {
                                         c_int, c_int, c_int, c_float, c_void_p]),
     "tkv_paged_decode": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                  c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64,
-                                 c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+                                 c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
                                  c_void_p]),
     "tkv_paged_fp16_decode": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
-                                      c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int,
+                                      c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
                                       c_int, c_int, c_int, c_float, c_void_p]),
     "tkv_paged_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
     "tkv_paged_append": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -268,9 +268,13 @@ def decode_plan(kernel_id: int, nbits: int, D: int, gs: int, B: int, HQ: int, HK
 _paged_bytes: dict = {}
 
 
+PAGED_TICKETS = 8192
+
+
 def paged_workspace(ws: dict | None, B: int, HQ: int, HKV: int, page: int, D: int, nbits: int, gs: int,
-                    device) -> torch.Tensor:
-    """The partials' buffer of a paged decode call, kept in the caller's dict ``ws`` (key ``paged``)."""
+                    device) -> tuple:
+    """(partials, their bytes, address of the tickets, tickets) of a paged decode call, kept in the caller's
+    dict ``ws`` (key ``paged``).  The tickets are zero at first, and left zero by every call."""
     key = (B, HQ, HKV, page, D, nbits, gs, _current_device())
     need = _paged_bytes.get(key)
     if need is None:
@@ -279,12 +283,17 @@ def paged_workspace(ws: dict | None, B: int, HQ: int, HKV: int, page: int, D: in
         need = v.value
         if len(_paged_bytes) < 4096:
             _paged_bytes[key] = need
-    t = None if ws is None else ws.get("paged")
-    if t is None or t.numel() < need or t.device != device:
-        t = torch.empty(need, dtype=torch.uint8, device=device)
+    kept = None if ws is None else ws.get("paged")
+    if kept is None or kept[1] < need or kept[0].device != device:
+        # what a captured graph may still use stays with the dict: the tickets, and smaller buffers
+        if kept is not None:
+            ws.setdefault("outgrown", []).append(kept)
+        tickets = kept[3] if kept is not None and kept[0].device == device else torch.zeros(
+            PAGED_TICKETS, dtype=torch.int32, device=device)
+        kept = (torch.empty(need, dtype=torch.uint8, device=device), need, tickets.data_ptr(), tickets)
         if ws is not None:
-            ws["paged"] = t
-    return t
+            ws["paged"] = kept
+    return kept
 
 
 _wave_cache: dict = {}

@@ -27,6 +27,9 @@
 namespace tkv {
 
 constexpr float kNoReference = -1e30f;  // below every score: the softmax reference before the first token
+constexpr int kFewUnits = 4;
+constexpr int kFewPartials = 10;   // of a unit, about: up to here the CTA that finishes it merges them
+constexpr int kTickets = 8192;     // units of a launch that can have a ticket
 constexpr int kMaxPagedB = 512;  // sequences whose tile prefix a CTA holds; larger batches go in parts
 
 struct PagedParams {
@@ -36,9 +39,10 @@ struct PagedParams {
   void* out;
   int out_dtype;
   int num_pages, page, max_pages, HKVc;
-  FastDiv dpage, dHch, dHKVc, dHQ, dgroup;
+  FastDiv dpage, dHch, dHKVc, dHQ, dgroup, dgrid;
   float *acc, *m, *l;     // (slots, 8, D), (slots, 8), (slots, 8)
   int2* info;             // (units): first slot and number of partials; none: the output is there
+  uint32_t* tickets;      // (units), zero between calls: partials stored so far -- the last CTA merges; or null
 };
 
 __device__ __forceinline__ void store_out4(void* out, int dtype, int64_t i, float4 v) {
@@ -73,20 +77,26 @@ __device__ __forceinline__ void paged_segment_of(PagedSegment& s, const int* pre
   s.ntiles = min(g1 - g, s.t_b - s.lo_tile);
   s.g_end = g + s.ntiles;
 }
-// The segment at tile g of the tile sequence
+// The segment at tile g of the tile sequence.  By all lanes of a warp: two ballots find the sequence (the
+// largest b with HKVc * pref[b] <= g; those without tiles are skipped), 32 candidates at a time.
 template <int kTok>
-__device__ __forceinline__ PagedSegment paged_segment_at(const int* pref, int B, int HKVc, int g, int g1) {
+__device__ __forceinline__ PagedSegment paged_segment_at(const int* pref, int B, int HKVc, int g, int g1, int lane) {
   PagedSegment s;
-  int lo = 0, hi = B;  // largest b with HKVc * pref[b] <= g (sequences without tiles are skipped)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (HKVc * (pref[mid] >> kRemBits) <= g) lo = mid; else hi = mid;
+  const int step = (B + 31) >> 5;  // at most kMaxPagedB / 32 = 16
+  const int i = min(lane * step, B);
+  const uint32_t coarse = __ballot_sync(kFullMask, i < B && HKVc * (pref[i] >> kRemBits) <= g);
+  int lo = (31 - __clz(coarse)) * step;  // (pref[0] = 0: lane 0 always votes)
+  if (step > 1) {
+    const int k = min(lo + lane, B);
+    lo += 31 - __clz(__ballot_sync(kFullMask, lane < step && k < B && HKVc * (pref[k] >> kRemBits) <= g));
   }
   lo = warp_uniform(lo);
   const int before = warp_uniform(pref[lo] >> kRemBits), t_b = warp_uniform(pref[lo + 1] >> kRemBits) - before;
   const int r = g - HKVc * before;
   s.b = lo;
-  s.hk = (int)((uint32_t)r / (uint32_t)t_b);
+  s.hk = (int)__fdividef((float)r, (float)t_b);  // off by one at most: heads of a sequence are few
+  if (s.hk * t_b > r) --s.hk;
+  else if ((s.hk + 1) * t_b <= r) ++s.hk;
   s.lo_tile = r - s.hk * t_b;
   paged_segment_of<kTok>(s, pref, g, g1);
   return s;
@@ -118,15 +128,87 @@ __device__ __forceinline__ uint32_t place_word(int row, int tokens) {
   return ((uint32_t)row >> 4) << 5 | (uint32_t)(tokens - 1);
 }
 
+// The merge of a unit's n partials (slot rows r0, r0 + 8, ...) by one whole CTA: kMergeAtOnce of them in flight,
+// a running maximum over more.
+constexpr int kMergeAtOnce = 8;
+template <int D, int THREADS>
+__device__ __forceinline__ void paged_merge_unit(const PagedParams& pp, int64_t r0, int n, int b, int hk) {
+  constexpr int D4 = D / 4, ITEMS = kHeadsPerCta * D4, ROUNDS = (ITEMS + THREADS - 1) / THREADS;
+  __shared__ float s_pm[kMergeAtOnce * kHeadsPerCta], s_pl[kMergeAtOnce * kHeadsPerCta];
+  const DecodeParams& p = pp.d;
+  float4 a[ROUNDS];
+  float L[ROUNDS], M[ROUNDS];
+#pragma unroll
+  for (int it = 0; it < ROUNDS; ++it) {
+    a[it] = make_float4(0.f, 0.f, 0.f, 0.f);
+    L[it] = 0.f;
+    M[it] = -INFINITY;
+  }
+  for (int s0 = 0; s0 < n; s0 += kMergeAtOnce) {
+    float4 x[ROUNDS][kMergeAtOnce];
+#pragma unroll
+    for (int it = 0; it < ROUNDS; ++it) {
+      const int idx = it * THREADS + threadIdx.x;
+#pragma unroll
+      for (int j = 0; j < kMergeAtOnce; ++j)
+        x[it][j] = idx < ITEMS && s0 + j < n
+                       ? __ldcg(reinterpret_cast<const float4*>(pp.acc + (r0 + (s0 + j) * kHeadsPerCta) * D) + idx)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const bool there = threadIdx.x < kMergeAtOnce * kHeadsPerCta && s0 + (int)threadIdx.x / kHeadsPerCta < n;
+    const float m = there ? __ldcg(pp.m + r0 + s0 * kHeadsPerCta + threadIdx.x) : -INFINITY;
+    const float l = there ? __ldcg(pp.l + r0 + s0 * kHeadsPerCta + threadIdx.x) : 0.f;
+    __syncthreads();
+    if (threadIdx.x < kMergeAtOnce * kHeadsPerCta) {
+      s_pm[threadIdx.x] = m;
+      s_pl[threadIdx.x] = l;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < ROUNDS; ++it) {
+      const int h = min(it * THREADS + (int)threadIdx.x, ITEMS - 1) / D4;
+      float top = M[it];
+#pragma unroll
+      for (int j = 0; j < kMergeAtOnce; ++j) top = fmaxf(top, s_pm[j * kHeadsPerCta + h]);
+      const float old = M[it] > -INFINITY ? ex2(M[it] - top) : 0.f;
+      L[it] *= old;
+      a[it].x *= old;
+      a[it].y *= old;
+      a[it].z *= old;
+      a[it].w *= old;
+      M[it] = top;
+#pragma unroll
+      for (int j = 0; j < kMergeAtOnce; ++j) {
+        const float mj = s_pm[j * kHeadsPerCta + h], w = mj > -INFINITY ? ex2(mj - top) : 0.f;
+        L[it] = fmaf(w, s_pl[j * kHeadsPerCta + h], L[it]);
+        a[it].x = fmaf(w, x[it][j].x, a[it].x);
+        a[it].y = fmaf(w, x[it][j].y, a[it].y);
+        a[it].z = fmaf(w, x[it][j].z, a[it].z);
+        a[it].w = fmaf(w, x[it][j].w, a[it].w);
+      }
+    }
+  }
+  const int hkv = fast_div(hk, pp.dHch), hc = hk - hkv * p.hchunks;
+#pragma unroll
+  for (int it = 0; it < ROUNDS; ++it) {
+    const int idx = it * THREADS + threadIdx.x, h = idx / D4, hg = hc * kHeadsPerCta + h;
+    if (idx < ITEMS && hg < p.group) {
+      const float inv = L[it] > 0.f ? 1.f / L[it] : 0.f;
+      store_out4(pp.out, pp.out_dtype, ((int64_t)b * p.HQ + hkv * p.group + hg) * D + (idx - h * D4) * 4,
+                 make_float4(a[it].x * inv, a[it].y * inv, a[it].z * inv, a[it].w * inv));
+    }
+  }
+}
+
 template <class Policy>
 __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     paged_split_kernel(const __grid_constant__ typename Policy::Maps maps, const PagedParams pp) {
   constexpr int WARPS = Policy::WARPS, STAGES = Policy::STAGES, D = Policy::D, PIECES = Policy::PIECES;
   constexpr int kTok = Policy::TOK, STAGE_BYTES = Policy::STAGE_BYTES;
   constexpr int kLog2D = D == 64 ? 6 : 7;
-  static_assert((1 << kLog2D) == D && Policy::PIPELINED && STAGES >= 3 && STAGE_BYTES % 1024 == 0 &&
+  static_assert((1 << kLog2D) == D && STAGES >= (Policy::PIPELINED ? 3 : 2) && STAGE_BYTES % 1024 == 0 &&
                     STAGE_BYTES >= kHeadsPerCta * D * 4 && STAGES * 2 <= 32,
-                "the software-pipelined ring");
+                "a ring of whole swizzle atoms that holds a warp's partial, two tiles resident or one");
   const DecodeParams& p = pp.d;
 
   extern __shared__ uint8_t smem_raw[];
@@ -135,6 +217,14 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   __shared__ float s_l[WARPS][kHeadsPerCta];
   __shared__ int s_slot[WARPS];
   __shared__ PagedCursor s_cursor[WARPS];
+  // units that this CTA shares with others: its first and its last at most
+  struct Shared {
+    int b, hk, slot, count;  // first slot, number of partials
+    uint32_t ticket;
+  };
+  __shared__ Shared s_shared[2];
+  int n_shared = 0;
+  uint32_t ticket[2] = {0, 0};  // (thread 0)
   const int warp = __shfl_sync(kFullMask, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
   pdl_launch_dependents();  // the whole grid is resident: the merge may take its place and wait
@@ -182,28 +272,47 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
 
   // ---- the tile sequence: word b = (tiles before sequence b) << kRemBits | tokens in its last tile - 1 ----
   pdl_wait();
-  for (int b = threadIdx.x; b < p.B; b += WARPS * 32) s_pref[b] = min(max(p.seq_lens[b], 0), p.S);
-  __syncthreads();
-  if (warp == 0) {
-    int carry = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int b = b0 + lane;
-      const int len = b < p.B ? s_pref[b] : 0;
-      const int t = (len + kTok - 1) / kTok;
+  {
+    constexpr int K = kMaxPagedB / (32 * WARPS);  // blocks of 32 sequences that a warp may have to take
+    const int blocks = (p.B + 31) >> 5, per_warp = (blocks + WARPS - 1) / WARPS, b0 = warp * per_warp * 32;
+    int len[K], before[K], sum = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int b = b0 + k * 32 + lane;
+      len[k] = k < per_warp && b < p.B ? min(max(p.seq_lens[b], 0), p.S) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (k >= per_warp) break;
+      const int t = (len[k] + kTok - 1) / kTok;
       int incl = t;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int y = __shfl_up_sync(kFullMask, incl, off);
         if (lane >= off) incl += y;
       }
-      if (b < p.B) s_pref[b] = ((carry + incl - t) << kRemBits) | (t > 0 ? len - (t - 1) * kTok - 1 : 0);
-      carry += __shfl_sync(kFullMask, incl, 31);
+      before[k] = sum + incl - t;
+      sum += __shfl_sync(kFullMask, incl, 31);
     }
-    if (lane == 0) s_pref[p.B] = carry << kRemBits;
+    if (lane == 0) s_slot[warp] = sum;
+    __syncthreads();
+    int base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      base += w < warp ? s_slot[w] : 0;
+      total += s_slot[w];
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int b = b0 + k * 32 + lane;
+      if (k < per_warp && b < p.B)
+        s_pref[b] = ((base + before[k]) << kRemBits) | (len[k] > 0 ? (len[k] - 1) % kTok : 0);
+    }
+    if (threadIdx.x == 0) s_pref[p.B] = total << kRemBits;
   }
   __syncthreads();
   const int T = pp.HKVc * warp_uniform(s_pref[p.B] >> kRemBits);
-  int TC = max(1, (T + (int)gridDim.x - 1) / (int)gridDim.x);
+  int TC = max(1, fast_div(T + (int)gridDim.x - 1, pp.dgrid));
   if (TC <= 4 * WARPS) TC = (TC + WARPS - 1) / WARPS * WARPS;  // no warp without a tile: fewer partials, same time
   const int g0 = min(cta * TC, T), g1 = min(g0 + TC, T);
   // sequences without tokens are touched by no range
@@ -217,23 +326,20 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
         if (hg < p.group)
           store_out4(pp.out, pp.out_dtype, ((int64_t)b * p.HQ + hkv * p.group + hg) * D + d, make_float4(0.f, 0.f, 0.f, 0.f));
       }
-      if (threadIdx.x == 0) pp.info[u] = make_int2(0, 0);
+      if (threadIdx.x == 0 && !pp.tickets) pp.info[u] = make_int2(0, 0);
     }
   };
   if (g0 >= g1) {
     empty_units();
     return;
   }
-  PagedSegment seg = paged_segment_at<kTok>(s_pref, p.B, pp.HKVc, g0, g1);
+  PagedSegment seg = paged_segment_at<kTok>(s_pref, p.B, pp.HKVc, g0, g1, lane);
 
   // ---- the warp's next 32 tiles, across segments: lane i has the place of the i-th ----
   PagedCursor* my_cursor = &s_cursor[warp];
-  if (lane == 0) *my_cursor = PagedCursor{seg, warp};
   uint32_t place[PIECES];
   int k_next = 0, n_listed = 0;  // the tile to issue next, and how many there are
-  auto look_up = [&]() {
-    __syncwarp();
-    PagedCursor cur = *my_cursor;
+  auto look_up = [&](PagedCursor cur) {
     k_next = n_listed = 0;
 #pragma unroll
     for (int h = 0; h < PIECES; ++h) place[h] = kNoPlace;
@@ -261,7 +367,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     __syncwarp();
     if (lane == 0) *my_cursor = cur;
   };
-  look_up();
+  look_up(PagedCursor{seg, warp});
   int iss_slot = 0;          // slot the next issue fills
   uint32_t valid = 0;        // bits [s*PIECES, (s+1)*PIECES): which pieces of slot s name a page
   constexpr uint32_t kAll = (1u << PIECES) - 1u;
@@ -286,11 +392,14 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     }
     valid = (valid & ~(kAll << (slot * PIECES))) | (ok << (slot * PIECES));
     Policy::issue_pieces(ist, p, maps, rows, tokens, ring_u32 + slot * STAGE_BYTES, bar_u32 + 8 * slot, lane);
-    if (++k_next == 32) look_up();
+    if (++k_next == 32) {
+      __syncwarp();
+      look_up(*my_cursor);
+    }
   };
   prefetch_q(0, seg);
 #pragma unroll 1
-  for (int s = 0; s < STAGES - 1; ++s) issue_next();
+  for (int s = 0; s < (Policy::PIPELINED ? STAGES - 1 : STAGES); ++s) issue_next();
   empty_units();
   if (seg.g_end < g1) {
     PagedSegment s = seg;
@@ -323,8 +432,28 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     auto update = [&](typename Policy::Scores& sc, int slot) {
       Policy::update(acc, qs, sc, ring_u32 + slot * STAGE_BYTES, ring + slot * STAGE_BYTES, left, lane);
     };
-    // Software pipeline: the scores of tile i+1 beside the softmax and output of tile i.
-    if (my_tiles > 0 && !timed_out) {
+    if (!Policy::PIPELINED) {
+      // One tile at a time; its stage is refilled as soon as it is finished -- after the segment's
+      // last tile, which carries the warp's partial, behind the epilogue.
+      for (int i = 0; i < my_tiles; ++i) {
+        if (!mbar_wait_bounded(bar_u32 + 8 * c_slot, c_phase)) {
+          timed_out = true;
+          break;
+        }
+        __syncwarp();
+        typename Policy::Scores sc;
+        scores(sc, c_slot, left);
+        update(sc, c_slot);
+        left -= WARPS * kTok;
+        if (++c_slot == STAGES) {
+          c_slot = 0;
+          c_phase ^= 1;
+        }
+        __syncwarp();
+        if (i + 1 < my_tiles) issue_next();
+      }
+    } else if (my_tiles > 0 && !timed_out) {
+      // Software pipeline: the scores of tile i+1 beside the softmax and output of tile i.
       typename Policy::Scores sc_cur;
       if (!mbar_wait_bounded(bar_u32 + 8 * c_slot, c_phase)) timed_out = true;
       __syncwarp();
@@ -361,6 +490,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     }
 
     // ---- merge the warps, store the partial or the output ----
+    bool shared_unit = false;
     const int vals_slot = (c_slot == 0 ? STAGES : c_slot) - 1;  // the stage consumed last
     SoftmaxState st{-INFINITY, -INFINITY, 0.f, 0.f};
     if (my_tiles > 0) Policy::finalize(acc, reinterpret_cast<float*>(ring + vals_slot * STAGE_BYTES), st, lane);
@@ -386,8 +516,9 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       const int count = (u1 <= g1 ? cta : (int)((uint32_t)(u1 - 1) / (uint32_t)TC)) - first + 1;
       const int64_t slot = (int64_t)(unit + cta) * kHeadsPerCta;
 #pragma unroll
-      for (int it = 0; it < ITEMS / (WARPS * 32); ++it) {
+      for (int it = 0; it < (ITEMS + WARPS * 32 - 1) / (WARPS * 32); ++it) {
         const int idx = it * (WARPS * 32) + threadIdx.x;
+        if (ITEMS % (WARPS * 32) != 0 && idx >= ITEMS) break;
         const int h = idx / D4, d = (idx - h * D4) * 4, hg = hc * kHeadsPerCta + h;
         if (hg >= p.group) continue;
         float mw[WARPS], M = -INFINITY;
@@ -421,11 +552,28 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
                      make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
         }
       }
-      if (threadIdx.x == 0 && first == cta) pp.info[unit] = count > 1 ? make_int2(unit + cta, count) : make_int2(0, 0);
+      if (!pp.tickets) {
+        if (threadIdx.x == 0 && first == cta) pp.info[unit] = count > 1 ? make_int2(unit + cta, count) : make_int2(0, 0);
+      } else if (count > 1 && threadIdx.x == 0) {
+        s_shared[n_shared] = Shared{seg.b, seg.hk, unit + first, count, 0};
+      }
+      shared_unit = count > 1;
     }
     __syncthreads();
+    // This CTA's partial is stored: draw the unit's ticket.  Nobody waits for it before the end, so that the
+    // answer travels while the next segment runs.
+    if (pp.tickets && shared_unit) {
+      if (threadIdx.x == 0) {
+        __threadfence();
+        const uint32_t t = atomicAdd(pp.tickets + seg.b * pp.HKVc + seg.hk, 1u);
+        if (n_shared == 0) ticket[0] = t;
+        else ticket[1] = t;
+      }
+      ++n_shared;
+    }
     need_proxy_fence = true;
     if (seg.g_end >= g1 || timed_out) break;
+    if (!Policy::PIPELINED && my_tiles > 0) issue_next();
     paged_segment_next<kTok>(seg, s_pref, pp.HKVc, g1);
     if (seg.g_end < g1) {  // the query slot just released takes the segment after the next
       PagedSegment s = seg;
@@ -435,6 +583,19 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     ++seg_k;
   }
   if (timed_out && lane == 0) Policy::report_timeout();
+  if (n_shared == 0) return;
+  if (threadIdx.x == 0) {
+    s_shared[0].ticket = ticket[0];
+    s_shared[1].ticket = ticket[1];
+  }
+  __syncthreads();
+  for (int i = 0; i < n_shared; ++i) {
+    if (s_shared[i].ticket != (uint32_t)s_shared[i].count - 1u) continue;  // others are still to come
+    __threadfence();
+    if (threadIdx.x == 0) pp.tickets[s_shared[i].b * pp.HKVc + s_shared[i].hk] = 0;
+    paged_merge_unit<D, WARPS * 32>(pp, (int64_t)s_shared[i].slot * kHeadsPerCta, s_shared[i].count, s_shared[i].b,
+                                    s_shared[i].hk);
+  }
 }
 
 // ---------------------------------------------------------------- merge of a unit's partials
@@ -594,6 +755,7 @@ struct PagedCall {  // one call, before it is cut into launches
   int B;
   void* workspace;
   int64_t workspace_bytes;
+  uint32_t* tickets;
 };
 
 template <class Policy>
@@ -652,6 +814,7 @@ struct PagedLaunch {
       const int n = c.B - b0 < part ? c.B - b0 : (int)part;
       const int64_t rows0 = (int64_t)b0 * pp.d.HQ * Policy::D;
       pp.d.B = n;
+      pp.dgrid = make_fastdiv(w);
       pp.d.q = (const uint8_t*)pp.d.q + rows0 * (pp.d.q_dtype == TKV_DTYPE_F32 ? 4 : 2);
       pp.out = (uint8_t*)pp.out + rows0 * (pp.out_dtype == TKV_DTYPE_F32 ? 4 : 2);
       pp.d.seq_lens += b0;
@@ -660,8 +823,18 @@ struct PagedLaunch {
       pp.m = pp.acc + slots * kHeadsPerCta * Policy::D;
       pp.l = pp.m + slots * kHeadsPerCta;
       pp.info = (int2*)(pp.l + slots * kHeadsPerCta);
+      // Who merges.  With at least a CTA per unit and few partials of each, the CTA that finishes a unit:
+      // one launch instead of two, 2.4 us of host time (17.0 -> 14.6 us per call), for the same time on the
+      // device (1 sequence of 500 tokens 7.9 / 7.9 us, 8 of 4096 20.1 / 21.0, 16 of 4096 26.6 / 27.1).  Else a
+      // kernel that spreads the partials over the device: one sequence of 65536 (222 partials a unit)
+      // 13.1 us against 23.2, and with more units than CTAs, where every CTA would draw two tickets,
+      // 53.1 against 53.8 (64 sequences at 2 bits).
+      const int64_t units_now = (int64_t)n * pp.HKVc;
+      const int64_t partials = 2 + (w / units_now < tiles / Policy::WARPS ? w / units_now : tiles / Policy::WARPS);
+      pp.tickets = units_now <= w && partials <= kFewPartials && units_now <= kTickets ? c.tickets : nullptr;
       TKV_CUDA(launch_pdl(paged_split_kernel<Policy>, dim3(w), dim3(Policy::WARPS * 32), (size_t)smem_bytes(n), stream,
                           maps, pp));
+      if (pp.tickets) continue;
       const int rows = n * pp.d.HQ;
       if (rows < kSmallCombineMinRows)
         TKV_CUDA(launch_pdl(paged_merge_long_kernel<Policy::D>, dim3(rows, Policy::D / 32), dim3(256), 0, stream, pp));
@@ -700,13 +873,26 @@ static int f16_run(const PagedCall& c, cudaStream_t stream) {
   return PagedLaunch<P>::run(maps, c, stream);
 }
 
+// Two families per format, as for contiguous caches (tkv_decode_fused.cu): 4 warps with rings of 3
+// stages in a software pipeline, 3 CTAs per SM; and 8 warps with rings of 2, one tile at a time, 2 CTAs per
+// SM, where few long units are to be spread thin.
 template <int NB, int DD, int GG, int PIECES>
 using PagedPolicy = FusedPolicy<NB, DD, GG, true, 32, 4, 3, 3, true, false, PIECES>;
+template <int NB, int DD, int GG, int PIECES>
+using PagedLongPolicy = FusedPolicy<NB, DD, GG, true, 32, 8, 2, 2, false, false, PIECES>;
 
 #define TKV_PAGED_ONE(NB, DD, GG, EXPR)                        \
   if (nbits == NB && D == DD && gs == GG) {                    \
     if (page % 32 == 0) {                                      \
+      if (few) {                                               \
+        using P = PagedLongPolicy<NB, DD, GG, 1>;              \
+        return EXPR;                                           \
+      }                                                        \
       using P = PagedPolicy<NB, DD, GG, 1>;                    \
+      return EXPR;                                             \
+    }                                                          \
+    if (few) {                                                 \
+      using P = PagedLongPolicy<NB, DD, GG, 2>;                \
       return EXPR;                                             \
     }                                                          \
     using P = PagedPolicy<NB, DD, GG, 2>;                      \
@@ -727,6 +913,10 @@ using PagedPolicy = FusedPolicy<NB, DD, GG, true, 32, 4, 3, 3, true, false, PIEC
   TKV_PAGED_ONE(2, 64, 16, EXPR)     \
   TKV_PAGED_ONE(2, 64, 32, EXPR)     \
   TKV_PAGED_ONE(2, 64, 64, EXPR)
+
+// Few units of work: the family that spreads them thinner (one sequence, 2 KV heads, 65536 tokens: 12.5 us
+// against 13.8; with 8 KV heads, 30000 tokens, it is 18.8 against 17.6, and 64 sequences are the same to 2 %).
+static bool few_units(int B, int HKVc) { return (int64_t)B * HKVc <= kFewUnits; }
 
 static int packed_unsupported(int nbits, int D, int gs) {
   set_error("paged decode: unsupported (nbits=%d, head_dim=%d, group_size=%d); built: nbits in {2,4}, head_dim in "
@@ -752,8 +942,8 @@ int paged_device_status_clear() {
 // Checks shared by the two entry points; fills everything but the pools.
 static int paged_fill(const char* who, PagedCall& c, const void* q, int q_dtype, const int32_t* table,
                       int64_t table_stride, const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
-                      int64_t workspace_bytes, int B, int HQ, int HKV, int num_pages, int page, int max_pages, int D,
-                      float sm_scale) {
+                      int64_t workspace_bytes, uint32_t* tickets, int B, int HQ, int HKV, int num_pages, int page,
+                      int max_pages, int D, float sm_scale) {
   TKV_REQUIRE(B > 0 && HQ > 0 && HKV > 0 && HQ % HKV == 0, TKV_ERR_INVALID,
               "%s: bad sizes B=%d HQ=%d HKV=%d (HQ must be a multiple of HKV)", who, B, HQ, HKV);
   TKV_REQUIRE(num_pages > 0 && page > 0 && max_pages >= 0, TKV_ERR_INVALID,
@@ -773,6 +963,7 @@ static int paged_fill(const char* who, PagedCall& c, const void* q, int q_dtype,
   c.B = B;
   c.workspace = workspace;
   c.workspace_bytes = workspace_bytes;
+  c.tickets = tickets;
   PagedParams& pp = c.pp;
   DecodeParams& p = pp.d;
   p.q = q;
@@ -815,6 +1006,7 @@ extern "C" int tkv_paged_workspace(int B, int HQ, int HKV, int page_size, int D,
     set_error("paged fp16 decode: unsupported head_dim=%d (built: 64, 128)", D);
     return TKV_ERR_UNSUPPORTED;
   }
+  const bool few = few_units(B, HKVc);
   TKV_PAGED_ALL(PagedLaunch<P>::bytes(B, HKVc, bytes))
   return packed_unsupported(nbits, D, gs);
 }
@@ -823,13 +1015,13 @@ extern "C" int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_pac
                                 const void* k_zero, const uint8_t* v_packed, const void* v_scale,
                                 const void* v_zero, const int32_t* block_table, int64_t table_stride,
                                 const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
-                                int64_t workspace_bytes, int B, int HQ, int HKV, int num_pages, int page_size,
+                                int64_t workspace_bytes, uint32_t* tickets, int B, int HQ, int HKV, int num_pages, int page_size,
                                 int max_pages, int D, int nbits, int gs, float sm_scale, void* stream) {
   using namespace tkv;
   TKV_REQUIRE(nbits == 2 || nbits == 4, TKV_ERR_INVALID, "nbits must be one of (2, 4), got %d", nbits);
   PagedCall c;
   const int rc = paged_fill("paged decode", c, q, q_dtype, block_table, table_stride, seq_lens, out, out_dtype,
-                            workspace, workspace_bytes, B, HQ, HKV, num_pages, page_size, max_pages, D, sm_scale);
+                            workspace, workspace_bytes, tickets, B, HQ, HKV, num_pages, page_size, max_pages, D, sm_scale);
   if (rc != TKV_OK) return rc;
   TKV_REQUIRE(k_packed && k_scale && k_zero && v_packed && v_scale && v_zero, TKV_ERR_INVALID, "paged decode: null pointer");
   TKV_REQUIRE(aligned16(k_packed) && aligned16(v_packed) && aligned16(k_scale) && aligned16(k_zero) &&
@@ -852,6 +1044,7 @@ extern "C" int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_pac
                gap >= (uint64_t)pool;
     p.k_second = p.kv_one && k_packed > v_packed;
   }
+  const bool few = few_units(B, c.pp.HKVc);
   TKV_PAGED_ALL(packed_run<P>(c, (cudaStream_t)stream))
   return packed_unsupported(nbits, D, gs);
 }
@@ -859,12 +1052,12 @@ extern "C" int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_pac
 extern "C" int tkv_paged_fp16_decode(const void* q, int q_dtype, const void* k, const void* v,
                                      const int32_t* block_table, int64_t table_stride,
                                      const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
-                                     int64_t workspace_bytes, int B, int HQ, int HKV, int num_pages, int page_size,
+                                     int64_t workspace_bytes, uint32_t* tickets, int B, int HQ, int HKV, int num_pages, int page_size,
                                      int max_pages, int D, float sm_scale, void* stream) {
   using namespace tkv;
   PagedCall c;
   const int rc = paged_fill("paged fp16 decode", c, q, q_dtype, block_table, table_stride, seq_lens, out, out_dtype,
-                            workspace, workspace_bytes, B, HQ, HKV, num_pages, page_size, max_pages, D, sm_scale);
+                            workspace, workspace_bytes, tickets, B, HQ, HKV, num_pages, page_size, max_pages, D, sm_scale);
   if (rc != TKV_OK) return rc;
   TKV_REQUIRE(k && v, TKV_ERR_INVALID, "paged fp16 decode: null pointer");
   TKV_REQUIRE(aligned16(k) && aligned16(v), TKV_ERR_ALIGN, "paged fp16 decode: the pools must be 16-byte aligned");

@@ -84,7 +84,7 @@ def paged_decode_attention(
         _cabi.check(lib.tkv_paged_decode(
             q.data_ptr(), _cabi.dtype_code(q), kt[0].data_ptr(), kt[1].data_ptr(), kt[2].data_ptr(), vt[0].data_ptr(),
             vt[1].data_ptr(), vt[2].data_ptr(), block_table.data_ptr(), stride, seq_lens.data_ptr(), out.data_ptr(),
-            _cabi.dtype_code(out), ws.data_ptr(), ws.numel(), B, HQ, HKV, NP, page, W, D, kq.nbits, kq.group_size,
+            _cabi.dtype_code(out), ws[0].data_ptr(), ws[1], ws[2], B, HQ, HKV, NP, page, W, D, kq.nbits, kq.group_size,
             1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _cabi.stream_ptr(dev)))
     return out
 
@@ -113,6 +113,6 @@ def paged_fp16_decode_attention(
         ws = _cabi.paged_workspace(_workspace, B, HQ, HKV, page, D, 16, 0, dev)
         _cabi.check(lib.tkv_paged_fp16_decode(
             q.data_ptr(), _cabi.dtype_code(q), kt[0].data_ptr(), vt[0].data_ptr(), block_table.data_ptr(), stride,
-            seq_lens.data_ptr(), out.data_ptr(), _cabi.dtype_code(out), ws.data_ptr(), ws.numel(), B, HQ, HKV, NP, page, W, D,
+            seq_lens.data_ptr(), out.data_ptr(), _cabi.dtype_code(out), ws[0].data_ptr(), ws[1], ws[2], B, HQ, HKV, NP, page, W, D,
             1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _cabi.stream_ptr(dev)))
     return out

@@ -209,12 +209,14 @@ def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
         need = n.value
         if len(_pages_words) < 4096:
             _pages_words[(B, NP)] = need
-    kept, t = (None, None) if ws is None else ws.get("pages", (None, None))
-    if kept != NP or t.numel() < need or t.device != dev:
-        t = torch.zeros(need, dtype=torch.int32, device=dev)
+    kept = None if ws is None else ws.get("pages")
+    if kept is None or kept[0] != NP or kept[1].numel() < need or kept[1].device != dev:
+        if kept is not None:  # a captured graph may still use it
+            ws.setdefault("outgrown", []).append(kept)
+        kept = (NP, torch.zeros(need, dtype=torch.int32, device=dev))
         if ws is not None:
-            ws["pages"] = (NP, t)
-    return t
+            ws["pages"] = kept
+    return kept[1]
 
 
 def _pool_args(ts):
