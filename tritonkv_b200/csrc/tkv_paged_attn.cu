@@ -39,6 +39,7 @@ struct PagedParams {
   void* out;
   int out_dtype;
   int num_pages, page, max_pages, HKVc;
+  int whole;              // a CTA takes part of one unit only: how many a unit can have; 0: equal ranges of all tiles
   FastDiv dpage, dHch, dHKVc, dHQ, dgroup, dgrid;
   float *acc, *m, *l;     // (slots, 8, D), (slots, 8), (slots, 8)
   int2* info;             // (units): first slot and number of partials; none: the output is there
@@ -60,6 +61,15 @@ __device__ __forceinline__ void store_out4(void* out, int dtype, int64_t i, floa
 // What all lanes of a warp hold, said so that the compiler sees it: ring slots, cursor and barrier
 // arithmetic that hangs off it can then go to the uniform datapath.
 __device__ __forceinline__ int warp_uniform(int x) { return __shfl_sync(kFullMask, x, 0); }
+
+// floor(a / b) by a float quotient, put right by at most one (a below 2^25, a quotient below 2^23)
+__device__ __forceinline__ int small_div(int a, int b) {
+  int q = (int)__fdividef((float)a, (float)b);
+  const int r = a - q * b;
+  if (r < 0) --q;
+  else if (r >= b) ++q;
+  return q;
+}
 
 // The part of a unit that a CTA processes.  `pref` is the prefix of tiles per sequence, see the kernel.
 struct PagedSegment {
@@ -94,12 +104,44 @@ __device__ __forceinline__ PagedSegment paged_segment_at(const int* pref, int B,
   const int before = warp_uniform(pref[lo] >> kRemBits), t_b = warp_uniform(pref[lo + 1] >> kRemBits) - before;
   const int r = g - HKVc * before;
   s.b = lo;
-  s.hk = (int)__fdividef((float)r, (float)t_b);  // off by one at most: heads of a sequence are few
-  if (s.hk * t_b > r) --s.hk;
-  else if ((s.hk + 1) * t_b <= r) ++s.hk;
+  s.hk = small_div(r, t_b);
   s.lo_tile = r - s.hk * t_b;
   paged_segment_of<kTok>(s, pref, g, g1);
   return s;
+}
+// The part of one unit that CTA `cta` takes where every unit has CTAs of its own, ceil(t / TC) of them for a unit
+// of t tiles; `first` is the unit's first CTA and `count` how many it has.  false: nothing is left for this CTA.  By
+// all lanes of a warp.
+template <int kTok>
+__device__ __forceinline__ bool paged_segment_whole(PagedSegment& s, const int* pref, int B, int HKVc, int TC, int cta,
+                                                    int lane, int& first, int& count) {
+  int carry = 0;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const int b = min(b0 + lane, B - 1), t = (pref[b + 1] >> kRemBits) - (pref[b] >> kRemBits);
+    const int n = b0 + lane < B ? small_div(t + TC - 1, TC) : 0, ctas = n * HKVc;
+    int incl = ctas;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(kFullMask, incl, off);
+      if (lane >= off) incl += y;
+    }
+    const uint32_t behind = __ballot_sync(kFullMask, carry + incl > cta);
+    if (behind) {
+      const int l = __ffs(behind) - 1;
+      count = warp_uniform(__shfl_sync(kFullMask, n, l));
+      first = carry + warp_uniform(__shfl_sync(kFullMask, incl - ctas, l));
+      s.b = warp_uniform(b0 + l);
+      s.hk = warp_uniform(small_div(cta - first, count));
+      first += s.hk * count;
+      const int j = cta - first, t_b = warp_uniform(__shfl_sync(kFullMask, t, l));
+      const int q = warp_uniform(small_div(t_b, count)), rem = t_b - q * count;
+      s.lo_tile = j * q + min(j, rem);
+      paged_segment_of<kTok>(s, pref, 0, q + (j < rem ? 1 : 0));
+      return true;
+    }
+    carry += warp_uniform(__shfl_sync(kFullMask, incl, 31));
+  }
+  return false;
 }
 // The one behind it (there is one: s.g_end < g1): the next unit from its start
 template <int kTok>
@@ -313,8 +355,37 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   __syncthreads();
   const int T = pp.HKVc * warp_uniform(s_pref[p.B] >> kRemBits);
   int TC = max(1, fast_div(T + (int)gridDim.x - 1, pp.dgrid));
+  if (pp.whole && p.B == 1) {
+    TC = max(1, small_div((s_pref[1] >> kRemBits) + pp.whole - 1, pp.whole));
+  } else if (pp.whole) {
+    // the smallest TC (of 32 * WARPS candidates up to twice the least) for which the CTAs are enough
+    const int mine = TC + threadIdx.x * (TC / (32 * WARPS) + 1);
+    int ctas = 0;
+    for (int b = 0, at = 0; b < p.B; ++b) {
+      const int end = s_pref[b + 1] >> kRemBits;
+      ctas += small_div(end - at + mine - 1, mine);
+      at = end;
+    }
+    const uint32_t fits = __ballot_sync(kFullMask, ctas * pp.HKVc <= (int)gridDim.x);
+    __syncthreads();  // (s_slot still holds the warps' sums)
+    if (lane == (fits ? __ffs(fits) - 1 : 0)) s_slot[warp] = fits ? mine : 1 << 24;
+    __syncthreads();
+    TC = s_slot[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) TC = min(TC, s_slot[w]);
+    TC = warp_uniform(TC);
+  }
   if (TC <= 4 * WARPS) TC = (TC + WARPS - 1) / WARPS * WARPS;  // no warp without a tile: fewer partials, same time
-  const int g0 = min(cta * TC, T), g1 = min(g0 + TC, T);
+  int g0, g1, whole_first = 0, whole_count = 0;
+  PagedSegment seg;
+  if (pp.whole) {
+    g0 = 0;
+    g1 = paged_segment_whole<kTok>(seg, s_pref, p.B, pp.HKVc, TC, cta, lane, whole_first, whole_count) ? seg.ntiles : 0;
+  } else {
+    g0 = min(cta * TC, T);
+    g1 = min(g0 + TC, T);
+    if (g0 < g1) seg = paged_segment_at<kTok>(s_pref, p.B, pp.HKVc, g0, g1, lane);
+  }
   // sequences without tokens are touched by no range
   auto empty_units = [&]() {
     for (int u = cta; u < p.B * pp.HKVc; u += gridDim.x) {
@@ -333,7 +404,6 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     empty_units();
     return;
   }
-  PagedSegment seg = paged_segment_at<kTok>(s_pref, p.B, pp.HKVc, g0, g1, lane);
 
   // ---- the warp's next 32 tiles, across segments: lane i has the place of the i-th ----
   PagedCursor* my_cursor = &s_cursor[warp];
@@ -510,11 +580,16 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       for (int w = 0; w < WARPS; ++w) voff[w] = (uint32_t)((w * STAGES + s_slot[w]) * STAGE_BYTES);
       const int hkv = fast_div(seg.hk, pp.dHch), hc = seg.hk - hkv * p.hchunks;
       const int unit = seg.b * pp.HKVc + seg.hk;
-      // the CTAs of the unit: only a unit that crosses a border of this one's range takes a division
-      const int u0 = seg.g_end - seg.ntiles - seg.lo_tile, u1 = u0 + seg.t_b;  // its tiles in the sequence
-      const int first = seg.lo_tile == 0 ? cta : (int)((uint32_t)u0 / (uint32_t)TC);
-      const int count = (u1 <= g1 ? cta : (int)((uint32_t)(u1 - 1) / (uint32_t)TC)) - first + 1;
-      const int64_t slot = (int64_t)(unit + cta) * kHeadsPerCta;
+      // the CTAs of the unit, and the slot of this one's partial: distinct, since the next unit begins no
+      // earlier than in the CTA where this one ends, or the CTA's own where it has one unit only
+      int first = whole_first, count = whole_count, slot0 = 0;
+      if (!pp.whole) {  // (only a unit that crosses a border of this CTA's range takes a division)
+        const int u0 = seg.g_end - seg.ntiles - seg.lo_tile, u1 = u0 + seg.t_b;  // its tiles in the sequence
+        first = seg.lo_tile == 0 ? cta : (int)((uint32_t)u0 / (uint32_t)TC);
+        count = (u1 <= g1 ? cta : (int)((uint32_t)(u1 - 1) / (uint32_t)TC)) - first + 1;
+        slot0 = unit;
+      }
+      const int64_t slot = (int64_t)(slot0 + cta) * kHeadsPerCta;
 #pragma unroll
       for (int it = 0; it < (ITEMS + WARPS * 32 - 1) / (WARPS * 32); ++it) {
         const int idx = it * (WARPS * 32) + threadIdx.x;
@@ -553,9 +628,9 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
         }
       }
       if (!pp.tickets) {
-        if (threadIdx.x == 0 && first == cta) pp.info[unit] = count > 1 ? make_int2(unit + cta, count) : make_int2(0, 0);
+        if (threadIdx.x == 0 && first == cta) pp.info[unit] = count > 1 ? make_int2(slot0 + cta, count) : make_int2(0, 0);
       } else if (count > 1 && threadIdx.x == 0) {
-        s_shared[n_shared] = Shared{seg.b, seg.hk, unit + first, count, 0};
+        s_shared[n_shared] = Shared{seg.b, seg.hk, slot0 + first, count, 0};
       }
       shared_unit = count > 1;
     }
@@ -830,6 +905,7 @@ struct PagedLaunch {
       // 13.1 us against 23.2, and with more units than CTAs, where every CTA would draw two tickets,
       // 53.1 against 53.8 (64 sequences at 2 bits).
       const int64_t units_now = (int64_t)n * pp.HKVc;
+      pp.whole = units_now * 2 <= w && tiles * Policy::WARPS < (1 << 23) ? (int)(w / units_now) : 0;
       const int64_t partials = 2 + (w / units_now < tiles / Policy::WARPS ? w / units_now : tiles / Policy::WARPS);
       pp.tickets = units_now <= w && partials <= kFewPartials && units_now <= kTickets ? c.tickets : nullptr;
       TKV_CUDA(launch_pdl(paged_split_kernel<Policy>, dim3(w), dim3(Policy::WARPS * 32), (size_t)smem_bytes(n), stream,

@@ -139,8 +139,10 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkArgs 
     int32_t* row = a.new_table + (int64_t)b * a.W;
     const bool live = par >= 0 && par < a.B_old;
     bool elder = false;
-    if (live)
+    if (live) {
+#pragma unroll 8
       for (int i = lane; i < b; i += 32) elder |= a.parents[i] == par;
+    }
     const bool first = !__any_sync(kFullMask, elder);
     const int n = live ? (int)min((int64_t)max(a.lens[par], 0), (int64_t)a.W * a.page) : 0;
     const ForkRow r = fork_row(a, b, n);

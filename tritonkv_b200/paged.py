@@ -183,18 +183,22 @@ def _pool_list(pools) -> tuple[list[torch.Tensor], int, int, torch.device]:
     """(tensors, num_pages, page_size, device) of pools that share one block table."""
     if isinstance(pools, (QuantizedTensor, torch.Tensor)):
         pools = [pools]
-    ts = [t for i, p in enumerate(pools) for t in pool_tensors(p, f"pools[{i}]")]
+    ts, shape, where = [], None, -1
+    for i, p in enumerate(pools):
+        t = pool_tensors(p, f"pools[{i}]")
+        if shape is None:
+            shape, where = t[0].shape, t[0].get_device()
+        else:
+            other = t[0].shape
+            if other[0] != shape[0] or other[2] != shape[2] or t[0].get_device() != where:
+                raise ValueError("pools that share a block table must have the same number and size of pages and one "
+                                 "device")
+        ts += t
     if not ts:
         raise ValueError("pools must name at least one pool")
-    NP, _, page, _ = ts[0].shape
-    where = ts[0].get_device()
-    for t in ts:
-        shape = t.shape
-        if shape[0] != NP or shape[2] != page or t.get_device() != where:
-            raise ValueError("pools that share a block table must have the same number and size of pages and one device")
-    if NP == 0 or page == 0 or ts[0].numel() == 0:
+    if ts[0].numel() == 0:
         raise ValueError("pools must have at least one page of at least one token")
-    return ts, NP, page, ts[0].device
+    return ts, shape[0], shape[2], ts[0].device
 
 
 _pages_words: dict = {}
@@ -223,23 +227,34 @@ def _pool_args(ts):
     """Addresses and bytes per page (of contiguous tensors: stride 0) as the C arrays of 64-bit words."""
     form = f"{len(ts)}q"
     return (struct.pack(form, *[t.data_ptr() for t in ts]),
-            struct.pack(form, *[t.stride(0) * t.element_size() for t in ts]), len(ts))
+            struct.pack(form, *[t.stride(0) * (1 if t.dtype is _U8 else 2) for t in ts]), len(ts))
 
 
-def _new_like(x, shape, dev, what):
+def _new_like(x, shape, like, what):
     if x is None:
-        return torch.empty(shape, dtype=_I32, device=dev)
-    if x.shape != shape or x.dtype is not _I32 or x.device != dev or not x.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)} on {dev}")
+        return like.new_empty(shape)
+    if x.shape != shape or x.dtype is not _I32 or x.device != like.device or not x.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)} on {like.device}")
     return x
 
 
-def _no_overlap(a: torch.Tensor, b: torch.Tensor, what: str) -> None:
-    if a.numel() and b.numel():
-        span = lambda t: (t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
-        (a0, a1), (b0, b1) = span(a), span(b)
-        if a0 < b1 and b0 < a1:
-            raise ValueError(f"{what} must not share memory with the tensor it is made from")
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First and last + 1 byte of an int32 tensor; empty ones overlap nothing."""
+    a, n = t.data_ptr(), t.numel()
+    if n == 0:
+        return 0, 0
+    if not t.is_contiguous():
+        n = 1 + sum((k - 1) * s for k, s in zip(t.shape, t.stride()))
+    return a, a + 4 * n
+
+
+def _no_overlap(outs, ins) -> None:
+    ins = [_span(t) for t in ins]
+    for i, t in enumerate(outs):
+        a0, a1 = _span(t)
+        for b0, b1 in ins:
+            if a0 < b1 and b0 < a1:
+                raise ValueError(f"out[{i}] must not share memory with a tensor it is made from")
 
 
 def fork_pages(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, reserve=0,
@@ -279,13 +294,11 @@ def fork_pages(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, parents
         if not 0 <= r0 < 2 ** 31:
             raise ValueError(f"reserve must be a number of tokens, got {r0}")
     table, lens, missing = (None, None, None) if out is None else out
-    table = _new_like(table, (B, W), dev, "out[0]")
-    lens = _new_like(lens, (B,), dev, "out[1]")
-    missing = _new_like(missing, (1,), dev, "out[2]")
+    table = _new_like(table, (B, W), block_table, "out[0]")
+    lens = _new_like(lens, (B,), block_table, "out[1]")
+    missing = _new_like(missing, (1,), block_table, "out[2]")
     if out is not None:
-        for x in (block_table, seq_lens, parents) + ((reserve,) if r_ptr is not None else ()):
-            for i, y in enumerate((table, lens, missing)):
-                _no_overlap(y, x, f"out[{i}]")
+        _no_overlap((table, lens, missing), (block_table, seq_lens, parents) + (() if r_ptr is None else (reserve,)))
     _cabi.require_cuda(ts[0], "pools")
     lib = _cabi.load()
     with _cabi.on_device(dev):
@@ -309,11 +322,10 @@ def compact_pages(pools, block_table: torch.Tensor, out: tuple | None = None, _w
     W, stride = check_table(block_table, None, dev)
     B = block_table.shape[0]
     table, live = (None, None) if out is None else out
-    table = _new_like(table, (B, W), dev, "out[0]")
-    live = _new_like(live, (1,), dev, "out[1]")
+    table = _new_like(table, (B, W), block_table, "out[0]")
+    live = _new_like(live, (1,), block_table, "out[1]")
     if out is not None:
-        _no_overlap(table, block_table, "out[0]")
-        _no_overlap(live, block_table, "out[1]")
+        _no_overlap((table, live), (block_table,))
     _cabi.require_cuda(ts[0], "pools")
     lib = _cabi.load()
     with _cabi.on_device(dev):
