@@ -71,24 +71,31 @@ __device__ __forceinline__ int small_div(int a, int b) {
   return q;
 }
 
-// The part of a unit that a CTA processes.  `pref` is the prefix of tiles per sequence, see the kernel.
+// The work is cut in steps: a unit of t > 0 tiles takes kSwitch + t of them, since a CTA that goes from one
+// unit to the next spends about as long as on kSwitch tiles (the merge of its warps, the next query's
+// fragments, the pipeline run down and up again).  Without it the CTAs that got many short sequences came
+// last.  `pref`: word b = (steps of one head unit of the sequences before b) << kRemBits | tokens in its last tile - 1.
+constexpr int kSwitch = 12;
+__device__ __forceinline__ int unit_tiles(int steps) { return max(steps - kSwitch, 0); }
+__device__ __forceinline__ int unit_steps(int tiles) { return tiles > 0 ? tiles + kSwitch : 0; }
+
+// The part of a unit that a CTA processes.
 struct PagedSegment {
   int b, hk;        // sequence; KV head and head chunk
   int hi, t_b;      // length of the sequence, tiles of the unit
   int lo_tile;      // first tile, within the unit
-  int ntiles, g_end;
+  int ntiles;
+  int g_end;        // the step behind it
 };
 
 template <int kTok>
-__device__ __forceinline__ void paged_segment_of(PagedSegment& s, const int* pref, int g, int g1) {
+__device__ __forceinline__ void paged_segment_of(PagedSegment& s, const int* pref) {
   const int word = warp_uniform(pref[s.b]);
-  s.t_b = warp_uniform(pref[s.b + 1] >> kRemBits) - (word >> kRemBits);
+  s.t_b = unit_tiles(warp_uniform(pref[s.b + 1] >> kRemBits) - (word >> kRemBits));
   s.hi = (s.t_b - 1) * kTok + (word & ((1 << kRemBits) - 1)) + 1;
-  s.ntiles = min(g1 - g, s.t_b - s.lo_tile);
-  s.g_end = g + s.ntiles;
 }
-// The segment at tile g of the tile sequence.  By all lanes of a warp: two ballots find the sequence (the
-// largest b with HKVc * pref[b] <= g; those without tiles are skipped), 32 candidates at a time.
+// The segment of steps [g, g1), g being a step of some unit.  By all lanes of a warp: two ballots find the
+// sequence (the largest b with HKVc * pref[b] <= g; empty ones are skipped), 32 candidates at a time.
 template <int kTok>
 __device__ __forceinline__ PagedSegment paged_segment_at(const int* pref, int B, int HKVc, int g, int g1, int lane) {
   PagedSegment s;
@@ -100,13 +107,14 @@ __device__ __forceinline__ PagedSegment paged_segment_at(const int* pref, int B,
     const int k = min(lo + lane, B);
     lo += 31 - __clz(__ballot_sync(kFullMask, lane < step && k < B && HKVc * (pref[k] >> kRemBits) <= g));
   }
-  lo = warp_uniform(lo);
-  const int before = warp_uniform(pref[lo] >> kRemBits), t_b = warp_uniform(pref[lo + 1] >> kRemBits) - before;
-  const int r = g - HKVc * before;
-  s.b = lo;
-  s.hk = small_div(r, t_b);
-  s.lo_tile = r - s.hk * t_b;
-  paged_segment_of<kTok>(s, pref, g, g1);
+  s.b = warp_uniform(lo);
+  paged_segment_of<kTok>(s, pref);
+  const int r = g - HKVc * warp_uniform(pref[s.b] >> kRemBits), steps = s.t_b + kSwitch;
+  s.hk = small_div(r, steps);
+  const int at = r - s.hk * steps, len = min(g1 - g, steps - at);
+  s.lo_tile = unit_tiles(at);
+  s.ntiles = unit_tiles(at + len) - s.lo_tile;
+  s.g_end = g + len;
   return s;
 }
 // The part of one unit that CTA `cta` takes where every unit has CTAs of its own, ceil(t / TC) of them for a unit
@@ -117,7 +125,7 @@ __device__ __forceinline__ bool paged_segment_whole(PagedSegment& s, const int* 
                                                     int lane, int& first, int& count) {
   int carry = 0;
   for (int b0 = 0; b0 < B; b0 += 32) {
-    const int b = min(b0 + lane, B - 1), t = (pref[b + 1] >> kRemBits) - (pref[b] >> kRemBits);
+    const int b = min(b0 + lane, B - 1), t = unit_tiles((pref[b + 1] >> kRemBits) - (pref[b] >> kRemBits));
     const int n = b0 + lane < B ? small_div(t + TC - 1, TC) : 0, ctas = n * HKVc;
     int incl = ctas;
 #pragma unroll
@@ -133,17 +141,19 @@ __device__ __forceinline__ bool paged_segment_whole(PagedSegment& s, const int* 
       s.b = warp_uniform(b0 + l);
       s.hk = warp_uniform(small_div(cta - first, count));
       first += s.hk * count;
-      const int j = cta - first, t_b = warp_uniform(__shfl_sync(kFullMask, t, l));
-      const int q = warp_uniform(small_div(t_b, count)), rem = t_b - q * count;
+      paged_segment_of<kTok>(s, pref);
+      const int j = cta - first, q = warp_uniform(small_div(s.t_b, count)), rem = s.t_b - q * count;
       s.lo_tile = j * q + min(j, rem);
-      paged_segment_of<kTok>(s, pref, 0, q + (j < rem ? 1 : 0));
+      s.ntiles = q + (j < rem ? 1 : 0);
+      s.g_end = 0;
       return true;
     }
     carry += warp_uniform(__shfl_sync(kFullMask, incl, 31));
   }
   return false;
 }
-// The one behind it (there is one: s.g_end < g1): the next unit from its start
+// Whether steps up to g1 reach into the unit behind a segment, and the segment there
+__device__ __forceinline__ bool paged_segment_more(const PagedSegment& s, int g1) { return g1 - s.g_end > kSwitch; }
 template <int kTok>
 __device__ __forceinline__ void paged_segment_next(PagedSegment& s, const int* pref, int HKVc, int g1) {
   s.lo_tile = 0;
@@ -151,11 +161,10 @@ __device__ __forceinline__ void paged_segment_next(PagedSegment& s, const int* p
     s.hk = 0;
     do ++s.b;
     while (warp_uniform(pref[s.b + 1] >> kRemBits) == warp_uniform(pref[s.b] >> kRemBits));
-    paged_segment_of<kTok>(s, pref, s.g_end, g1);
-  } else {
-    s.ntiles = min(g1 - s.g_end, s.t_b);
-    s.g_end += s.ntiles;
+    paged_segment_of<kTok>(s, pref);
   }
+  s.ntiles = min(g1 - s.g_end - kSwitch, s.t_b);
+  s.g_end += s.ntiles + kSwitch;
 }
 
 // Where a warp's copies stand, segments ahead of the one being computed.  Kept in shared memory: only
@@ -257,7 +266,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ float s_m[WARPS][kHeadsPerCta];
   __shared__ float s_l[WARPS][kHeadsPerCta];
-  __shared__ int s_slot[WARPS];
+  __shared__ int s_slot[WARPS], s_tiles[WARPS];
   __shared__ PagedCursor s_cursor[WARPS];
   // units that this CTA shares with others: its first and its last at most
   struct Shared {
@@ -312,12 +321,13 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   typename Policy::Query qs;
   Policy::lane_init(qs, p, lane);
 
-  // ---- the tile sequence: word b = (tiles before sequence b) << kRemBits | tokens in its last tile - 1 ----
+  // ---- the steps of the sequences, one after the other ----
   pdl_wait();
+  int total_tiles = 0;
   {
     constexpr int K = kMaxPagedB / (32 * WARPS);  // blocks of 32 sequences that a warp may have to take
     const int blocks = (p.B + 31) >> 5, per_warp = (blocks + WARPS - 1) / WARPS, b0 = warp * per_warp * 32;
-    int len[K], before[K], sum = 0;
+    int len[K], before[K], sum = 0, tiles = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int b = b0 + k * 32 + lane;
@@ -326,7 +336,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k >= per_warp) break;
-      const int t = (len[k] + kTok - 1) / kTok;
+      const int t = unit_steps((len[k] + kTok - 1) / kTok);
       int incl = t;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -335,14 +345,20 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       }
       before[k] = sum + incl - t;
       sum += __shfl_sync(kFullMask, incl, 31);
+      tiles += unit_tiles(t);
     }
-    if (lane == 0) s_slot[warp] = sum;
+    tiles = __reduce_add_sync(kFullMask, (unsigned)tiles);
+    if (lane == 0) {
+      s_slot[warp] = sum;
+      s_tiles[warp] = tiles;
+    }
     __syncthreads();
     int base = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       base += w < warp ? s_slot[w] : 0;
       total += s_slot[w];
+      total_tiles += s_tiles[w];
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -355,35 +371,44 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
   __syncthreads();
   const int T = pp.HKVc * warp_uniform(s_pref[p.B] >> kRemBits);
   int TC = max(1, fast_div(T + (int)gridDim.x - 1, pp.dgrid));
-  if (pp.whole && p.B == 1) {
-    TC = max(1, small_div((s_pref[1] >> kRemBits) + pp.whole - 1, pp.whole));
-  } else if (pp.whole) {
-    // the smallest TC (of 32 * WARPS candidates up to twice the least) for which the CTAs are enough
-    const int mine = TC + threadIdx.x * (TC / (32 * WARPS) + 1);
-    int ctas = 0;
-    for (int b = 0, at = 0; b < p.B; ++b) {
-      const int end = s_pref[b + 1] >> kRemBits;
-      ctas += small_div(end - at + mine - 1, mine);
-      at = end;
-    }
-    const uint32_t fits = __ballot_sync(kFullMask, ctas * pp.HKVc <= (int)gridDim.x);
-    __syncthreads();  // (s_slot still holds the warps' sums)
-    if (lane == (fits ? __ffs(fits) - 1 : 0)) s_slot[warp] = fits ? mine : 1 << 24;
-    __syncthreads();
-    TC = s_slot[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) TC = min(TC, s_slot[w]);
-    TC = warp_uniform(TC);
-  }
-  if (TC <= 4 * WARPS) TC = (TC + WARPS - 1) / WARPS * WARPS;  // no warp without a tile: fewer partials, same time
   int g0, g1, whole_first = 0, whole_count = 0;
   PagedSegment seg;
   if (pp.whole) {
-    g0 = 0;
-    g1 = paged_segment_whole<kTok>(seg, s_pref, p.B, pp.HKVc, TC, cta, lane, whole_first, whole_count) ? seg.ntiles : 0;
+    if (p.B == 1) {
+      TC = max(1, small_div(unit_tiles(s_pref[1] >> kRemBits) + pp.whole - 1, pp.whole));
+    } else {
+      // the smallest TC for which the CTAs are enough, of PER * WARPS candidates from an even share up to twice that
+      constexpr int PER = 4;
+      TC = max(1, fast_div(pp.HKVc * warp_uniform(total_tiles) + (int)gridDim.x - 1, pp.dgrid));
+      int mine[PER], ctas[PER], best = 1 << 24;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        mine[k] = TC + small_div(TC * (k * WARPS + warp) + PER * WARPS - 2, PER * WARPS - 1);
+        ctas[k] = 0;
+      }
+      for (int b = lane; b < p.B; b += 32) {
+        const int t = unit_tiles((s_pref[b + 1] >> kRemBits) - (s_pref[b] >> kRemBits));
+#pragma unroll
+        for (int k = 0; k < PER; ++k) ctas[k] += small_div(t + mine[k] - 1, mine[k]);
+      }
+#pragma unroll
+      for (int k = PER - 1; k >= 0; --k)
+        if ((int)__reduce_add_sync(kFullMask, (unsigned)ctas[k]) * pp.HKVc <= (int)gridDim.x) best = mine[k];
+      __syncthreads();  // (s_slot still holds the warps' sums)
+      if (lane == 0) s_slot[warp] = best;
+      __syncthreads();
+      TC = s_slot[0];
+#pragma unroll
+      for (int w = 1; w < WARPS; ++w) TC = min(TC, s_slot[w]);
+      TC = warp_uniform(TC);
+    }
+    if (TC <= 4 * WARPS) TC = (TC + WARPS - 1) / WARPS * WARPS;  // no warp without a tile: fewer partials, same time
+    g0 = g1 = 0;
+    if (!paged_segment_whole<kTok>(seg, s_pref, p.B, pp.HKVc, TC, cta, lane, whole_first, whole_count)) seg.ntiles = 0;
   } else {
     g0 = min(cta * TC, T);
     g1 = min(g0 + TC, T);
+    seg.ntiles = 0;
     if (g0 < g1) seg = paged_segment_at<kTok>(s_pref, p.B, pp.HKVc, g0, g1, lane);
   }
   // sequences without tokens are touched by no range
@@ -400,7 +425,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       if (threadIdx.x == 0 && !pp.tickets) pp.info[u] = make_int2(0, 0);
     }
   };
-  if (g0 >= g1) {
+  if (seg.ntiles == 0) {
     empty_units();
     return;
   }
@@ -430,7 +455,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       }
       n_listed += take;
       cur.tile += take * WARPS;
-      if (n_listed == 32 || cur.seg.g_end >= g1) break;
+      if (n_listed == 32 || !paged_segment_more(cur.seg, g1)) break;
       paged_segment_next<kTok>(cur.seg, s_pref, pp.HKVc, g1);
       cur.tile = warp;
     }
@@ -471,7 +496,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
 #pragma unroll 1
   for (int s = 0; s < (Policy::PIPELINED ? STAGES - 1 : STAGES); ++s) issue_next();
   empty_units();
-  if (seg.g_end < g1) {
+  if (paged_segment_more(seg, g1)) {
     PagedSegment s = seg;
     paged_segment_next<kTok>(s, s_pref, pp.HKVc, g1);
     prefetch_q(1, s);
@@ -584,8 +609,8 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       // earlier than in the CTA where this one ends, or the CTA's own where it has one unit only
       int first = whole_first, count = whole_count, slot0 = 0;
       if (!pp.whole) {  // (only a unit that crosses a border of this CTA's range takes a division)
-        const int u0 = seg.g_end - seg.ntiles - seg.lo_tile, u1 = u0 + seg.t_b;  // its tiles in the sequence
-        first = seg.lo_tile == 0 ? cta : (int)((uint32_t)u0 / (uint32_t)TC);
+        const int u0 = pp.HKVc * (s_pref[seg.b] >> kRemBits) + seg.hk * (seg.t_b + kSwitch), u1 = u0 + kSwitch + seg.t_b;
+        first = seg.lo_tile == 0 ? cta : (int)((uint32_t)(u0 + kSwitch) / (uint32_t)TC);
         count = (u1 <= g1 ? cta : (int)((uint32_t)(u1 - 1) / (uint32_t)TC)) - first + 1;
         slot0 = unit;
       }
@@ -647,10 +672,10 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
       ++n_shared;
     }
     need_proxy_fence = true;
-    if (seg.g_end >= g1 || timed_out) break;
+    if (!paged_segment_more(seg, g1) || timed_out) break;
     if (!Policy::PIPELINED && my_tiles > 0) issue_next();
     paged_segment_next<kTok>(seg, s_pref, pp.HKVc, g1);
-    if (seg.g_end < g1) {  // the query slot just released takes the segment after the next
+    if (paged_segment_more(seg, g1)) {  // the query slot just released takes the segment after the next
       PagedSegment s = seg;
       paged_segment_next<kTok>(s, s_pref, pp.HKVc, g1);
       prefetch_q(seg_k & 1, s);
@@ -877,10 +902,10 @@ struct PagedLaunch {
     TKV_REQUIRE(c.workspace && c.workspace_bytes >= need, TKV_ERR_INVALID,
                 "paged decode: a workspace of %lld bytes is needed, got %lld; size it with tkv_paged_workspace",
                 (long long)need, (long long)c.workspace_bytes);
-    const int64_t tiles = ((int64_t)c.pp.d.S + Policy::TOK - 1) / Policy::TOK;  // of one sequence, at most
-    int64_t part = kMaxPagedB;  // sequences of a launch: tile numbers fit the prefix words and 30 bits
-    if (part * tiles >= (1 << 25)) part = ((1 << 25) - 1) / tiles;
-    if (part * tiles * c.pp.HKVc >= (1 << 30)) part = ((1 << 30) - 1) / (tiles * c.pp.HKVc);
+    const int64_t tiles = ((int64_t)c.pp.d.S + Policy::TOK - 1) / Policy::TOK, steps = tiles + kSwitch;  // of one sequence, at most
+    int64_t part = kMaxPagedB;  // sequences of a launch: step numbers fit the prefix words and 30 bits
+    if (part * steps >= (1 << 25)) part = ((1 << 25) - 1) / steps;
+    if (part * steps * c.pp.HKVc >= (1 << 30)) part = ((1 << 30) - 1) / (steps * c.pp.HKVc);
     TKV_REQUIRE(part >= 1, TKV_ERR_INVALID, "paged decode: %lld tiles of %d head units per sequence are too many",
                 (long long)tiles, c.pp.HKVc);
     const int64_t units = (int64_t)(c.B < kMaxPagedB ? c.B : kMaxPagedB) * c.pp.HKVc, slots = units + w;
