@@ -221,6 +221,45 @@ def test_no_allocation_with_workspace():
     assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_random_batches(seed, ws={}):
+    """Batches of every kind in turn, all with one workspace: few and many units, one merge and the other, ranges
+    that cross units, skewed lengths, holes."""
+    import random
+
+    rng = random.Random(seed)
+    D = rng.choice((64, 128))
+    nbits, gs = rng.choice(((4, 32), (2, 16), (4, 64), (2, 64), (16, 0), (16, 0)))
+    HKV, G, page = rng.choice((1, 2, 4, 8)), rng.choice((1, 3, 4, 8, 12)), rng.choice((16, 32, 48, 64, 128))
+    B = rng.choice((1, 2, 3, 7, 16, 28, 40, 64, 100, 230))
+    top = max(2, min(3000, 60000 // (B * HKV)))
+    lens = [rng.choice((0, 1, rng.randrange(top), top, rng.randrange(1, 40))) for _ in range(B)]
+    if seed % 4 == 0:
+        lens[rng.randrange(B)] = 6 * top
+    k, v, table, NP = make_pools(lens, HKV, D, nbits, gs, page, seed=seed)
+    if seed % 3 == 0:
+        for _ in range(B):
+            table[rng.randrange(B), rng.randrange(table.shape[1])] = rng.choice((-1, NP, -2 ** 31))
+    q = make_q(B, HKV * G, D, seed)
+    out = torch.full((B, HKV * G, D), float("nan"), device=DEV)
+    attend(q, k, v, table, lens_t(lens), out=out, _workspace=ws)
+    check(out, q, k, v, table, lens, f"B={B} HKV={HKV} G={G} D={D} {nbits} bits page={page}")
+    again = attend(q, k, v, table, lens_t(lens), _workspace=ws)
+    assert torch.equal(out, again) and torch.equal(out, attend(q, k, v, table, lens_t(lens)))
+
+
+def test_too_small_a_workspace_is_refused():
+    from tritonkv_b200 import _cabi
+
+    k, v, table, NP = make_pools([64], 1, 64, 4, 32, 16, seed=1)
+    q, sl, out = make_q(1, 2, 64, 0), lens_t([64]), torch.empty(1, 2, 64, device=DEV)
+    rc = _cabi.load().tkv_paged_decode(
+        q.data_ptr(), 0, *(t.data_ptr() for p in (k, v) for t in (p.packed, p.scale, p.zero)), table.data_ptr(),
+        table.stride(0), sl.data_ptr(), out.data_ptr(), 2, out.data_ptr(), 64, None, 1, 2, 1, NP, 16, table.shape[1], 64, 4,
+        32, 0.125, _cabi.stream_ptr(q.device))
+    assert rc == _cabi.TKV_ERR_INVALID and "tkv_paged_workspace" in _cabi.last_error()
+
+
 def test_pool_past_two_to_the_31_bytes():
     """Pages whose bytes lie past 2^31 and 2^32 of the pool."""
     D, page, HKV = 128, 64, 8

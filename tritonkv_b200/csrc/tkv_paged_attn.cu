@@ -9,28 +9,42 @@
 // The tiles, their arithmetic and the per-warp copy rings are those of the contiguous kernels
 // (tkv_fused_policy.cuh, tkv_fp16_policy.cuh); what differs is where a tile comes from and how the
 // work is cut.  A tile of 32 packed tokens is one run of rows where the page is a multiple of 32
-// tokens, else two runs of 16 (PIECES).  When a warp enters a segment its lanes look up the pool
-// rows of the warp's next 32 tiles, one each; an issue takes its row by a shuffle, so the table's
-// latency is paid once per 32 tiles and hidden behind the tiles in flight.
+// tokens, else two runs of 16 (PIECES: 64 sequences at 4 bits 57 us against 53.8 in one).  The lanes of a warp look
+// up the pool rows of the warp's next 32 tiles, one each, across the segments to come; an issue takes
+// its row by a shuffle, so the table's latency is paid once per 32 tiles, behind tiles in flight, and the
+// tile loop holds no cursor (with one, 100 instructions a tile more, and spills).
 //
-// Lengths live on the device.  Every CTA builds the prefix of tiles per sequence in shared memory
-// and takes an equal range of the tile sequence, whatever the lengths are; a range that crosses
-// from one unit (sequence, KV head, 8 query heads) to the next is processed segment by segment.  A
-// unit that one CTA has to itself goes straight to the output.  Else segment (unit u, CTA c) leaves
-// its partial (acc, m, l) in slot u + c -- distinct for all segments, since the next unit starts no
-// earlier than in the CTA where this one ends -- and the unit's first CTA notes where its slots
-// begin and how many they are, for the merge that follows.  So the workspace holds units + CTAs
-// partials whatever the lengths, and no slot has to be marked empty.
+// Lengths live on the device, so the plan is made there, by every CTA for itself: the prefix of the
+// sequences' work in shared memory, then either
+//   * whole (units -- sequence, KV head, 8 query heads -- at most half the CTAs): every unit has CTAs of its
+//     own, ceil(t / TC) for t tiles with the smallest TC for which they suffice; or
+//   * equal ranges of all work, whatever the lengths are; a range that crosses from one unit to the next is
+//     processed segment by segment, and the switch counts as kSwitch tiles when the ranges are cut.
+// A unit that one CTA has to itself goes straight to the output.  Else segment (unit u, CTA c) leaves
+// its partial (acc, m, l) in slot u + c (whole: c) -- distinct for all segments, since the next unit
+// starts no earlier than in the CTA where this one ends.  So the workspace holds units + CTAs partials
+// whatever the lengths, and no slot has to be marked empty.  They are merged by the CTA that draws the unit's last
+// ticket, or by a kernel of their own: see PagedLaunch::run.
+//
+// What is rounded: q to f16; the probabilities, formed and summed in f32 against a running maximum, to
+// f16 for the second product (on packed pages once more when the values' scale is multiplied in, since
+// the codes are exact in f16 and the scales differ by token); the output once.  All sums are f32.  Against float64 the output
+// is 3.4e-4 off on packed pages and 2.5e-4 on float16 ones (2-norm), where rounding it to f16 alone is 2.0e-4.  Carrying
+// the second rounding's error through a second product took 8-10 % (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.
+//
+// What bounds it: with many tiles the instructions of the tile loop (packed; about 600 a tile and warp) or the
+// memory (float16: 32 sequences, 338 MB, 60.3 us, 5.6 TB/s); with few, the chain of latencies: lengths, table, first tile
+// (3.3 us before it is asked for), 1.2 us a tile, the merge (2.5 us).
 #include "tkv_fp16_policy.cuh"
 #include "tkv_fused_policy.cuh"
 
 namespace tkv {
 
 constexpr float kNoReference = -1e30f;  // below every score: the softmax reference before the first token
-constexpr int kFewUnits = 4;
+constexpr int kFewUnits = 4;       // up to here the family of 8 warps, see few_units
 constexpr int kFewPartials = 10;   // of a unit, about: up to here the CTA that finishes it merges them
 constexpr int kTickets = 8192;     // units of a launch that can have a ticket
-constexpr int kMaxPagedB = 512;  // sequences whose tile prefix a CTA holds; larger batches go in parts
+constexpr int kMaxPagedB = 512;    // sequences whose prefix a CTA holds; larger batches go in parts
 
 struct PagedParams {
   DecodeParams d;         // what the tile policies read; d.B sequences of this launch
@@ -73,8 +87,9 @@ __device__ __forceinline__ int small_div(int a, int b) {
 
 // The work is cut in steps: a unit of t > 0 tiles takes kSwitch + t of them, since a CTA that goes from one
 // unit to the next spends about as long as on kSwitch tiles (the merge of its warps, the next query's
-// fragments, the pipeline run down and up again).  Without it the CTAs that got many short sequences came
-// last.  `pref`: word b = (steps of one head unit of the sequences before b) << kRemBits | tokens in its last tile - 1.
+// fragments, the pipeline run down and up again).  With 0 / 4 / 8 / 12 / 20: 40 sequences of 100-2000 tokens 28.8 /
+// 23.7 / 22.4 / 22.2 / 22.4 us, 55 of 1000-4096 45.4 / 43.7 / 42.8 / 42.7 / 43.0, 64 at 2 bits 53.8 / 52.9 / 52.2 / 51.4 / 51.9.
+// `pref`: word b = (steps of one head unit of the sequences before b) << kRemBits | tokens in its last tile - 1.
 constexpr int kSwitch = 12;
 __device__ __forceinline__ int unit_tiles(int steps) { return max(steps - kSwitch, 0); }
 __device__ __forceinline__ int unit_steps(int tiles) { return tiles > 0 ? tiles + kSwitch : 0; }
@@ -923,14 +938,18 @@ struct PagedLaunch {
       pp.m = pp.acc + slots * kHeadsPerCta * Policy::D;
       pp.l = pp.m + slots * kHeadsPerCta;
       pp.info = (int2*)(pp.l + slots * kHeadsPerCta);
+      // How the work is cut.  CTAs of its own for every unit where there are two or more: nobody pays for a
+      // second unit (16 sequences of 1024-4096 tokens, 8 KV heads: 19.8 us against 22.2 in equal ranges, 16 of 1000 13.0
+      // against 16.2, 27 of 4096 33.3 against 37.5).  With fewer the rounding to whole units costs more (55 of
+      // 1000-4096: 52.6 against 47.1).
+      const int64_t units_now = (int64_t)n * pp.HKVc;
+      pp.whole = units_now * 2 <= w && tiles * Policy::WARPS < (1 << 23) ? (int)(w / units_now) : 0;
       // Who merges.  With at least a CTA per unit and few partials of each, the CTA that finishes a unit:
       // one launch instead of two, 2.4 us of host time (17.0 -> 14.6 us per call), for the same time on the
       // device (1 sequence of 500 tokens 7.9 / 7.9 us, 8 of 4096 20.1 / 21.0, 16 of 4096 26.6 / 27.1).  Else a
       // kernel that spreads the partials over the device: one sequence of 65536 (222 partials a unit)
       // 13.1 us against 23.2, and with more units than CTAs, where every CTA would draw two tickets,
       // 53.1 against 53.8 (64 sequences at 2 bits).
-      const int64_t units_now = (int64_t)n * pp.HKVc;
-      pp.whole = units_now * 2 <= w && tiles * Policy::WARPS < (1 << 23) ? (int)(w / units_now) : 0;
       const int64_t partials = 2 + (w / units_now < tiles / Policy::WARPS ? w / units_now : tiles / Policy::WARPS);
       pp.tickets = units_now <= w && partials <= kFewPartials && units_now <= kTickets ? c.tickets : nullptr;
       TKV_CUDA(launch_pdl(paged_split_kernel<Policy>, dim3(w), dim3(Policy::WARPS * 32), (size_t)smem_bytes(n), stream,
@@ -1015,8 +1034,9 @@ using PagedLongPolicy = FusedPolicy<NB, DD, GG, true, 32, 8, 2, 2, false, false,
   TKV_PAGED_ONE(2, 64, 32, EXPR)     \
   TKV_PAGED_ONE(2, 64, 64, EXPR)
 
-// Few units of work: the family that spreads them thinner (one sequence, 2 KV heads, 65536 tokens: 12.5 us
-// against 13.8; with 8 KV heads, 30000 tokens, it is 18.8 against 17.6, and 64 sequences are the same to 2 %).
+// Few units of work: the family that spreads them thinner.  One sequence of 65536 tokens with 1 / 2 / 4 / 8 KV heads:
+// 11.4 / 12.8 / 12.3 / 23.4 us against 13.5 / 13.7 / 12.6 / 24.4; but with 8 heads 4096 tokens are 10.6 against 9.9,
+// and 64 sequences are the same to 2 %.
 static bool few_units(int B, int HKVc) { return (int64_t)B * HKVc <= kFewUnits; }
 
 static int packed_unsupported(int nbits, int D, int gs) {
