@@ -211,6 +211,28 @@ def test_streams_graphs_and_workspaces(nbits):
         assert torch.equal(attend(q, k, v, tb, sl), runs[0][1])
 
 
+def test_graphed_step_over_pages():
+    """The captured host-in, host-out step on a paged cache: equal to the direct call, as the lengths grow and
+    the table moves."""
+    from tritonkv_b200 import GraphedDecodeStep
+
+    lens = [300, 77, 0]
+    k, v, table, _ = make_pools([300, 90, 40], 2, 128, 4, 32, 16, seed=21)
+    sl, tb = lens_t(lens), table.clone()
+    step = GraphedDecodeStep(k, v, 6, seq_lens=sl, block_table=tb)
+    for i in range(4):
+        q = make_q(3, 6, 128, i)
+        step.run(q.cpu())
+        got = step.result().clone().to(DEV)
+        assert torch.equal(got, attend(q, k, v, tb, sl))
+        check(got, q, k, v, tb, sl.tolist(), f"step {i}")
+        if i < 2:  # (what make_pools filled: up to 300, 90 and 40 tokens)
+            sl.add_(lens_t([0, 4, 10]))
+        if i == 1:
+            tb.copy_(tb[[2, 1, 0]])
+            sl.copy_(sl[[2, 1, 0]])
+
+
 def test_no_allocation_with_workspace():
     k, v, table, _ = make_pools([900, 40], 2, 128, 4, 32, 16, seed=1)
     q, sl, out, ws = make_q(2, 8, 128, 1), lens_t([900, 40]), torch.empty(2, 8, 128, device=DEV), {}

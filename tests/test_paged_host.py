@@ -133,6 +133,16 @@ def test_compact_refuses():
         compact_pages(pool(), t, out=(t, i32(1)))
 
 
+def test_paged_graphed_step_refuses():
+    from tritonkv_b200 import GraphedDecodeStep
+
+    for kw in (dict(), dict(seq_lens=i32(3), zero_copy=True), dict(seq_lens=i32(3), num_splits=2)):
+        with pytest.raises(ValueError, match="paged step"):
+            GraphedDecodeStep(pool(), pool(), 4, block_table=i32(3, 5), **kw)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        GraphedDecodeStep(pool(), pool(), 4, block_table=i32(3, 5), seq_lens=i32(3))
+
+
 def test_c_entries_refuse():
     """Argument errors of the C ABI come back before any launch."""
     lib, P = _cabi.load(), 4096  # a pointer that nothing follows: every call fails before that

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from .kernels import fused_decode_attention
+from .kernels import fused_decode_attention, paged_decode_attention
 from .quantize import QuantizedTensor
 
 
@@ -29,16 +29,23 @@ class GraphedDecodeStep:
     The query keeps its copy node: every CTA of the split kernel reads the query rows, which
     costs nothing from L2 but made the step 2.4x slower when each of those reads crossed
     the bus.
+
+    ``block_table`` (int32 ``(B, max_pages)`` on the device): ``kq`` and ``vq`` are pools of pages
+    (:mod:`tritonkv_b200.paged`) and the step is ``paged_decode_attention``; ``seq_lens`` is then
+    required.  The table, like ``seq_lens``, is read at every step from where it was at capture:
+    ``fork_pages`` and ``compact_pages`` results are copied into it between steps.  Not with ``zero_copy``.
     """
 
     def __init__(self, kq: QuantizedTensor, vq: QuantizedTensor, HQ: int,
                  q_dtype: torch.dtype = torch.float16, seq_lens: torch.Tensor | None = None,
                  sm_scale: float | None = None, num_splits: int | None = None,
-                 zero_copy: bool = False):
+                 zero_copy: bool = False, block_table: torch.Tensor | None = None):
         dev = kq.packed.device
+        if block_table is not None and (seq_lens is None or zero_copy or num_splits is not None):
+            raise ValueError("a paged step needs seq_lens, and takes neither zero_copy nor num_splits")
         if dev.type != "cuda":
             raise RuntimeError("GraphedDecodeStep needs a CUDA cache; this package has no CPU path")
-        B, D = kq.packed.shape[0], kq.head_dim
+        B, D = (kq.packed if block_table is None else block_table).shape[0], kq.head_dim
         self.q_host = torch.zeros(B, HQ, D, dtype=q_dtype).pin_memory()
         self.out_host = torch.zeros(B, HQ, D, dtype=torch.float32).pin_memory()
         self.q_dev = torch.zeros(B, HQ, D, dtype=q_dtype, device=dev)
@@ -51,6 +58,11 @@ class GraphedDecodeStep:
 
         def step():
             self.q_dev.copy_(self.q_host, non_blocking=True)
+            if block_table is not None:
+                paged_decode_attention(self.q_dev, kq, vq, block_table, seq_lens, sm_scale=sm_scale,
+                                       out=self.out_dev, _workspace=self._ws)
+                self.out_host.copy_(self.out_dev, non_blocking=True)
+                return
             if zero_copy:
                 fused_decode_attention(self.q_dev, kq, vq, sm_scale=sm_scale, num_splits=num_splits,
                                        out=self.out_host, _workspace=self._ws, seq_lens=seq_lens,
