@@ -29,7 +29,7 @@
 // What is rounded: q to f16; the probabilities, formed and summed in f32 against a running maximum, to
 // f16 for the second product (on packed pages once more when the values' scale is multiplied in, since
 // the codes are exact in f16 and the scales differ by token); the output once.  All sums are f32.  Against float64 the output
-// is 3.4e-4 off on packed pages and 2.5e-4 on float16 ones (2-norm), where rounding it to f16 alone is 2.0e-4.  Carrying
+// is 3.4e-4 to 4.5e-4 off on packed pages and 2.5e-4 on float16 ones (2-norm), where rounding it to f16 alone is 2.0e-4.  Carrying
 // the second rounding's error through a second product took 8-10 % (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.
 //
 // What bounds it: with many tiles the instructions of the tile loop (packed; about 600 a tile and warp) or the
