@@ -138,46 +138,51 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkArgs 
     const int par = a.parents[b];
     int32_t* row = a.new_table + (int64_t)b * a.W;
     const bool live = par >= 0 && par < a.B_old;
+    // (the loads that hang on the parent alone are on their way while its earlier children are looked for)
+    const int32_t* old = a.table + (live ? par : 0) * a.table_stride;
+    const int tokens = live ? a.lens[par] : 0;
+    int id0 = live && lane < a.W ? old[lane] : -1;
     bool elder = false;
     if (live) {
 #pragma unroll 8
       for (int i = lane; i < b; i += 32) elder |= a.parents[i] == par;
     }
-    const bool first = !__any_sync(kFullMask, elder);
-    const int n = live ? (int)min((int64_t)max(a.lens[par], 0), (int64_t)a.W * a.page) : 0;
+    const int n = (int)min((int64_t)max(tokens, 0), (int64_t)a.W * a.page);
     const ForkRow r = fork_row(a, b, n);
-    const int32_t* old = a.table + (live ? par : 0) * a.table_stride;
+    const int last = r.held > r.full ? old[r.full] : -1;  // the partly filled page
+    const bool first = !__any_sync(kFullMask, elder);
     const int keep = live ? (first ? r.held : r.full) : 0;
     for (int i = lane; i < a.W; i += 32) {
       int id = -1;
       if (i < keep) {
-        id = old[i];
+        id = i < 32 ? id0 : old[i];
         if (!page_ok(id, a.num_pages)) id = -1;
         else atomicOr(a.used + (id >> 5), 1u << (id & 31));
       }
       row[i] = id;
     }
     if (lane == 0) {
-      const bool copy = live && r.held > r.full && !first && page_ok(old[r.full], a.num_pages);
-      a.src[b] = copy ? old[r.full] : -1;
+      const bool copy = !first && page_ok(last, a.num_pages);
+      a.src[b] = copy ? last : -1;
       a.new_lens[b] = n;
       a.start[b] = live ? (copy ? 1 : 0) + max(0, r.want - r.held) : 0;
     }
   }
   if (!last_cta(a.ticket)) return;
   int need = 0, have = 0, total;
+  const int words = (a.num_pages + 31) / 32;
+  const uint32_t used0 = tid < words ? __ldcg(a.used + tid) : 0;  // (beside the first needs)
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
     const int b = b0 + tid, x = b < a.B ? __ldcg(a.start + b) : 0;
     const int before = block_scan(x, total);
     if (b < a.B) a.start[b] = need + before;
     need += total;
   }
-  const int words = (a.num_pages + 31) / 32;
   for (int w0 = 0; w0 < words; w0 += kPlanThreads) {
     const int w = w0 + tid;
     uint32_t free = 0;
     if (w < words) {
-      free = ~__ldcg(a.used + w) & word_mask(w, a.num_pages);
+      free = ~(w0 == 0 ? used0 : __ldcg(a.used + w)) & word_mask(w, a.num_pages);
       a.used[w] = 0;
     }
     if (have >= need) continue;  // (the same for all threads) enough: the rest is only wiped
