@@ -88,7 +88,8 @@ __device__ __forceinline__ int small_div(int a, int b) {
 // The work is cut in steps: a unit of t > 0 tiles takes kSwitch + t of them, since a CTA that goes from one
 // unit to the next spends about as long as on kSwitch tiles (the merge of its warps, the next query's
 // fragments, the pipeline run down and up again).  With 0 / 4 / 8 / 12 / 20: 40 sequences of 100-2000 tokens 28.8 /
-// 23.7 / 22.4 / 22.2 / 22.4 us, 55 of 1000-4096 45.4 / 43.7 / 42.8 / 42.7 / 43.0, 64 at 2 bits 53.8 / 52.9 / 52.2 / 51.4 / 51.9.
+// 23.7 / 22.4 / 22.2 / 22.4 us, 55 of 1000-4096 45.4 / 43.7 / 42.8 / 42.7 / 43.0, 64 at 2 bits 53.8 / 52.9 / 52.2 / 51.4 / 51.9;
+// 200 of 20-500 53.3 / 36.0 / 31.9 / 32.1 with up to 12, and 64 of 4096 the same to 1 %.
 // `pref`: word b = (steps of one head unit of the sequences before b) << kRemBits | tokens in its last tile - 1.
 constexpr int kSwitch = 12;
 __device__ __forceinline__ int unit_tiles(int steps) { return max(steps - kSwitch, 0); }
