@@ -226,46 +226,56 @@ int tkv_combine_exchange(const float* acc, const float* m, const float* l, float
  * block_table[b*table_stride + n / page_size]; an entry outside [0, num_pages) names no page.
  * block_table, seq_lens, positions, lengths, parents and reserve are int32 device pointers.
  *
+ * The calls take their arguments in a struct, every field filled in.
+ *
  * Decode attention over a paged cache: sequence b attends its first seq_lens[b] tokens (clamped
  * to max_pages*page_size), without those of entries that name no page; with none left its rows
  * of out are zero.  q as in tkv_fused_decode; out (B, HQ, D) of out_dtype.  page_size is a
- * multiple of 16; D is 64 or 128; gs in {16,32,64,128}, at most D. */
-int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_packed, const void* k_scale,
-                     const void* k_zero, const uint8_t* v_packed, const void* v_scale,
-                     const void* v_zero, const int32_t* block_table, int64_t table_stride,
-                     const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
-                     int64_t workspace_bytes, uint32_t* tickets, int B, int HQ, int HKV, int num_pages,
-                     int page_size, int max_pages, int D, int nbits, int gs, float sm_scale, void* stream);
-int tkv_paged_fp16_decode(const void* q, int q_dtype, const void* k, const void* v,
-                          const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
-                          void* out, int out_dtype, void* workspace, int64_t workspace_bytes,
-                          uint32_t* tickets, int B, int HQ, int HKV, int num_pages, int page_size, int max_pages, int D,
-                          float sm_scale, void* stream);
-
-/* Bytes of device workspace (partials of the split history) that the two calls above need on the
- * current device; nbits = 16 for the f16 form.  tickets: null, or TKV_PAGED_TICKETS words of the
- * caller's that are zero before their first use and that every call leaves zero (unless it ends
- * with a nonzero tkv_device_status): with them, units of few partials are merged by the split
- * kernel itself, a launch less.  Calls that may run at the same time need workspaces and tickets
- * of their own. */
+ * multiple of 16; D is 64 or 128; gs in {16,32,64,128}, at most D.  nbits = 16: f16 pages, k and v
+ * are the pools and the scales and zeros are not looked at.
+ * workspace: tkv_paged_workspace bytes.  tickets: null, or TKV_PAGED_TICKETS words of the caller's
+ * that are zero before their first use and that every call leaves zero (unless it ends with a
+ * nonzero tkv_device_status): with them, units of few partials are merged by the split kernel
+ * itself, a launch less.  Calls that may run at the same time need workspaces and tickets of
+ * their own. */
 #define TKV_PAGED_TICKETS 8192
+typedef struct {
+  const void *q, *k, *k_scale, *k_zero, *v, *v_scale, *v_zero;
+  const int32_t *block_table, *seq_lens;
+  void *out, *workspace;
+  uint32_t* tickets;
+  int64_t table_stride, workspace_bytes;
+  int q_dtype, out_dtype, B, HQ, HKV, num_pages, page_size, max_pages, D, nbits, gs;
+  float sm_scale;
+} tkv_paged_decode_args;
+int tkv_paged_decode(const tkv_paged_decode_args* a, void* stream);
+
+/* Bytes of device workspace (partials of the split history) that tkv_paged_decode needs on the
+ * current device. */
 int tkv_paged_workspace(int B, int HQ, int HKV, int page_size, int D, int nbits, int gs,
                         int64_t* bytes);
 
 /* Quantise T new tokens per (sequence, head) of K and of V -- element (b, h, t, d) of k at
  * strides[0]*b + strides[1]*h + strides[2]*t + d, of v with strides[3..5] -- into their pages, at
- * positions[b] + t (or pos0 + t), for t < lengths[b] (all T if null).  The bytes are those of
- * tkv_quantize_pack.  nbits = 16: f16 pages, k_packed and v_packed are the pools and scale / zero
- * are null.  k_values / v_values (null or of in_dtype, value_strides laid out like strides)
+ * positions[b] + t (pos0 + t if null), for t < lengths[b] (all T if null).  The bytes are those of
+ * tkv_quantize_pack.  nbits = 16: f16 pages, k_pool and v_pool are the pools and scale / zero are
+ * not looked at.  k_values / v_values (null or of in_dtype, value_strides laid out like strides)
  * receive code*scale + zero.  Positions outside the table and entries that name no page drop
  * their tokens. */
-int tkv_paged_append(const void* k, const void* v, int in_dtype, const int64_t* strides,
-                     uint8_t* k_packed, void* k_scale, void* k_zero, uint8_t* v_packed,
-                     void* v_scale, void* v_zero, void* k_values, void* v_values,
-                     const int64_t* value_strides, const int32_t* block_table, int64_t table_stride,
-                     const int32_t* positions, int pos0, const int32_t* lengths, int B, int HKV, int T,
-                     int num_pages, int page_size, int max_pages, int D, int nbits, int gs,
-                     void* stream);
+typedef struct {
+  const void *k, *v;
+  void *k_pool, *k_scale, *k_zero, *v_pool, *v_scale, *v_zero, *k_values, *v_values;
+  const int32_t *block_table, *positions, *lengths;
+  int64_t strides[6], value_strides[6], table_stride;
+  int in_dtype, pos0, B, HKV, T, num_pages, page_size, max_pages, D, nbits, gs;
+} tkv_paged_append_args;
+int tkv_paged_append(const tkv_paged_append_args* a, void* stream);
+
+/* One tensor whose pages move: its base and the bytes of a page. */
+typedef struct {
+  void* base;
+  int64_t page_bytes;
+} tkv_page_pool;
 
 /* 32-bit words of device workspace that tkv_pages_fork (B rows of the new table) and
  * tkv_pages_compact need.  It is zero before its first use, serves one num_pages (its first words
@@ -275,21 +285,28 @@ int tkv_pages_workspace(int B, int num_pages, int64_t* words);
 /* New table (B, max_pages) and lengths (B,) whose row b continues row parents[b] of the old ones
  * (B_old rows of max_pages entries, table_stride apart): full pages shared, a partly filled page
  * kept by the first row that continues this parent and copied for the others in all n_pools
- * tensors of page_bytes[i] per page, pages added for reserve[b] (or reserve0) further
- * tokens.  Fresh pages are the lowest that no kept entry names, in order of (row, position);
- * `missing` (1,) receives how many the pool was short of.  The outputs must not overlap the
- * inputs. */
-int tkv_pages_fork(const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
-                   int B_old, const int32_t* parents, const int32_t* reserve, int reserve0, int B,
-                   int max_pages, int num_pages, int page_size, int32_t* new_table, int32_t* new_lens,
-                   int32_t* missing, int32_t* workspace, void* const* pools,
-                   const int64_t* page_bytes, int n_pools, void* stream);
+ * tensors, pages added for reserve[b] (reserve0 if null) further tokens.  Fresh pages are the
+ * lowest that no kept entry names, in order of (row, position); `missing` (1,) receives how many
+ * the pool was short of.  The outputs must not overlap the inputs. */
+typedef struct {
+  const int32_t *block_table, *seq_lens, *parents, *reserve;
+  int32_t *new_table, *new_lens, *missing, *workspace;
+  int64_t table_stride;
+  int B_old, reserve0, B, max_pages, num_pages, page_size;
+} tkv_pages_fork_args;
+int tkv_pages_fork(const tkv_pages_fork_args* a, const tkv_page_pool* pools, int n_pools,
+                   void* stream);
 
 /* With n pages named by the table (B, max_pages), move the k-th named page at or above n to the
  * k-th unnamed one below n in all pools; new_table has the new numbers, `live` (1,) receives n. */
-int tkv_pages_compact(const int32_t* block_table, int64_t table_stride, int B, int max_pages,
-                      int num_pages, int32_t* new_table, int32_t* live, int32_t* workspace,
-                      void* const* pools, const int64_t* page_bytes, int n_pools, void* stream);
+typedef struct {
+  const int32_t* block_table;
+  int32_t *new_table, *live, *workspace;
+  int64_t table_stride;
+  int B, max_pages, num_pages;
+} tkv_pages_compact_args;
+int tkv_pages_compact(const tkv_pages_compact_args* a, const tkv_page_pool* pools, int n_pools,
+                      void* stream);
 
 /* Device-side status word of the current device (synchronises with it): 0 = ok,
  * bit 0 = a bounded wait on a copy barrier inside a decode kernel gave up (the kernel then

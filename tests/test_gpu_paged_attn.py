@@ -275,10 +275,10 @@ def test_too_small_a_workspace_is_refused():
 
     k, v, table, NP = make_pools([64], 1, 64, 4, 32, 16, seed=1)
     q, sl, out = make_q(1, 2, 64, 0), lens_t([64]), torch.empty(1, 2, 64, device=DEV)
-    rc = _cabi.load().tkv_paged_decode(
-        q.data_ptr(), 0, *(t.data_ptr() for p in (k, v) for t in (p.packed, p.scale, p.zero)), table.data_ptr(),
-        table.stride(0), sl.data_ptr(), out.data_ptr(), 2, out.data_ptr(), 64, None, 1, 2, 1, NP, 16, table.shape[1], 64, 4,
-        32, 0.125, _cabi.stream_ptr(q.device))
+    pools = [t.data_ptr() for p in (k, v) for t in (p.packed, p.scale, p.zero)]
+    rc = _cabi.load().tkv_paged_decode(_cabi.PAGED_DECODE_ARGS.pack(
+        q.data_ptr(), *pools, table.data_ptr(), sl.data_ptr(), out.data_ptr(), out.data_ptr(), 0, table.stride(0), 64, 0, 2, 1,
+        2, 1, NP, 16, table.shape[1], 64, 4, 32, 0.125), _cabi.stream_ptr(q.device))
     assert rc == _cabi.TKV_ERR_INVALID and "tkv_paged_workspace" in _cabi.last_error()
 
 

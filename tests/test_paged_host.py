@@ -1,6 +1,7 @@
 """What the paged-cache functions refuse, checked without a GPU."""
 
-import ctypes
+import os
+import struct
 
 import pytest
 import torch
@@ -147,37 +148,68 @@ def test_c_entries_refuse():
     """Argument errors of the C ABI come back before any launch."""
     lib, P = _cabi.load(), 4096  # a pointer that nothing follows: every call fails before that
 
-    def decode(q=P, out=P, B=1, HQ=4, HKV=2, NP=8, page=16, W=4, D=64, nbits=4, gs=32, dt=0, scale=P):
-        return lib.tkv_paged_decode(q, dt, P, scale, P, P, P, P, P, W, P, out, 0, P, 1 << 30, None, B, HQ, HKV, NP, page, W, D, nbits, gs, 1.0, None)
+    def decode(q=P, out=P, B=1, HQ=4, HKV=2, NP=8, page=16, W=4, D=64, nbits=4, gs=32, dt=0, scale=P, v=P):
+        return lib.tkv_paged_decode(_cabi.PAGED_DECODE_ARGS.pack(q, P, scale, P, v, P, P, P, P, out, P, 0, W, 1 << 30, dt, 0, B,
+                                                                 HQ, HKV, NP, page, W, D, nbits, gs, 1.0), None)
 
     I, U, A = _cabi.TKV_ERR_INVALID, _cabi.TKV_ERR_UNSUPPORTED, _cabi.TKV_ERR_ALIGN
-    for rc, kw in ((I, dict(q=None)), (I, dict(B=0)), (I, dict(HQ=5)), (I, dict(NP=0)), (I, dict(nbits=3)), (I, dict(dt=7)),
+    for rc, kw in ((I, dict(q=0)), (I, dict(B=0)), (I, dict(HQ=5)), (I, dict(NP=0)), (I, dict(nbits=3)), (I, dict(dt=7)),
                    (I, dict(NP=1 << 27)), (I, dict(W=1 << 27)), (U, dict(page=24)), (U, dict(D=96)), (U, dict(gs=8)),
-                   (U, dict(gs=128)), (A, dict(q=P + 8)), (A, dict(scale=P + 2)), (A, dict(out=P + 4))):
+                   (U, dict(gs=128)), (A, dict(q=P + 8)), (A, dict(scale=P + 2)), (A, dict(out=P + 4)), (I, dict(scale=0)),
+                   (I, dict(nbits=16, v=0)), (A, dict(nbits=16, v=P + 2)), (U, dict(nbits=16, D=32))):
         assert decode(**kw) == rc, (kw, _cabi.last_error())
-    assert lib.tkv_paged_fp16_decode(P, 0, P, None, P, 4, P, P, 0, P, 1 << 30, None, 1, 4, 2, 8, 16, 4, 64, 1.0, None) == I
-    i6 = (ctypes.c_int64 * 6)(*[64] * 6)
+    assert lib.tkv_paged_decode(None, None) == I
 
-    def append(k=P, st=i6, B=1, T=1, D=64, nbits=4, gs=32, dt=0, val=None, vs=None, scale=P):
-        return lib.tkv_paged_append(k, P, dt, st, P, scale, P, P, P, P, val, None, vs, P, 4, None, 0, None, B, 2, T, 8, 16, 4, D,
-                                    nbits, gs, None)
+    def append(k=P, st=64, B=1, T=1, D=64, nbits=4, gs=32, dt=0, val=0, vst=64, scale=P):
+        return lib.tkv_paged_append(_cabi.PAGED_APPEND_ARGS.pack(k, P, P, scale, P, P, P, P, val, 0, P, 0, 0, *[st] * 6,
+                                                                 *[vst] * 6, 4, dt, 0, B, 2, T, 8, 16, 4, D, nbits, gs), None)
 
-    odd = (ctypes.c_int64 * 6)(*[63] * 6)
-    for rc, kw in ((I, dict(k=None)), (I, dict(nbits=3)), (I, dict(B=-1)), (I, dict(dt=5)), (I, dict(scale=None)),
-                   (I, dict(val=P)), (U, dict(D=48)), (U, dict(gs=4)), (U, dict(gs=128)), (U, dict(D=16, gs=16, nbits=2)),
-                   (A, dict(st=odd)), (A, dict(k=P + 2)), (I, dict(T=1 << 30, B=4))):
+    for rc, kw in ((I, dict(k=0)), (I, dict(nbits=3)), (I, dict(B=-1)), (I, dict(dt=5)), (I, dict(scale=0)),
+                   (U, dict(D=48)), (U, dict(gs=4)), (U, dict(gs=128)), (U, dict(D=16, gs=16, nbits=2)), (A, dict(st=63)),
+                   (A, dict(val=P, vst=63)), (A, dict(k=P + 2)), (I, dict(T=1 << 30, B=4))):
         assert append(**kw) == rc, (kw, _cabi.last_error())
-    assert append(B=0) == 0 and append(T=0) == 0
-    ptrs, sizes = (ctypes.c_void_p * 1)(P), (ctypes.c_int64 * 1)(64)
+    assert append(B=0) == 0 and append(T=0) == 0 and lib.tkv_paged_append(None, None) == I
+    one = struct.pack("2q", P, 64)
 
-    def fork(B=2, Bo=2, W=4, NP=8, page=16, par=P, ws=P, pools=ptrs, n=1):
-        return lib.tkv_pages_fork(P, W, P, Bo, par, None, 0, B, W, NP, page, P, P, P, ws, pools, sizes, n, None)
+    def fork(B=2, Bo=2, W=4, NP=8, page=16, par=P, ws=P, pools=one, n=1):
+        return lib.tkv_pages_fork(_cabi.PAGES_FORK_ARGS.pack(P, P, par, 0, P, P, P, ws, W, Bo, 0, B, W, NP, page), pools, n, None)
 
-    for kw in (dict(par=None), dict(ws=None), dict(NP=0), dict(page=0), dict(B=-1), dict(W=1 << 29), dict(pools=None), dict(n=-1)):
+    for kw in (dict(par=0), dict(ws=0), dict(NP=0), dict(page=0), dict(B=-1), dict(W=1 << 29), dict(pools=None), dict(n=-1),
+               dict(pools=struct.pack("2q", 0, 64)), dict(pools=struct.pack("2q", P, 0))):
         assert fork(**kw) == I, (kw, _cabi.last_error())
+    assert lib.tkv_pages_fork(None, one, 1, None) == I
 
     def compact(B=2, W=4, NP=8, live=P, n=1):
-        return lib.tkv_pages_compact(P, W, B, W, NP, P, live, P, ptrs, sizes, n, None)
+        return lib.tkv_pages_compact(_cabi.PAGES_COMPACT_ARGS.pack(P, P, live, P, W, B, W, NP), one, n, None)
 
-    for kw in (dict(B=-1), dict(NP=0), dict(live=None), dict(W=1 << 29), dict(n=-1)):
+    for kw in (dict(B=-1), dict(NP=0), dict(live=0), dict(W=1 << 29), dict(n=-1)):
         assert compact(**kw) == I, (kw, _cabi.last_error())
+    assert lib.tkv_pages_compact(None, one, 1, None) == I
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    """The packed layouts of the binding against the compiler's, field by field."""
+    import shutil
+    import subprocess
+
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no C compiler")
+    fields = {"tkv_paged_decode_args": ("workspace", "tickets", "table_stride", "workspace_bytes", "q_dtype", "gs", "sm_scale"),
+              "tkv_paged_append_args": ("k", "lengths", "strides", "value_strides", "table_stride", "in_dtype", "gs"),
+              "tkv_pages_fork_args": ("reserve", "workspace", "table_stride", "B_old", "page_size"),
+              "tkv_pages_compact_args": ("workspace", "table_stride", "B", "num_pages")}
+    src = tmp_path / "t.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "tritonkv_b200.h"\nint main(void) {\n' + "".join(
+        f'printf("%zu\\n", offsetof({t}, {f}));\n' for t, fs in fields.items() for f in fs) + "return 0; }\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = tmp_path / "t"
+    subprocess.run([gcc, "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    at = lambda form: struct.calcsize("@" + form)  # the offset of what follows `form`
+    want = [at("10P"), at("11P"), at("12P"), at("12Pq"), at("12P2q"), at("12P2q10i"), at("12P2q11i"),
+            0, at("12P"), at("13P"), at("13P6q"), at("13P12q"), at("13P13q"), at("13P13q10i"),
+            at("3P"), at("7P"), at("8P"), at("8Pq"), at("8Pq5i"), at("3P"), at("4P"), at("4Pq"), at("4Pq2i")]
+    assert got == want
+    assert _cabi.PAGED_DECODE_ARGS.size == at("12P2q11if") and _cabi.PAGED_APPEND_ARGS.size == at("13P13q11i")
+    assert _cabi.PAGES_FORK_ARGS.size == at("8Pq6i") and _cabi.PAGES_COMPACT_ARGS.size == at("4Pq3i")

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p, POINTER
 
 import torch
@@ -30,6 +31,14 @@ KERNEL_FUSED_SPLIT, KERNEL_FP16_SPLIT = 0, 1
 KERNEL_FUSED_SPLIT_KCHAN = 4
 
 _TORCH_DTYPE = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
+
+# The argument structs of the paged-cache entries, packed field by field: pointers, 64-bit words, ints
+# (and a float) in the order of their declarations, so there is no padding.  One packed argument costs a
+# fraction of converting two dozen.
+PAGED_DECODE_ARGS = struct.Struct("@12P2q11if")
+PAGED_APPEND_ARGS = struct.Struct("@13P13q11i")
+PAGES_FORK_ARGS = struct.Struct("@8Pq6i")
+PAGES_COMPACT_ARGS = struct.Struct("@4Pq3i")
 
 # Every symbol include/tritonkv_b200.h declares: (restype, argtypes).
 SIGNATURES = {
@@ -76,24 +85,12 @@ SIGNATURES = {
     "tkv_fused_decode_static": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                         c_int, c_int, c_int, c_float, c_void_p]),
-    "tkv_paged_decode": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                 c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64,
-                                 c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
-                                 c_void_p]),
-    "tkv_paged_fp16_decode": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
-                                      c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
-                                      c_int, c_int, c_int, c_float, c_void_p]),
+    "tkv_paged_decode": (c_int, [c_void_p, c_void_p]),
     "tkv_paged_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
-    "tkv_paged_append": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                 c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
-                                 c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "tkv_paged_append": (c_int, [c_void_p, c_void_p]),
     "tkv_pages_workspace": (c_int, [c_int, c_int, POINTER(c_int64)]),
-    "tkv_pages_fork": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
-                               c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                               c_void_p, c_int, c_void_p]),
-    "tkv_pages_compact": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
-                                  c_void_p, c_void_p, c_int, c_void_p]),
+    "tkv_pages_fork": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
+    "tkv_pages_compact": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
 }
 
 _lib = None
@@ -271,28 +268,32 @@ _paged_bytes: dict = {}
 PAGED_TICKETS = 8192
 
 
-def paged_workspace(ws: dict | None, B: int, HQ: int, HKV: int, page: int, D: int, nbits: int, gs: int,
-                    device) -> tuple:
-    """(partials, their bytes, address of the tickets, tickets) of a paged decode call, kept in the caller's
-    dict ``ws`` (key ``paged``).  The tickets are zero at first, and left zero by every call."""
-    key = (B, HQ, HKV, page, D, nbits, gs, _current_device())
+def paged_workspace(ws: dict | None, key: tuple, device) -> tuple:
+    """(key, address of the partials, their bytes, address of the tickets, partials, tickets) of a paged decode
+    call with ``key`` = (B, HQ, HKV, page, D, nbits, group_size, device index), kept in the caller's dict
+    ``ws`` (as ``paged``).  The tickets are zero at first, and left zero by every call."""
+    kept = None if ws is None else ws.get("paged")
+    if kept is not None and kept[0] == key:
+        return kept
     need = _paged_bytes.get(key)
     if need is None:
         v = c_int64(0)
-        check(load().tkv_paged_workspace(B, HQ, HKV, page, D, nbits, gs, ctypes.byref(v)))
+        check(load().tkv_paged_workspace(*key[:7], ctypes.byref(v)))
         need = v.value
         if len(_paged_bytes) < 4096:
             _paged_bytes[key] = need
-    kept = None if ws is None else ws.get("paged")
-    if kept is None or kept[1] < need or kept[0].device != device:
+    if kept is not None and kept[2] >= need and kept[0][7] == key[7]:
+        kept = (key, *kept[1:])
+    else:
         # what a captured graph may still use stays with the dict: the tickets, and smaller buffers
         if kept is not None:
             ws.setdefault("outgrown", []).append(kept)
-        tickets = kept[3] if kept is not None and kept[0].device == device else torch.zeros(
+        tickets = kept[5] if kept is not None and kept[0][7] == key[7] else torch.zeros(
             PAGED_TICKETS, dtype=torch.int32, device=device)
-        kept = (torch.empty(need, dtype=torch.uint8, device=device), need, tickets.data_ptr(), tickets)
-        if ws is not None:
-            ws["paged"] = kept
+        partials = torch.empty(need, dtype=torch.uint8, device=device)
+        kept = (key, partials.data_ptr(), need, tickets.data_ptr(), partials, tickets)
+    if ws is not None:
+        ws["paged"] = kept
     return kept
 
 

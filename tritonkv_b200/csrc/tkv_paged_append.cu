@@ -230,20 +230,17 @@ static int launch_append(const AppendArgs& a, int D, int nbits, int gs, cudaStre
 
 }  // namespace tkv
 
-extern "C" int tkv_paged_append(const void* k, const void* v, int in_dtype, const int64_t* strides,
-                                uint8_t* k_packed, void* k_scale, void* k_zero, uint8_t* v_packed,
-                                void* v_scale, void* v_zero, void* k_values, void* v_values,
-                                const int64_t* value_strides, const int32_t* block_table,
-                                int64_t table_stride, const int32_t* positions, int pos0,
-                                const int32_t* lengths, int B, int HKV, int T, int num_pages, int page_size,
-                                int max_pages, int D, int nbits, int gs, void* stream) {
+extern "C" int tkv_paged_append(const tkv_paged_append_args* args, void* stream) {
   using namespace tkv;
+  TKV_REQUIRE(args, TKV_ERR_INVALID, "paged append: null arguments");
+  const tkv_paged_append_args& in = *args;
+  const int nbits = in.nbits, D = in.D, gs = in.gs;
   TKV_REQUIRE(nbits == 2 || nbits == 4 || nbits == 16, TKV_ERR_INVALID,
               "paged append: nbits must be 2, 4 or 16 (float16 pages), got %d", nbits);
-  TKV_REQUIRE(B >= 0 && HKV > 0 && T >= 0 && num_pages > 0 && page_size > 0 && max_pages >= 0, TKV_ERR_INVALID,
-              "paged append: bad sizes B=%d HKV=%d T=%d num_pages=%d page_size=%d max_pages=%d", B, HKV, T,
-              num_pages, page_size, max_pages);
-  TKV_REQUIRE(in_dtype >= 0 && in_dtype <= 2, TKV_ERR_INVALID, "paged append: bad dtype %d", in_dtype);
+  TKV_REQUIRE(in.B >= 0 && in.HKV > 0 && in.T >= 0 && in.num_pages > 0 && in.page_size > 0 && in.max_pages >= 0,
+              TKV_ERR_INVALID, "paged append: bad sizes B=%d HKV=%d T=%d num_pages=%d page_size=%d max_pages=%d", in.B,
+              in.HKV, in.T, in.num_pages, in.page_size, in.max_pages);
+  TKV_REQUIRE(in.in_dtype >= 0 && in.in_dtype <= 2, TKV_ERR_INVALID, "paged append: bad dtype %d", in.in_dtype);
   TKV_REQUIRE(is_pow2(D) && D >= 16 && D <= 256, TKV_ERR_UNSUPPORTED,
               "paged append: unsupported head_dim=%d (a power of two from 16 to 256)", D);
   if (nbits != 16) {
@@ -252,51 +249,49 @@ extern "C" int tkv_paged_append(const void* k, const void* v, int in_dtype, cons
     TKV_REQUIRE((D * nbits / 8) % 8 == 0, TKV_ERR_UNSUPPORTED,
                 "paged append: packed row of %d bytes is not a multiple of 8", D * nbits / 8);
   }
-  if (B == 0 || T == 0 || max_pages == 0) return TKV_OK;
-  TKV_REQUIRE(k && v && strides && k_packed && v_packed && block_table, TKV_ERR_INVALID,
-              "paged append: null pointer");
-  TKV_REQUIRE(nbits == 16 || (k_scale && k_zero && v_scale && v_zero), TKV_ERR_INVALID,
+  if (in.B == 0 || in.T == 0 || in.max_pages == 0) return TKV_OK;
+  TKV_REQUIRE(in.k && in.v && in.k_pool && in.v_pool && in.block_table, TKV_ERR_INVALID, "paged append: null pointer");
+  TKV_REQUIRE(nbits == 16 || (in.k_scale && in.k_zero && in.v_scale && in.v_zero), TKV_ERR_INVALID,
               "paged append: null scale or zero pointer");
-  TKV_REQUIRE((k_values == nullptr && v_values == nullptr) || value_strides, TKV_ERR_INVALID,
-              "paged append: values need their strides");
-  const int al = in_dtype == TKV_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+  const int al = in.in_dtype == TKV_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
   for (int i = 0; i < 6; ++i)
-    TKV_REQUIRE(strides[i] % al == 0 && ((i < 3 ? k_values : v_values) == nullptr || value_strides[i] % al == 0),
+    TKV_REQUIRE(in.strides[i] % al == 0 && ((i < 3 ? in.k_values : in.v_values) == nullptr || in.value_strides[i] % al == 0),
                 TKV_ERR_ALIGN, "paged append: rows of the new tokens must start on 16-byte boundaries");
-  TKV_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_packed) && aligned16(v_packed) && aligned16(k_values) &&
-                  aligned16(v_values), TKV_ERR_ALIGN, "paged append: pointers must be 16-byte aligned");
-  TKV_REQUIRE((int64_t)max_pages * page_size < (1LL << 30), TKV_ERR_INVALID,
-              "paged append: a table row of %lld tokens exceeds 2^30", (long long)max_pages * page_size);
-  TKV_REQUIRE((int64_t)B * HKV * T < (1LL << 31) - 4096, TKV_ERR_INVALID, "paged append: %lld token rows exceed 2^31",
-              (long long)B * HKV * T);
-  TKV_REQUIRE((int64_t)num_pages * HKV * page_size < (1LL << 31), TKV_ERR_INVALID,
-              "paged append: a pool of %lld token rows exceeds 2^31", (long long)num_pages * HKV * page_size);
+  TKV_REQUIRE(aligned16(in.k) && aligned16(in.v) && aligned16(in.k_pool) && aligned16(in.v_pool) &&
+                  aligned16(in.k_values) && aligned16(in.v_values), TKV_ERR_ALIGN,
+              "paged append: pointers must be 16-byte aligned");
+  TKV_REQUIRE((int64_t)in.max_pages * in.page_size < (1LL << 30), TKV_ERR_INVALID,
+              "paged append: a table row of %lld tokens exceeds 2^30", (long long)in.max_pages * in.page_size);
+  TKV_REQUIRE((int64_t)in.B * in.HKV * in.T < (1LL << 31) - 4096, TKV_ERR_INVALID,
+              "paged append: %lld token rows exceed 2^31", (long long)in.B * in.HKV * in.T);
+  TKV_REQUIRE((int64_t)in.num_pages * in.HKV * in.page_size < (1LL << 31), TKV_ERR_INVALID,
+              "paged append: a pool of %lld token rows exceeds 2^31", (long long)in.num_pages * in.HKV * in.page_size);
   AppendArgs a{};
-  a.t[0] = {k, k_packed, (__half*)k_scale, (__half*)k_zero, k_values, strides[0], strides[1], strides[2], 0, 0, 0, 0};
-  a.t[1] = {v, v_packed, (__half*)v_scale, (__half*)v_zero, v_values, strides[3], strides[4], strides[5], 0, 0, 0, 0};
-  if (k_values) a.t[0].vb = value_strides[0], a.t[0].vh = value_strides[1], a.t[0].vt = value_strides[2];
-  if (v_values) a.t[1].vb = value_strides[3], a.t[1].vh = value_strides[4], a.t[1].vt = value_strides[5];
+  a.t[0] = {in.k, (uint8_t*)in.k_pool, (__half*)in.k_scale, (__half*)in.k_zero, in.k_values, 0, 0, 0, 0, 0, 0, 0};
+  a.t[1] = {in.v, (uint8_t*)in.v_pool, (__half*)in.v_scale, (__half*)in.v_zero, in.v_values, 0, 0, 0, 0, 0, 0, 0};
   for (int i = 0; i < 2; ++i) {
-    const AppendTensor& t = a.t[i];
-    a.t[i].values32 = in_dtype != TKV_DTYPE_F32 && ((uintptr_t)t.values & 31) == 0 && t.vb % 16 == 0 && t.vh % 16 == 0 &&
-                      t.vt % 16 == 0;
+    AppendTensor& t = a.t[i];
+    t.sb = in.strides[3 * i], t.sh = in.strides[3 * i + 1], t.st = in.strides[3 * i + 2];
+    if (t.values) t.vb = in.value_strides[3 * i], t.vh = in.value_strides[3 * i + 1], t.vt = in.value_strides[3 * i + 2];
+    t.values32 = in.in_dtype != TKV_DTYPE_F32 && ((uintptr_t)t.values & 31) == 0 && t.vb % 16 == 0 && t.vh % 16 == 0 &&
+                 t.vt % 16 == 0;
   }
-  a.table = block_table;
-  a.positions = positions;
-  a.lengths = lengths;
-  a.table_stride = table_stride;
-  a.pos0 = pos0;
-  a.B = B;
-  a.HKV = HKV;
-  a.T = T;
-  a.dpage = make_fastdiv(page_size);
-  a.dT = make_fastdiv(T);
-  a.dHKV = make_fastdiv(HKV);
-  a.num_pages = num_pages;
-  a.page = page_size;
-  a.limit = max_pages * page_size;
+  a.table = in.block_table;
+  a.positions = in.positions;
+  a.lengths = in.lengths;
+  a.table_stride = in.table_stride;
+  a.pos0 = in.pos0;
+  a.B = in.B;
+  a.HKV = in.HKV;
+  a.T = in.T;
+  a.dpage = make_fastdiv(in.page_size);
+  a.dT = make_fastdiv(in.T);
+  a.dHKV = make_fastdiv(in.HKV);
+  a.num_pages = in.num_pages;
+  a.page = in.page_size;
+  a.limit = in.max_pages * in.page_size;
   cudaStream_t s = (cudaStream_t)stream;
-  if (in_dtype == TKV_DTYPE_F16) return launch_append<__half>(a, D, nbits, gs, s);
-  if (in_dtype == TKV_DTYPE_BF16) return launch_append<__nv_bfloat16>(a, D, nbits, gs, s);
+  if (in.in_dtype == TKV_DTYPE_F16) return launch_append<__half>(a, D, nbits, gs, s);
+  if (in.in_dtype == TKV_DTYPE_BF16) return launch_append<__nv_bfloat16>(a, D, nbits, gs, s);
   return launch_append<float>(a, D, nbits, gs, s);
 }

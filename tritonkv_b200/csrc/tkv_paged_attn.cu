@@ -1061,56 +1061,58 @@ int paged_device_status_clear() {
   return TKV_OK;
 }
 
-// Checks shared by the two entry points; fills everything but the pools.
-static int paged_fill(const char* who, PagedCall& c, const void* q, int q_dtype, const int32_t* table,
-                      int64_t table_stride, const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
-                      int64_t workspace_bytes, uint32_t* tickets, int B, int HQ, int HKV, int num_pages, int page,
-                      int max_pages, int D, float sm_scale) {
-  TKV_REQUIRE(B > 0 && HQ > 0 && HKV > 0 && HQ % HKV == 0, TKV_ERR_INVALID,
-              "%s: bad sizes B=%d HQ=%d HKV=%d (HQ must be a multiple of HKV)", who, B, HQ, HKV);
-  TKV_REQUIRE(num_pages > 0 && page > 0 && max_pages >= 0, TKV_ERR_INVALID,
-              "%s: bad sizes num_pages=%d page_size=%d max_pages=%d", who, num_pages, page, max_pages);
-  TKV_REQUIRE(page % 16 == 0, TKV_ERR_UNSUPPORTED, "%s: unsupported page_size=%d (a multiple of 16 tokens)", who, page);
-  TKV_REQUIRE((int64_t)num_pages * HKV * page < (1LL << 31), TKV_ERR_INVALID,
-              "%s: a pool of %lld token rows exceeds 2^31", who, (long long)num_pages * HKV * page);
-  TKV_REQUIRE((int64_t)max_pages * page < (1LL << 30), TKV_ERR_INVALID,
-              "%s: a table row of %lld tokens exceeds 2^30", who, (long long)max_pages * page);
-  TKV_REQUIRE((int64_t)kMaxPagedB * HQ < (1LL << 31), TKV_ERR_INVALID, "%s: HQ=%d is too large", who, HQ);
-  TKV_REQUIRE(q_dtype >= 0 && q_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, TKV_ERR_INVALID,
-              "%s: bad dtype codes %d, %d", who, q_dtype, out_dtype);
-  TKV_REQUIRE(q && seq_lens && out && (table || max_pages == 0), TKV_ERR_INVALID, "%s: null pointer", who);
-  TKV_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace), TKV_ERR_ALIGN,
-              "%s: q, out and the workspace must be 16-byte aligned", who);
+static int paged_fill(PagedCall& c, const tkv_paged_decode_args& a) {
+  TKV_REQUIRE(a.nbits == 2 || a.nbits == 4 || a.nbits == 16, TKV_ERR_INVALID,
+              "paged decode: nbits must be 2, 4 or 16 (float16 pages), got %d", a.nbits);
+  TKV_REQUIRE(a.B > 0 && a.HQ > 0 && a.HKV > 0 && a.HQ % a.HKV == 0, TKV_ERR_INVALID,
+              "paged decode: bad sizes B=%d HQ=%d HKV=%d (HQ must be a multiple of HKV)", a.B, a.HQ, a.HKV);
+  TKV_REQUIRE(a.num_pages > 0 && a.page_size > 0 && a.max_pages >= 0, TKV_ERR_INVALID,
+              "paged decode: bad sizes num_pages=%d page_size=%d max_pages=%d", a.num_pages, a.page_size, a.max_pages);
+  TKV_REQUIRE(a.page_size % 16 == 0, TKV_ERR_UNSUPPORTED, "paged decode: unsupported page_size=%d (a multiple of 16 tokens)",
+              a.page_size);
+  TKV_REQUIRE((int64_t)a.num_pages * a.HKV * a.page_size < (1LL << 31), TKV_ERR_INVALID,
+              "paged decode: a pool of %lld token rows exceeds 2^31", (long long)a.num_pages * a.HKV * a.page_size);
+  TKV_REQUIRE((int64_t)a.max_pages * a.page_size < (1LL << 30), TKV_ERR_INVALID,
+              "paged decode: a table row of %lld tokens exceeds 2^30", (long long)a.max_pages * a.page_size);
+  TKV_REQUIRE((int64_t)kMaxPagedB * a.HQ < (1LL << 31), TKV_ERR_INVALID, "paged decode: HQ=%d is too large", a.HQ);
+  TKV_REQUIRE(a.q_dtype >= 0 && a.q_dtype <= 2 && a.out_dtype >= 0 && a.out_dtype <= 2, TKV_ERR_INVALID,
+              "paged decode: bad dtype codes %d, %d", a.q_dtype, a.out_dtype);
+  TKV_REQUIRE(a.q && a.seq_lens && a.out && a.k && a.v && (a.block_table || a.max_pages == 0) &&
+                  (a.nbits == 16 || (a.k_scale && a.k_zero && a.v_scale && a.v_zero)),
+              TKV_ERR_INVALID, "paged decode: null pointer");
+  TKV_REQUIRE(aligned16(a.q) && aligned16(a.out) && aligned16(a.workspace) && aligned16(a.k) && aligned16(a.v) &&
+                  (a.nbits == 16 || (aligned16(a.k_scale) && aligned16(a.k_zero) && aligned16(a.v_scale) && aligned16(a.v_zero))),
+              TKV_ERR_ALIGN, "paged decode: q, out, the workspace and the pools must be 16-byte aligned");
   c = PagedCall{};
-  c.B = B;
-  c.workspace = workspace;
-  c.workspace_bytes = workspace_bytes;
-  c.tickets = tickets;
+  c.B = a.B;
+  c.workspace = a.workspace;
+  c.workspace_bytes = a.workspace_bytes;
+  c.tickets = a.tickets;
   PagedParams& pp = c.pp;
   DecodeParams& p = pp.d;
-  p.q = q;
-  p.q_dtype = q_dtype;
-  p.seq_lens = seq_lens;
-  p.HQ = HQ;
-  p.HKV = HKV;
-  p.S = max_pages * page;
-  p.group = HQ / HKV;
+  p.q = a.q;
+  p.q_dtype = a.q_dtype;
+  p.seq_lens = a.seq_lens;
+  p.HQ = a.HQ;
+  p.HKV = a.HKV;
+  p.S = a.max_pages * a.page_size;
+  p.group = a.HQ / a.HKV;
   p.hchunks = (p.group + kHeadsPerCta - 1) / kHeadsPerCta;
-  p.qk_scale = sm_scale * kLog2e;
+  p.qk_scale = a.sm_scale * kLog2e;
   p.meta_aligned = 16;
   p.wide = 1;
-  pp.table = table;
-  pp.table_stride = table_stride;
-  pp.out = out;
-  pp.out_dtype = out_dtype;
-  pp.num_pages = num_pages;
-  pp.page = page;
-  pp.max_pages = max_pages;
-  pp.HKVc = HKV * p.hchunks;
-  pp.dpage = make_fastdiv(page);
+  pp.table = a.block_table;
+  pp.table_stride = a.table_stride;
+  pp.out = a.out;
+  pp.out_dtype = a.out_dtype;
+  pp.num_pages = a.num_pages;
+  pp.page = a.page_size;
+  pp.max_pages = a.max_pages;
+  pp.HKVc = a.HKV * p.hchunks;
+  pp.dpage = make_fastdiv(a.page_size);
   pp.dHch = make_fastdiv(p.hchunks);
   pp.dHKVc = make_fastdiv(pp.HKVc);
-  pp.dHQ = make_fastdiv(HQ);
+  pp.dHQ = make_fastdiv(a.HQ);
   pp.dgroup = make_fastdiv(p.group);
   return TKV_OK;
 }
@@ -1133,60 +1135,40 @@ extern "C" int tkv_paged_workspace(int B, int HQ, int HKV, int page_size, int D,
   return packed_unsupported(nbits, D, gs);
 }
 
-extern "C" int tkv_paged_decode(const void* q, int q_dtype, const uint8_t* k_packed, const void* k_scale,
-                                const void* k_zero, const uint8_t* v_packed, const void* v_scale,
-                                const void* v_zero, const int32_t* block_table, int64_t table_stride,
-                                const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
-                                int64_t workspace_bytes, uint32_t* tickets, int B, int HQ, int HKV, int num_pages, int page_size,
-                                int max_pages, int D, int nbits, int gs, float sm_scale, void* stream) {
+extern "C" int tkv_paged_decode(const tkv_paged_decode_args* args, void* stream) {
   using namespace tkv;
-  TKV_REQUIRE(nbits == 2 || nbits == 4, TKV_ERR_INVALID, "nbits must be one of (2, 4), got %d", nbits);
+  TKV_REQUIRE(args, TKV_ERR_INVALID, "paged decode: null arguments");
+  const tkv_paged_decode_args& a = *args;
   PagedCall c;
-  const int rc = paged_fill("paged decode", c, q, q_dtype, block_table, table_stride, seq_lens, out, out_dtype,
-                            workspace, workspace_bytes, tickets, B, HQ, HKV, num_pages, page_size, max_pages, D, sm_scale);
+  const int rc = paged_fill(c, a);
   if (rc != TKV_OK) return rc;
-  TKV_REQUIRE(k_packed && k_scale && k_zero && v_packed && v_scale && v_zero, TKV_ERR_INVALID, "paged decode: null pointer");
-  TKV_REQUIRE(aligned16(k_packed) && aligned16(v_packed) && aligned16(k_scale) && aligned16(k_zero) &&
-                  aligned16(v_scale) && aligned16(v_zero), TKV_ERR_ALIGN, "paged decode: the pools must be 16-byte aligned");
   DecodeParams& p = c.pp.d;
-  p.kp = k_packed;
-  p.vp = v_packed;
-  p.ks = (const __half*)k_scale;
-  p.kz = (const __half*)k_zero;
-  p.vs = (const __half*)v_scale;
-  p.vz = (const __half*)v_zero;
-  const int page = page_size;
+  const int nbits = a.nbits, D = a.D, gs = a.gs, page = a.page_size;
+  if (nbits == 16) {
+    p.k = (const __half*)a.k;
+    p.v = (const __half*)a.v;
+    if (D == 128) return f16_run<Fp16Policy<128>>(c, (cudaStream_t)stream);
+    if (D == 64) return f16_run<Fp16Policy<64>>(c, (cudaStream_t)stream);
+    set_error("paged fp16 decode: unsupported head_dim=%d (built: 64, 128)", D);
+    return TKV_ERR_UNSUPPORTED;
+  }
+  p.kp = (const uint8_t*)a.k;
+  p.vp = (const uint8_t*)a.v;
+  p.ks = (const __half*)a.k_scale;
+  p.kz = (const __half*)a.k_zero;
+  p.vs = (const __half*)a.v_scale;
+  p.vz = (const __half*)a.v_zero;
   {
     // one tensor map over both code pools, where a K and a V run land side by side in whole swizzle
     // atoms (or the stage is laid out for it: two pieces)
-    const uint8_t *lo = k_packed < v_packed ? k_packed : v_packed, *hi = k_packed < v_packed ? v_packed : k_packed;
+    const uint8_t *lo = p.kp < p.vp ? p.kp : p.vp, *hi = p.kp < p.vp ? p.vp : p.kp;
     const uint64_t gap = (uint64_t)(hi - lo);
-    const int64_t pool = (int64_t)num_pages * HKV * page * (D * nbits / 8);
+    const int64_t pool = (int64_t)a.num_pages * a.HKV * page * (D * nbits / 8);
     p.kv_one = (page % 32 != 0 || (32 * (D * nbits / 8)) % 1024 == 0) && gap % 16 == 0 && gap < (1ull << 40) &&
                gap >= (uint64_t)pool;
-    p.k_second = p.kv_one && k_packed > v_packed;
+    p.k_second = p.kv_one && p.kp > p.vp;
   }
-  const bool few = few_units(B, c.pp.HKVc);
+  const bool few = few_units(a.B, c.pp.HKVc);
   TKV_PAGED_ALL(packed_run<P>(c, (cudaStream_t)stream))
   return packed_unsupported(nbits, D, gs);
-}
-
-extern "C" int tkv_paged_fp16_decode(const void* q, int q_dtype, const void* k, const void* v,
-                                     const int32_t* block_table, int64_t table_stride,
-                                     const int32_t* seq_lens, void* out, int out_dtype, void* workspace,
-                                     int64_t workspace_bytes, uint32_t* tickets, int B, int HQ, int HKV, int num_pages, int page_size,
-                                     int max_pages, int D, float sm_scale, void* stream) {
-  using namespace tkv;
-  PagedCall c;
-  const int rc = paged_fill("paged fp16 decode", c, q, q_dtype, block_table, table_stride, seq_lens, out, out_dtype,
-                            workspace, workspace_bytes, tickets, B, HQ, HKV, num_pages, page_size, max_pages, D, sm_scale);
-  if (rc != TKV_OK) return rc;
-  TKV_REQUIRE(k && v, TKV_ERR_INVALID, "paged fp16 decode: null pointer");
-  TKV_REQUIRE(aligned16(k) && aligned16(v), TKV_ERR_ALIGN, "paged fp16 decode: the pools must be 16-byte aligned");
-  c.pp.d.k = (const __half*)k;
-  c.pp.d.v = (const __half*)v;
-  if (D == 128) return f16_run<Fp16Policy<128>>(c, (cudaStream_t)stream);
-  if (D == 64) return f16_run<Fp16Policy<64>>(c, (cudaStream_t)stream);
-  set_error("paged fp16 decode: unsupported head_dim=%d (built: 64, 128)", D);
-  return TKV_ERR_UNSUPPORTED;
 }

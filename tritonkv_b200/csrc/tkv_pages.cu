@@ -296,22 +296,22 @@ __global__ void __launch_bounds__(256) compact_apply_kernel(const CompactArgs a,
 }
 
 // ------------------------------------------------------------------ host side
-static int check_pools(const char* who, void* const* pools, const int64_t* page_bytes, int n) {
-  TKV_REQUIRE(n >= 0 && (n == 0 || (pools && page_bytes)), TKV_ERR_INVALID, "%s: bad list of %d pools", who, n);
+static int check_pools(const char* who, const tkv_page_pool* pools, int n) {
+  TKV_REQUIRE(n >= 0 && (n == 0 || pools), TKV_ERR_INVALID, "%s: bad list of %d pools", who, n);
   for (int i = 0; i < n; ++i)
-    TKV_REQUIRE(pools[i] && page_bytes[i] > 0 && page_bytes[i] < (1LL << 40), TKV_ERR_INVALID, "%s: bad pool tensor %d",
-                who, i);
+    TKV_REQUIRE(pools[i].base && pools[i].page_bytes > 0 && pools[i].page_bytes < (1LL << 40), TKV_ERR_INVALID,
+                "%s: bad pool tensor %d", who, i);
   return TKV_OK;
 }
 
 // Tensors [i0, i0 + kMaxPoolTensors) of the list.
-static PoolTensors some_pools(void* const* pools, const int64_t* page_bytes, int n, int i0) {
+static PoolTensors some_pools(const tkv_page_pool* pools, int n, int i0) {
   PoolTensors t{};
   t.n = n - i0 < kMaxPoolTensors ? n - i0 : kMaxPoolTensors;
   t.wide = 1;
   for (int i = 0; i < t.n; ++i) {
-    t.base[i] = static_cast<uint8_t*>(pools[i0 + i]);
-    t.page_bytes[i] = page_bytes[i0 + i];
+    t.base[i] = static_cast<uint8_t*>(pools[i0 + i].base);
+    t.page_bytes[i] = pools[i0 + i].page_bytes;
     t.first[i] = t.slices;
     t.slices += (int)((t.page_bytes[i] + kSlice - 1) / kSlice);
     if ((reinterpret_cast<uintptr_t>(t.base[i]) | (uintptr_t)t.page_bytes[i]) & 15) t.wide = 0;
@@ -333,51 +333,49 @@ extern "C" int tkv_pages_workspace(int B, int num_pages, int64_t* words) {
   return TKV_OK;
 }
 
-extern "C" int tkv_pages_fork(const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
-                              int B_old, const int32_t* parents, const int32_t* reserve, int reserve0, int B,
-                              int max_pages, int num_pages, int page_size, int32_t* new_table,
-                              int32_t* new_lens, int32_t* missing, int32_t* workspace, void* const* pools,
-                              const int64_t* page_bytes, int n_pools, void* stream) {
+extern "C" int tkv_pages_fork(const tkv_pages_fork_args* args, const tkv_page_pool* pools, int n_pools, void* stream) {
   using namespace tkv;
-  TKV_REQUIRE(B >= 0 && B_old >= 0 && max_pages >= 0 && num_pages > 0 && page_size > 0, TKV_ERR_INVALID,
-              "fork: bad sizes B=%d B_old=%d max_pages=%d num_pages=%d page_size=%d", B, B_old, max_pages,
-              num_pages, page_size);
-  TKV_REQUIRE((int64_t)max_pages * page_size < (1LL << 30) && (int64_t)B * max_pages < (1LL << 30), TKV_ERR_INVALID,
-              "fork: a table of %d x %d pages of %d tokens is too large", B, max_pages, page_size);
-  TKV_REQUIRE(missing && workspace, TKV_ERR_INVALID, "fork: null pointer");
-  TKV_REQUIRE(B == 0 || (parents && new_lens), TKV_ERR_INVALID, "fork: null pointer");
-  TKV_REQUIRE(B == 0 || max_pages == 0 || new_table, TKV_ERR_INVALID, "fork: null pointer");
-  TKV_REQUIRE(B_old == 0 || ((block_table || max_pages == 0) && seq_lens), TKV_ERR_INVALID, "fork: null pointer");
-  const int rc = check_pools("fork", pools, page_bytes, n_pools);
+  TKV_REQUIRE(args, TKV_ERR_INVALID, "fork: null arguments");
+  const tkv_pages_fork_args& in = *args;
+  TKV_REQUIRE(in.B >= 0 && in.B_old >= 0 && in.max_pages >= 0 && in.num_pages > 0 && in.page_size > 0, TKV_ERR_INVALID,
+              "fork: bad sizes B=%d B_old=%d max_pages=%d num_pages=%d page_size=%d", in.B, in.B_old, in.max_pages,
+              in.num_pages, in.page_size);
+  TKV_REQUIRE((int64_t)in.max_pages * in.page_size < (1LL << 30) && (int64_t)in.B * in.max_pages < (1LL << 30),
+              TKV_ERR_INVALID, "fork: a table of %d x %d pages of %d tokens is too large", in.B, in.max_pages, in.page_size);
+  TKV_REQUIRE(in.missing && in.workspace, TKV_ERR_INVALID, "fork: null pointer");
+  TKV_REQUIRE(in.B == 0 || (in.parents && in.new_lens), TKV_ERR_INVALID, "fork: null pointer");
+  TKV_REQUIRE(in.B == 0 || in.max_pages == 0 || in.new_table, TKV_ERR_INVALID, "fork: null pointer");
+  TKV_REQUIRE(in.B_old == 0 || ((in.block_table || in.max_pages == 0) && in.seq_lens), TKV_ERR_INVALID, "fork: null pointer");
+  const int rc = check_pools("fork", pools, n_pools);
   if (rc != TKV_OK) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  const int words = (num_pages + 31) / 32;
+  const int B = in.B, words = (in.num_pages + 31) / 32;
   ForkArgs a{};
-  a.table = block_table;
-  a.lens = seq_lens;
-  a.parents = parents;
-  a.reserve = reserve;
-  a.new_table = new_table;
-  a.new_lens = new_lens;
-  a.missing = missing;
-  a.ticket = (uint32_t*)workspace;  // [ticket, listed, -, -][bitmap][fresh][src][start]
-  a.listed = workspace + 1;
-  a.used = (uint32_t*)workspace + 4;
-  a.fresh = workspace + 4 + words;
-  a.src = a.fresh + num_pages;
+  a.table = in.block_table;
+  a.lens = in.seq_lens;
+  a.parents = in.parents;
+  a.reserve = in.reserve;
+  a.new_table = in.new_table;
+  a.new_lens = in.new_lens;
+  a.missing = in.missing;
+  a.ticket = (uint32_t*)in.workspace;  // [ticket, listed, -, -][bitmap][fresh][src][start]
+  a.listed = in.workspace + 1;
+  a.used = (uint32_t*)in.workspace + 4;
+  a.fresh = in.workspace + 4 + words;
+  a.src = a.fresh + in.num_pages;
   a.start = a.src + B;
-  a.table_stride = table_stride;
-  a.reserve0 = reserve0;
-  a.B_old = B_old;
+  a.table_stride = in.table_stride;
+  a.reserve0 = in.reserve0;
+  a.B_old = in.B_old;
   a.B = B;
-  a.num_pages = num_pages;
-  a.page = page_size;
-  a.W = max_pages;
+  a.num_pages = in.num_pages;
+  a.page = in.page_size;
+  a.W = in.max_pages;
   fork_plan_kernel<<<plan_grid(B), kPlanThreads, 0, s>>>(a);
   TKV_CUDA(cudaGetLastError());
   if (B == 0) return TKV_OK;
   for (int i0 = 0; i0 == 0 || i0 < n_pools; i0 += kMaxPoolTensors) {
-    const PoolTensors t = some_pools(pools, page_bytes, n_pools, i0);
+    const PoolTensors t = some_pools(pools, n_pools, i0);
     // CTAs of a row: about four waves in all where every row copies
     int parts = (148 * 32 + B - 1) / B;
     parts = parts < 1 ? 1 : parts > t.slices ? (t.slices > 0 ? t.slices : 1) : parts;
@@ -386,39 +384,40 @@ extern "C" int tkv_pages_fork(const int32_t* block_table, int64_t table_stride, 
   return TKV_OK;
 }
 
-extern "C" int tkv_pages_compact(const int32_t* block_table, int64_t table_stride, int B, int max_pages,
-                                 int num_pages, int32_t* new_table, int32_t* live, int32_t* workspace,
-                                 void* const* pools, const int64_t* page_bytes, int n_pools, void* stream) {
+extern "C" int tkv_pages_compact(const tkv_pages_compact_args* args, const tkv_page_pool* pools, int n_pools,
+                                 void* stream) {
   using namespace tkv;
-  TKV_REQUIRE(B >= 0 && max_pages >= 0 && num_pages > 0, TKV_ERR_INVALID,
-              "compact: bad sizes B=%d max_pages=%d num_pages=%d", B, max_pages, num_pages);
-  TKV_REQUIRE((int64_t)B * max_pages < (1LL << 30), TKV_ERR_INVALID, "compact: a table of %d x %d entries is too large",
-              B, max_pages);
-  TKV_REQUIRE(live && workspace, TKV_ERR_INVALID, "compact: null pointer");
-  TKV_REQUIRE(B == 0 || max_pages == 0 || (block_table && new_table), TKV_ERR_INVALID, "compact: null pointer");
-  const int rc = check_pools("compact", pools, page_bytes, n_pools);
+  TKV_REQUIRE(args, TKV_ERR_INVALID, "compact: null arguments");
+  const tkv_pages_compact_args& in = *args;
+  TKV_REQUIRE(in.B >= 0 && in.max_pages >= 0 && in.num_pages > 0, TKV_ERR_INVALID,
+              "compact: bad sizes B=%d max_pages=%d num_pages=%d", in.B, in.max_pages, in.num_pages);
+  TKV_REQUIRE((int64_t)in.B * in.max_pages < (1LL << 30), TKV_ERR_INVALID,
+              "compact: a table of %d x %d entries is too large", in.B, in.max_pages);
+  TKV_REQUIRE(in.live && in.workspace, TKV_ERR_INVALID, "compact: null pointer");
+  TKV_REQUIRE(in.B == 0 || in.max_pages == 0 || (in.block_table && in.new_table), TKV_ERR_INVALID, "compact: null pointer");
+  const int rc = check_pools("compact", pools, n_pools);
   if (rc != TKV_OK) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  const int words = (num_pages + 31) / 32;
+  const int words = (in.num_pages + 31) / 32;
   CompactArgs a{};
-  a.table = block_table;
-  a.new_table = new_table;
-  a.live = live;
-  a.ticket = (uint32_t*)workspace;  // [ticket, moves, -, -][bitmap][before][src][dst][to]
-  a.n_moves = workspace + 1;
-  a.used = (uint32_t*)workspace + 4;
-  a.before = workspace + 4 + words;
+  a.table = in.block_table;
+  a.new_table = in.new_table;
+  a.live = in.live;
+  a.ticket = (uint32_t*)in.workspace;  // [ticket, moves, -, -][bitmap][before][src][dst][to]
+  a.n_moves = in.workspace + 1;
+  a.used = (uint32_t*)in.workspace + 4;
+  a.before = in.workspace + 4 + words;
   a.src = a.before + words;
-  a.dst = a.src + num_pages;
-  a.to = a.dst + num_pages;
-  a.table_stride = table_stride;
-  a.B = B;
-  a.W = max_pages;
-  a.num_pages = num_pages;
-  compact_plan_kernel<<<plan_grid(B), kPlanThreads, 0, s>>>(a);
+  a.dst = a.src + in.num_pages;
+  a.to = a.dst + in.num_pages;
+  a.table_stride = in.table_stride;
+  a.B = in.B;
+  a.W = in.max_pages;
+  a.num_pages = in.num_pages;
+  compact_plan_kernel<<<plan_grid(in.B), kPlanThreads, 0, s>>>(a);
   TKV_CUDA(cudaGetLastError());
   for (int i0 = 0; i0 == 0 || i0 < n_pools; i0 += kMaxPoolTensors) {
-    const PoolTensors t = some_pools(pools, page_bytes, n_pools, i0);
+    const PoolTensors t = some_pools(pools, n_pools, i0);
     TKV_CUDA(launch_pdl(compact_apply_kernel, dim3(148 * 8), dim3(256), 0, s, a, t, i0 == 0 ? 1 : 0));
   }
   return TKV_OK;

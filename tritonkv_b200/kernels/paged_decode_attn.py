@@ -7,8 +7,6 @@ caches are one contiguous tensor per batch.
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from .. import _cabi
@@ -19,11 +17,11 @@ from ._launch import q_for_kernel
 __all__ = ["paged_decode_attention", "paged_fp16_decode_attention"]
 
 
-_OUT = {torch.float32, torch.float16, torch.bfloat16}
+_CODE = {torch.float16: _cabi.DTYPE_F16, torch.bfloat16: _cabi.DTYPE_BF16, torch.float32: _cabi.DTYPE_F32}
+_PACK = _cabi.PAGED_DECODE_ARGS.pack
 
 
-def _check(q, k, v, block_table, seq_lens, out):
-    """Checked arguments shared by the two forms: (k tensors, v tensors, q, seq_lens, out, sizes)."""
+def _attend(q, k, v, nbits, group_size, block_table, seq_lens, sm_scale, out, workspace):
     kt, vt = pool_tensors(k, "k"), pool_tensors(v, "v")
     shape = kt[0].shape
     if len(kt) != len(vt) or vt[0].shape != shape:
@@ -32,20 +30,36 @@ def _check(q, k, v, block_table, seq_lens, out):
         raise ValueError(f"q must be (B, HQ, head_dim), got {tuple(q.shape)}")
     B, HQ, D = q.shape
     NP, HKV, page, row = shape
-    if D != (k.head_dim if len(kt) == 3 else row):
+    if D != (row if nbits == 16 else k.head_dim):
         raise ValueError(f"q {tuple(q.shape)} is incompatible with pools of {tuple(shape)}")
     if HKV == 0 or HQ == 0 or HQ % HKV != 0:
         raise ValueError(f"HQ={HQ} must be a multiple of HKV={HKV}")
-    dev = q.device
-    if kt[0].device != dev or vt[0].device != dev:
-        raise ValueError(f"the pools are on {kt[0].device} and {vt[0].device}, q on {dev}")
-    W, stride = check_table(block_table, B, dev)
-    seq_lens = check_lens(seq_lens, B, dev, "seq_lens")
+    where = q.get_device()
+    if kt[0].get_device() != where or vt[0].get_device() != where:
+        raise ValueError(f"the pools are on {kt[0].device} and {vt[0].device}, q on {q.device}")
+    W, stride = check_table(block_table, B, where)
+    seq_lens = check_lens(seq_lens, B, where, "seq_lens")
     if out is None:
-        out = torch.empty((B, HQ, D), device=dev, dtype=torch.float32)
-    elif out.shape != q.shape or out.dtype not in _OUT or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous float32, float16 or bfloat16 tensor of shape {(B, HQ, D)} on {dev}")
-    return kt, vt, q_for_kernel(q), seq_lens, out, (B, HQ, HKV, NP, page, W, D), stride
+        out = torch.empty((B, HQ, D), device=q.device, dtype=torch.float32)
+    elif out.shape != q.shape or out.dtype not in _CODE or out.get_device() != where or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous float32, float16 or bfloat16 tensor of shape {(B, HQ, D)} on {q.device}")
+    _cabi.require_cuda(q, "q")
+    lib = _cabi.load()
+    if B == 0:
+        return out
+    q = q_for_kernel(q)
+    if nbits == 16:
+        k, v, ks, kz, vs, vz = kt[0].data_ptr(), vt[0].data_ptr(), 0, 0, 0, 0
+    else:
+        k, ks, kz = [t.data_ptr() for t in kt]
+        v, vs, vz = [t.data_ptr() for t in vt]
+    with _cabi.on_device(q.device):
+        ws = _cabi.paged_workspace(workspace, (B, HQ, HKV, page, D, nbits, group_size, where), q.device)
+        _cabi.check(lib.tkv_paged_decode(
+            _PACK(q.data_ptr(), k, ks, kz, v, vs, vz, block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ws[1],
+                  ws[3], stride, ws[2], _CODE[q.dtype], _CODE[out.dtype], B, HQ, HKV, NP, page, W, D, nbits, group_size,
+                  D ** -0.5 if sm_scale is None else sm_scale), _cabi.stream_ptr(q.device)))
+    return out
 
 
 def paged_decode_attention(
@@ -73,20 +87,7 @@ def paged_decode_attention(
         raise TypeError("paged_decode_attention reads packed pools (QuantizedTensor); see paged_fp16_decode_attention")
     if kq.nbits != vq.nbits or kq.group_size != vq.group_size:
         raise ValueError("K and V must use the same nbits/group_size")
-    kt, vt, q, seq_lens, out, (B, HQ, HKV, NP, page, W, D), stride = _check(q, kq, vq, block_table, seq_lens, out)
-    _cabi.require_cuda(q, "q")
-    lib = _cabi.load()
-    if B == 0:
-        return out
-    dev = q.device
-    with _cabi.on_device(dev):
-        ws = _cabi.paged_workspace(_workspace, B, HQ, HKV, page, D, kq.nbits, kq.group_size, dev)
-        _cabi.check(lib.tkv_paged_decode(
-            q.data_ptr(), _cabi.dtype_code(q), kt[0].data_ptr(), kt[1].data_ptr(), kt[2].data_ptr(), vt[0].data_ptr(),
-            vt[1].data_ptr(), vt[2].data_ptr(), block_table.data_ptr(), stride, seq_lens.data_ptr(), out.data_ptr(),
-            _cabi.dtype_code(out), ws[0].data_ptr(), ws[1], ws[2], B, HQ, HKV, NP, page, W, D, kq.nbits, kq.group_size,
-            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _cabi.stream_ptr(dev)))
-    return out
+    return _attend(q, kq, vq, kq.nbits, kq.group_size, block_table, seq_lens, sm_scale, out, _workspace)
 
 
 def paged_fp16_decode_attention(
@@ -103,16 +104,4 @@ def paged_fp16_decode_attention(
     ``(num_pages, HKV, page_size, D)``; everything else as in :func:`paged_decode_attention`."""
     if not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor):
         raise TypeError("paged_fp16_decode_attention reads float16 pools; see paged_decode_attention")
-    kt, vt, q, seq_lens, out, (B, HQ, HKV, NP, page, W, D), stride = _check(q, k, v, block_table, seq_lens, out)
-    _cabi.require_cuda(q, "q")
-    lib = _cabi.load()
-    if B == 0:
-        return out
-    dev = q.device
-    with _cabi.on_device(dev):
-        ws = _cabi.paged_workspace(_workspace, B, HQ, HKV, page, D, 16, 0, dev)
-        _cabi.check(lib.tkv_paged_fp16_decode(
-            q.data_ptr(), _cabi.dtype_code(q), kt[0].data_ptr(), vt[0].data_ptr(), block_table.data_ptr(), stride,
-            seq_lens.data_ptr(), out.data_ptr(), _cabi.dtype_code(out), ws[0].data_ptr(), ws[1], ws[2], B, HQ, HKV, NP, page, W, D,
-            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _cabi.stream_ptr(dev)))
-    return out
+    return _attend(q, k, v, 16, 0, block_table, seq_lens, sm_scale, out, _workspace)

@@ -61,11 +61,15 @@ def pool_tensors(pool, what: str) -> tuple[torch.Tensor, ...]:
     raise ValueError(f"{what} must be contiguous: a pool is used in place")
 
 
-def check_table(block_table: torch.Tensor, B: int | None, device) -> tuple[int, int]:
-    """(entries per row, row stride) of an int32 table (B, max_pages) whose rows are contiguous."""
+def _on(where: int) -> str:
+    return f"cuda:{where}" if where >= 0 else "the pools' device"
+
+
+def check_table(block_table: torch.Tensor, B: int | None, where: int) -> tuple[int, int]:
+    """(entries per row, row stride) of an int32 table (B, max_pages) on device ``where`` whose rows are contiguous."""
     shape = block_table.shape
-    if len(shape) != 2 or block_table.dtype is not _I32 or block_table.device != device:
-        raise ValueError(f"block_table must be an int32 tensor (B, max_pages) on {device}")
+    if len(shape) != 2 or block_table.dtype is not _I32 or block_table.get_device() != where:
+        raise ValueError(f"block_table must be an int32 tensor (B, max_pages) on {_on(where)}")
     if B is not None and shape[0] != B:
         raise ValueError(f"block_table has {shape[0]} rows for {B} sequences")
     stride = block_table.stride()
@@ -74,10 +78,10 @@ def check_table(block_table: torch.Tensor, B: int | None, device) -> tuple[int, 
     return shape[1], stride[0]
 
 
-def check_lens(lens: torch.Tensor, B: int, device, what: str) -> torch.Tensor:
+def check_lens(lens: torch.Tensor, B: int, where: int, what: str) -> torch.Tensor:
     shape = lens.shape
-    if len(shape) != 1 or shape[0] != B or lens.dtype is not _I32 or lens.device != device:
-        raise ValueError(f"{what} must be an int32 tensor of shape ({B},) on {device}")
+    if len(shape) != 1 or shape[0] != B or lens.dtype is not _I32 or lens.get_device() != where:
+        raise ValueError(f"{what} must be an int32 tensor of shape ({B},) on {_on(where)}")
     return lens if lens.is_contiguous() else lens.contiguous()
 
 
@@ -93,7 +97,18 @@ def _row_strides(x: torch.Tensor) -> tuple | None:
     return None if (kept[0] | kept[1] | kept[2]) & al else kept
 
 
-_PACK6 = struct.Struct("6q").pack
+_NO_STRIDES = (0, 0, 0)
+_APPEND = _cabi.PAGED_APPEND_ARGS.pack
+
+
+def _place(values: torch.Tensor, new: torch.Tensor, what: str) -> tuple[int, tuple]:
+    """Address and strides of the tensor that the values of ``new`` go to."""
+    if values.shape != new.shape or values.dtype != new.dtype or values.get_device() != new.get_device():
+        raise ValueError(f"{what} must be a {new.dtype} tensor of shape {tuple(new.shape)} on {new.device}")
+    strides = _row_strides(values)
+    if strides is None:
+        raise ValueError(f"{what} must have contiguous rows that start on 16-byte boundaries: it is written in place")
+    return values.data_ptr(), strides
 
 
 def append_kv_paged(kq, vq, k_new: torch.Tensor, v_new: torch.Tensor, block_table: torch.Tensor, positions,
@@ -124,7 +139,7 @@ def append_kv_paged(kq, vq, k_new: torch.Tensor, v_new: torch.Tensor, block_tabl
     NP, HKV, page, D = kt[0].shape
     if packed:
         D = kq.head_dim
-    dev = kt[0].device
+    where = kt[0].get_device()
     shape, dtype = k_new.shape, k_new.dtype
     if len(shape) != 4 or shape != v_new.shape:
         raise ValueError(f"k_new and v_new must both be (B, HKV, T, head_dim), got {tuple(shape)} and {tuple(v_new.shape)}")
@@ -133,30 +148,23 @@ def append_kv_paged(kq, vq, k_new: torch.Tensor, v_new: torch.Tensor, block_tabl
         raise ValueError(f"k_new {tuple(shape)} does not match pools of {HKV} heads of {D}")
     if dtype != v_new.dtype:
         raise ValueError(f"k_new and v_new must have the same dtype, got {dtype} and {v_new.dtype}")
-    if k_new.device != dev or v_new.device != dev or vt[0].device != dev:
-        raise ValueError(f"the pools and the new tokens must be on one device, got {dev}, {vt[0].device}, {k_new.device}")
-    W, stride = check_table(block_table, B, dev)
-    pos_ptr, pos0, len_ptr = None, 0, None
+    if k_new.get_device() != where or v_new.get_device() != where or vt[0].get_device() != where:
+        raise ValueError(f"the pools and the new tokens must be on one device, got {kt[0].device}, {vt[0].device}, "
+                         f"{k_new.device}, {v_new.device}")
+    W, stride = check_table(block_table, B, where)
+    pos_ptr = pos0 = len_ptr = 0
     if isinstance(positions, torch.Tensor):
-        positions = check_lens(positions, B, dev, "positions")
+        positions = check_lens(positions, B, where, "positions")
         pos_ptr = positions.data_ptr()
     else:
         pos0 = int(positions)
-        if pos0 < 0 or pos0 + T > W * page:
+        if pos0 < 0 or pos0 + T > min(W * page, 2 ** 30):  # the longest row of tokens a table may name
             raise ValueError(f"tokens [{pos0}, {pos0 + T}) do not fit a table of {W} pages of {page}")
     if lengths is not None:
-        lengths = check_lens(lengths, B, dev, "lengths")
+        lengths = check_lens(lengths, B, where, "lengths")
         len_ptr = lengths.data_ptr()
-    places, vstrides = [None, None], [(0, 0, 0), (0, 0, 0)]
-    for i, (val, what) in enumerate(((k_values, "k_values"), (v_values, "v_values"))):
-        if val is None:
-            continue
-        if val.shape != shape or val.dtype != dtype or val.device != dev:
-            raise ValueError(f"{what} must be a {dtype} tensor of shape {tuple(shape)} on {dev}")
-        vstrides[i] = _row_strides(val)
-        if vstrides[i] is None:
-            raise ValueError(f"{what} must have contiguous rows that start on 16-byte boundaries: it is written in place")
-        places[i] = val.data_ptr()
+    k_place, k_vs = (0, _NO_STRIDES) if k_values is None else _place(k_values, k_new, "k_values")
+    v_place, v_vs = (0, _NO_STRIDES) if v_values is None else _place(v_values, v_new, "v_values")
     code = _cabi.dtype_code(k_new)
     _cabi.require_cuda(kt[0], "kq")
     lib = _cabi.load()
@@ -169,18 +177,19 @@ def append_kv_paged(kq, vq, k_new: torch.Tensor, v_new: torch.Tensor, block_tabl
     if v_strides is None:
         v_new = v_new.clone(memory_format=torch.contiguous_format)
         v_strides = _row_strides(v_new)
-    meta = [t.data_ptr() for t in (*kt[1:], *vt[1:])] if packed else (None,) * 4
+    kp, ks, kz = (t.data_ptr() for t in kt) if packed else (kt[0].data_ptr(), 0, 0)
+    vp, vs, vz = (t.data_ptr() for t in vt) if packed else (vt[0].data_ptr(), 0, 0)
+    dev = k_new.device
     with _cabi.on_device(dev):
         _cabi.check(lib.tkv_paged_append(
-            k_new.data_ptr(), v_new.data_ptr(), code, _PACK6(*k_strides, *v_strides), kt[0].data_ptr(), meta[0], meta[1],
-            vt[0].data_ptr(), meta[2], meta[3], places[0], places[1], _PACK6(*vstrides[0], *vstrides[1]),
-            block_table.data_ptr(), stride, pos_ptr, pos0, len_ptr, B, HKV, T, NP, page, W, D,
-            kq.nbits if packed else 16, kq.group_size if packed else 0, _cabi.stream_ptr(dev)))
+            _APPEND(k_new.data_ptr(), v_new.data_ptr(), kp, ks, kz, vp, vs, vz, k_place, v_place, block_table.data_ptr(),
+                    pos_ptr, len_ptr, *k_strides, *v_strides, *k_vs, *v_vs, stride, code, pos0, B, HKV, T, NP, page, W, D,
+                    kq.nbits if packed else 16, kq.group_size if packed else 0), _cabi.stream_ptr(dev)))
     return kq, vq
 
 
-def _pool_list(pools) -> tuple[list[torch.Tensor], int, int, torch.device]:
-    """(tensors, num_pages, page_size, device) of pools that share one block table."""
+def _pool_list(pools) -> tuple[list[torch.Tensor], int, int, int]:
+    """(tensors, num_pages, page_size, device index) of pools that share one block table."""
     if isinstance(pools, (QuantizedTensor, torch.Tensor)):
         pools = [pools]
     ts, shape, where = [], None, -1
@@ -198,9 +207,11 @@ def _pool_list(pools) -> tuple[list[torch.Tensor], int, int, torch.device]:
         raise ValueError("pools must name at least one pool")
     if ts[0].numel() == 0:
         raise ValueError("pools must have at least one page of at least one token")
-    return ts, shape[0], shape[2], ts[0].device
+    return ts, shape[0], shape[2], where
 
 
+_FORK = _cabi.PAGES_FORK_ARGS.pack
+_COMPACT = _cabi.PAGES_COMPACT_ARGS.pack
 _pages_words: dict = {}
 
 
@@ -224,10 +235,11 @@ def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
 
 
 def _pool_args(ts):
-    """Addresses and bytes per page (of contiguous tensors: stride 0) as the C arrays of 64-bit words."""
-    form = f"{len(ts)}q"
-    return (struct.pack(form, *[t.data_ptr() for t in ts]),
-            struct.pack(form, *[t.stride(0) * (1 if t.dtype is _U8 else 2) for t in ts]), len(ts))
+    """(address, bytes per page) of every tensor as the C array, and how many."""
+    words = []
+    for t in ts:
+        words += (t.data_ptr(), t.stride(0) * (1 if t.dtype is _U8 else 2))
+    return struct.pack(f"{len(words)}q", *words), len(ts)
 
 
 def _new_like(x, shape, like, what):
@@ -277,17 +289,17 @@ def fork_pages(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, parents
     tensors, supplied by the caller; they must not share memory with the inputs.  The old
     table is not changed.  A partly filled page that two different rows name (which this
     function never makes) stays shared."""
-    ts, NP, page, dev = _pool_list(pools)
-    W, stride = check_table(block_table, None, dev)
+    ts, NP, page, where = _pool_list(pools)
+    W, stride = check_table(block_table, None, where)
     B_old = block_table.shape[0]
-    seq_lens = check_lens(seq_lens, B_old, dev, "seq_lens")
+    seq_lens = check_lens(seq_lens, B_old, where, "seq_lens")
     if parents.dim() != 1:
-        raise ValueError(f"parents must be an int32 tensor (B_new,) on {dev}")
+        raise ValueError(f"parents must be an int32 tensor (B_new,) on {_on(where)}")
     B = parents.shape[0]
-    parents = check_lens(parents, B, dev, "parents")
-    r_ptr, r0 = None, 0
+    parents = check_lens(parents, B, where, "parents")
+    r_ptr = r0 = 0
     if isinstance(reserve, torch.Tensor):
-        reserve = check_lens(reserve, B, dev, "reserve")
+        reserve = check_lens(reserve, B, where, "reserve")
         r_ptr = reserve.data_ptr()
     else:
         r0 = int(reserve)
@@ -298,14 +310,15 @@ def fork_pages(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, parents
     lens = _new_like(lens, (B,), block_table, "out[1]")
     missing = _new_like(missing, (1,), block_table, "out[2]")
     if out is not None:
-        _no_overlap((table, lens, missing), (block_table, seq_lens, parents) + (() if r_ptr is None else (reserve,)))
+        _no_overlap((table, lens, missing), (block_table, seq_lens, parents) + ((reserve,) if r_ptr else ()))
     _cabi.require_cuda(ts[0], "pools")
-    lib = _cabi.load()
+    lib, dev = _cabi.load(), block_table.device
     with _cabi.on_device(dev):
         ws = _pages_workspace(_workspace, B, NP, dev)
         _cabi.check(lib.tkv_pages_fork(
-            block_table.data_ptr(), stride, seq_lens.data_ptr(), B_old, parents.data_ptr(), r_ptr, r0, B, W, NP, page,
-            table.data_ptr(), lens.data_ptr(), missing.data_ptr(), ws.data_ptr(), *_pool_args(ts), _cabi.stream_ptr(dev)))
+            _FORK(block_table.data_ptr(), seq_lens.data_ptr(), parents.data_ptr(), r_ptr, table.data_ptr(), lens.data_ptr(),
+                  missing.data_ptr(), ws.data_ptr(), stride, B_old, r0, B, W, NP, page),
+            *_pool_args(ts), _cabi.stream_ptr(dev)))
     return table, lens, missing
 
 
@@ -318,8 +331,8 @@ def compact_pages(pools, block_table: torch.Tensor, out: tuple | None = None, _w
     on are then unused.  The old table stays valid as long as the freed places are not written:
     pages are copied, and only into places that it did not name.  ``out``: these two tensors,
     supplied by the caller."""
-    ts, NP, page, dev = _pool_list(pools)
-    W, stride = check_table(block_table, None, dev)
+    ts, NP, page, where = _pool_list(pools)
+    W, stride = check_table(block_table, None, where)
     B = block_table.shape[0]
     table, live = (None, None) if out is None else out
     table = _new_like(table, (B, W), block_table, "out[0]")
@@ -327,10 +340,10 @@ def compact_pages(pools, block_table: torch.Tensor, out: tuple | None = None, _w
     if out is not None:
         _no_overlap((table, live), (block_table,))
     _cabi.require_cuda(ts[0], "pools")
-    lib = _cabi.load()
+    lib, dev = _cabi.load(), block_table.device
     with _cabi.on_device(dev):
         ws = _pages_workspace(_workspace, B, NP, dev)
         _cabi.check(lib.tkv_pages_compact(
-            block_table.data_ptr(), stride, B, W, NP, table.data_ptr(), live.data_ptr(), ws.data_ptr(), *_pool_args(ts),
-            _cabi.stream_ptr(dev)))
+            _COMPACT(block_table.data_ptr(), table.data_ptr(), live.data_ptr(), ws.data_ptr(), stride, B, W, NP),
+            *_pool_args(ts), _cabi.stream_ptr(dev)))
     return table, live
