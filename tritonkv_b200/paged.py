@@ -234,17 +234,17 @@ def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
     return kept[1]
 
 
-def _pool_args(ts):
+def _pool_args(ts, NP: int):
     """(address, bytes per page) of every tensor as the C array, and how many."""
     words = []
     for t in ts:
-        words += (t.data_ptr(), t.stride(0) * (1 if t.dtype is _U8 else 2))
+        words += (t.data_ptr(), t.nbytes // NP)
     return struct.pack(f"{len(words)}q", *words), len(ts)
 
 
 def _new_like(x, shape, like, what):
-    if x is None:
-        return like.new_empty(shape)
+    if x is None:  # (empty_like is the cheaper call)
+        return torch.empty_like(like) if like.shape == shape and like.is_contiguous() else like.new_empty(shape)
     if x.shape != shape or x.dtype is not _I32 or x.device != like.device or not x.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)} on {like.device}")
     return x
@@ -307,7 +307,7 @@ def fork_pages(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, parents
             raise ValueError(f"reserve must be a number of tokens, got {r0}")
     table, lens, missing = (None, None, None) if out is None else out
     table = _new_like(table, (B, W), block_table, "out[0]")
-    lens = _new_like(lens, (B,), block_table, "out[1]")
+    lens = _new_like(lens, (B,), parents, "out[1]")
     missing = _new_like(missing, (1,), block_table, "out[2]")
     if out is not None:
         _no_overlap((table, lens, missing), (block_table, seq_lens, parents) + ((reserve,) if r_ptr else ()))
@@ -318,7 +318,7 @@ def fork_pages(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, parents
         _cabi.check(lib.tkv_pages_fork(
             _FORK(block_table.data_ptr(), seq_lens.data_ptr(), parents.data_ptr(), r_ptr, table.data_ptr(), lens.data_ptr(),
                   missing.data_ptr(), ws.data_ptr(), stride, B_old, r0, B, W, NP, page),
-            *_pool_args(ts), _cabi.stream_ptr(dev)))
+            *_pool_args(ts, NP), _cabi.stream_ptr(dev)))
     return table, lens, missing
 
 
@@ -345,5 +345,5 @@ def compact_pages(pools, block_table: torch.Tensor, out: tuple | None = None, _w
         ws = _pages_workspace(_workspace, B, NP, dev)
         _cabi.check(lib.tkv_pages_compact(
             _COMPACT(block_table.data_ptr(), table.data_ptr(), live.data_ptr(), ws.data_ptr(), stride, B, W, NP),
-            *_pool_args(ts), _cabi.stream_ptr(dev)))
+            *_pool_args(ts, NP), _cabi.stream_ptr(dev)))
     return table, live
