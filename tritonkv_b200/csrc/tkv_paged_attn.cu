@@ -26,11 +26,15 @@
 // whatever the lengths, and no slot has to be marked empty.  They are merged by the CTA that draws the unit's last
 // ticket, or by a kernel of their own: see PagedLaunch::run.
 //
-// What is rounded: q to f16; the probabilities, formed and summed in f32 against a running maximum, to
-// f16 for the second product (on packed pages once more when the values' scale is multiplied in, since
-// the codes are exact in f16 and the scales differ by token); the output once.  All sums are f32.  Against float64 the output
-// is 3.4e-4 to 4.5e-4 off on packed pages and 2.5e-4 on float16 ones (2-norm), where rounding it to f16 alone is 2.0e-4.  Carrying
-// the second rounding's error through a second product took 8-10 % (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.
+// What is rounded: q to f16; the probabilities, formed in f32 against a running maximum, to f16 for
+// the second product (on packed pages their sum counts the rounded ones, and they are rounded once
+// more when the values' scale is multiplied in, since the codes are exact in f16 and the scales differ
+// by token); the output once.  All sums are f32.  Against float64 the output is 3.3e-4 to 5.0e-4 off
+// on packed pages and 2.5e-4 on float16 ones (2-norm), where rounding it to f16 alone is 2.0e-4.  The
+// larger figure is that of one sequence of 65536: codes run from 0, so the mean of many tokens is a
+// difference of two larger sums, of scale * code and of the zero points, and only the first has the
+// second rounding in it.  Carrying the second rounding's error through a second product took 8-10 %
+// (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.
 //
 // What bounds it: with many tiles the instructions of the tile loop (packed; about 600 a tile and warp) or the
 // memory (float16: 32 sequences, 338 MB, 60.3 us, 5.6 TB/s); with few, the chain of latencies: lengths, table, first tile
