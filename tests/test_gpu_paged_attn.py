@@ -156,6 +156,18 @@ def test_rising_scores():
         check(attend(q, k, v, table, lens_t(lens)), q, k, v, table, lens, f"rising {nbits}")
 
 
+@pytest.mark.parametrize("power", [-8, -4, 8, 12])
+@pytest.mark.parametrize("nbits", [2, 4, 16])
+def test_small_and_large_values(nbits, power):
+    """Values far from 1: weights times scales at both ends of float16."""
+    lens = [700, 31]
+    k, v, table, _ = make_pools(lens, 2, 64, nbits, 32, 32, seed=power + 20)
+    for t in ([v] if nbits == 16 else [v.scale, v.zero]):
+        t.mul_(2.0 ** power)
+    q = make_q(2, 8, 64, 3)
+    check(attend(q, k, v, table, lens_t(lens)), q, k, v, table, lens, f"2^{power}")
+
+
 def test_agrees_with_the_contiguous_kernel():
     """Pages in order are the contiguous cache: the two kernels round alike."""
     from oracle.workloads import make_random_kv

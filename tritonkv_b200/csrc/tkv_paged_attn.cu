@@ -34,7 +34,9 @@
 // larger figure is that of one sequence of 65536: codes run from 0, so the mean of many tokens is a
 // difference of two larger sums, of scale * code and of the zero points, and only the first has the
 // second rounding in it.  Carrying the second rounding's error through a second product took 8-10 %
-// (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.
+// (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.  Weights (at most 2^-4 where a reference is set) times
+// scales leave the normal range of f16 where values are small: 4-bit values of 1/16 are 4e-4 off, of
+// 1/64 6e-4, of 1/256 2.6e-3 (256 to 65536 tokens).
 //
 // What bounds it: with many tiles the instructions of the tile loop (packed; about 600 a tile and warp) or the
 // memory (float16: 32 sequences, 338 MB, 60.3 us, 5.6 TB/s); with few, the chain of latencies: lengths, table, first tile
