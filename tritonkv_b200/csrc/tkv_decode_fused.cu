@@ -40,7 +40,9 @@
 // Softmax.  Probabilities are taken relative to a reference exponent m_ref that is
 // only raised (to tile max + 4) when a tile exceeds it, so accumulators are rescaled
 // a handful of times per split instead of at almost every tile; the true running
-// maximum is tracked separately and the partial is converted to it in the epilogue.
+// maximum is tracked separately and the partial is converted to it in the epilogue.  A
+// probability at the reference is 2^top, as high as float16 allows beside the value scales
+// (FusedPolicy::kTopMax): below 2^-14 an f16 operand loses bits.
 #include "tkv_fused_policy.cuh"
 
 namespace tkv {

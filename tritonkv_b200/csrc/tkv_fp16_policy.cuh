@@ -37,6 +37,7 @@ struct Fp16Policy {
   };
   struct Accum {
     float m_ref0, m_ref1, m_true0, m_true1, l0, l1;
+    float p_ref0, p_ref1;  // m_ref - kTop
     float acc[NCH][4];
   };
 
@@ -117,8 +118,12 @@ struct Fp16Policy {
     }
   }
 
+  // The probability at the reference is 2^kTop, p = 2^(score - m_ref + kTop) <= 2^15: as an f16 operand it
+  // keeps its bits down to 2^-29 of that (with p at most 1, down to 2^-14: a token of weight 0.99 left
+  // the others, 1/100 in all, with one or two bits each).
+  static constexpr float kTop = 15.f;
   __device__ static __forceinline__ void reset(Accum& ac) {
-    ac.m_ref0 = ac.m_ref1 = ac.m_true0 = ac.m_true1 = -INFINITY;
+    ac.m_ref0 = ac.m_ref1 = ac.p_ref0 = ac.p_ref1 = ac.m_true0 = ac.m_true1 = -INFINITY;
     ac.l0 = ac.l1 = 0.f;
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch)
@@ -181,6 +186,8 @@ struct Fp16Policy {
         const float alpha1 = ex2(ac.m_ref1 - n1);
         ac.m_ref0 = n0;
         ac.m_ref1 = n1;
+        ac.p_ref0 = n0 - kTop;
+        ac.p_ref1 = n1 - kTop;
         ac.l0 *= alpha0;
         ac.l1 *= alpha1;
 #pragma unroll
@@ -191,10 +198,10 @@ struct Fp16Policy {
           ac.acc[ch][3] *= alpha1;
         }
       }
-      sc[0] = ex2(sc[0] - ac.m_ref0);
-      sc[1] = ex2(sc[1] - ac.m_ref1);
-      sc[2] = ex2(sc[2] - ac.m_ref0);
-      sc[3] = ex2(sc[3] - ac.m_ref1);
+      sc[0] = ex2(sc[0] - ac.p_ref0);
+      sc[1] = ex2(sc[1] - ac.p_ref1);
+      sc[2] = ex2(sc[2] - ac.p_ref0);
+      sc[3] = ex2(sc[3] - ac.p_ref1);
       ac.l0 += sc[0] + sc[2];
       ac.l1 += sc[1] + sc[3];
     }
@@ -217,8 +224,8 @@ struct Fp16Policy {
       ac.l0 += __shfl_xor_sync(kFullMask, ac.l0, off);
       ac.l1 += __shfl_xor_sync(kFullMask, ac.l1, off);
     }
-    const float f0 = (ac.m_true0 == -INFINITY) ? 0.f : ex2(ac.m_ref0 - ac.m_true0);
-    const float f1 = (ac.m_true1 == -INFINITY) ? 0.f : ex2(ac.m_ref1 - ac.m_true1);
+    const float f0 = (ac.m_true0 == -INFINITY) ? 0.f : ex2(ac.p_ref0 - ac.m_true0);
+    const float f1 = (ac.m_true1 == -INFINITY) ? 0.f : ex2(ac.p_ref1 - ac.m_true1);
     st = SoftmaxState{ac.m_true0, ac.m_true1, ac.l0 * f0, ac.l1 * f1};
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch) {

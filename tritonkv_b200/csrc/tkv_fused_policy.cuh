@@ -127,8 +127,10 @@ struct FusedPolicy {
     uint32_t kofs, vofs;  // where the K and the V tile sit inside a stage
   };
   struct Accum {
-    float m_ref0, m_ref1;    // exponent the probabilities refer to (same on the 8 lanes of a head)
+    float m_ref0, m_ref1;    // score that the probabilities refer to (same on the 8 lanes of a head)
     float m_true0, m_true1;  // this lane's running maxima (reduced over lanes in finalize)
+    float top, p_ref0, p_ref1;  // the probability at m_ref is 2^top; m_ref - top
+    uint32_t vcap;           // room_for(top)
     float acc[NCH][4];
     float zacc[4];  // rows 0..NG-1: sum_n p_n z_n[group]; row 8: sum_n p_n
   };
@@ -442,8 +444,22 @@ struct FusedPolicy {
     qq.qz1 = pack_half2(lo[0], lo[1]);
   }
 
+  // Where the probabilities stand.  A token's p = 2^(score - m_ref + top) and its products with the value
+  // scales are f16 operands, so what is far below the largest p of the warp's tokens leaves the normal range:
+  // with p at most 1, one token of weight 0.74 with values near 0 beside 4095 others with values of 1 (of 1/16)
+  // put the output 1.2e-2 (0.41) off, in the 2-norm.  `top` is as high as f16 allows: p <= 2^15, and the products
+  // with scales below 2 are below 2^16.  Where a tile has a scale x in [2^e, 2^(e+1)), e >= 1, `top` comes
+  // down to 15 - e for the rest of the segment.  In the same place: 5.5e-4 (5.6e-4).  The look at the scales
+  // costs 1.1 % with 4 bits and 1.2 % with 2 (64 sequences of 4096: 61.3 -> 61.9 us, 55.3 -> 56.0; paged 0.3 %).
+  static constexpr float kTopMax = 15.f;
+  // The bits of a half x >= 0 plus this stay below 2^15 where x < 2^(16 - top); for a pair of them.
+  __device__ static __forceinline__ uint32_t room_for(float top) { return (uint32_t)((int)top + 1) * 0x04000400u; }
+
   __device__ static __forceinline__ void reset(Accum& ac) {
     ac.m_ref0 = ac.m_ref1 = ac.m_true0 = ac.m_true1 = -INFINITY;
+    ac.top = kTopMax;
+    ac.vcap = room_for(kTopMax);
+    ac.p_ref0 = ac.p_ref1 = -INFINITY;
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch)
 #pragma unroll
@@ -669,7 +685,17 @@ struct FusedPolicy {
       }
       ac.m_true0 = fmaxf(ac.m_true0, mx0);
       ac.m_true1 = fmaxf(ac.m_true1, mx1);
-      if (__any_sync(kFullMask, (mx0 > ac.m_ref0) || (mx1 > ac.m_ref1))) {
+      // the largest of the value scales of token `lane` (and lane + 32), two halves
+      uint32_t vmax = 0;
+#pragma unroll
+      for (int i = 0; i < kTok / 32; ++i) {
+        const MetaRow<NG> r = lds_meta_row<NG>(ms + 2 * C::META_STRIDE + (i * 32 + lane) * (NG * 2));
+#pragma unroll
+        for (int k = 0; k < (NG + 1) / 2; ++k) vmax = __vmaxu2(vmax, r.w[k] & 0x7fff7fffu);
+      }
+      if (__any_sync(kFullMask, (mx0 > ac.m_ref0) || (mx1 > ac.m_ref1) || ((vmax + ac.vcap) & 0x80008000u) != 0)) {
+        const uint32_t x = __reduce_max_sync(kFullMask, max(vmax & 0xffffu, vmax >> 16));
+        const float top = fminf(ac.top, 30.f - (float)(x >> 10));  // (bits 10-14: e + 15)
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) {
           mx0 = fmaxf(mx0, __shfl_xor_sync(kFullMask, mx0, off));
@@ -677,10 +703,14 @@ struct FusedPolicy {
         }
         const float n0 = (mx0 > ac.m_ref0) ? mx0 + kLazyTau : ac.m_ref0;
         const float n1 = (mx1 > ac.m_ref1) ? mx1 + kLazyTau : ac.m_ref1;
-        const float alpha0 = ex2(ac.m_ref0 - n0);  // first tile: 2^(-inf) = 0; unchanged: 1
-        const float alpha1 = ex2(ac.m_ref1 - n1);
+        const float alpha0 = ex2(ac.m_ref0 - n0 + (top - ac.top));  // first tile: 2^(-inf) = 0; unchanged: 1
+        const float alpha1 = ex2(ac.m_ref1 - n1 + (top - ac.top));
         ac.m_ref0 = n0;
         ac.m_ref1 = n1;
+        ac.p_ref0 = n0 - top;
+        ac.p_ref1 = n1 - top;
+        ac.top = top;
+        ac.vcap = room_for(top);
 #pragma unroll
         for (int ch = 0; ch < NCH; ++ch) {
           ac.acc[ch][0] *= alpha0;
@@ -695,10 +725,10 @@ struct FusedPolicy {
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        sc[mt][0] = ex2(sc[mt][0] - ac.m_ref0);
-        sc[mt][1] = ex2(sc[mt][1] - ac.m_ref1);
-        sc[mt][2] = ex2(sc[mt][2] - ac.m_ref0);
-        sc[mt][3] = ex2(sc[mt][3] - ac.m_ref1);
+        sc[mt][0] = ex2(sc[mt][0] - ac.p_ref0);
+        sc[mt][1] = ex2(sc[mt][1] - ac.p_ref1);
+        sc[mt][2] = ex2(sc[mt][2] - ac.p_ref0);
+        sc[mt][3] = ex2(sc[mt][3] - ac.p_ref1);
       }
     }
 
@@ -775,8 +805,8 @@ struct FusedPolicy {
     // row 8 of the zero-point accumulator (lanes 0-3, registers 2 and 3) holds sum_n p_n
     const float l0 = __shfl_sync(kFullMask, ac.zacc[2], t);
     const float l1 = __shfl_sync(kFullMask, ac.zacc[3], t);
-    const float f0 = (ac.m_true0 == -INFINITY) ? 0.f : ex2(ac.m_ref0 - ac.m_true0);
-    const float f1 = (ac.m_true1 == -INFINITY) ? 0.f : ex2(ac.m_ref1 - ac.m_true1);
+    const float f0 = (ac.m_true0 == -INFINITY) ? 0.f : ex2(ac.p_ref0 - ac.m_true0);
+    const float f1 = (ac.m_true1 == -INFINITY) ? 0.f : ex2(ac.p_ref1 - ac.m_true1);
     st = SoftmaxState{ac.m_true0, ac.m_true1, l0 * f0, l1 * f1};
     const uint32_t vals_s = smem_u32(vals);
 #pragma unroll

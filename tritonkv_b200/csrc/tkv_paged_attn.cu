@@ -34,9 +34,9 @@
 // larger figure is that of one sequence of 65536: codes run from 0, so the mean of many tokens is a
 // difference of two larger sums, of scale * code and of the zero points, and only the first has the
 // second rounding in it.  Carrying the second rounding's error through a second product took 8-10 %
-// (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.  Weights (at most 2^-4 where a reference is set) times
-// scales leave the normal range of f16 where values are small: 4-bit values of 1/16 are 4e-4 off, of
-// 1/64 6e-4, of 1/256 2.6e-3 (256 to 65536 tokens).
+// (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.  Small weights and small values keep their bits (FusedPolicy::kTopMax,
+// Fp16Policy::kTop): 4-bit values of 1/256 are as far off as values of 1, and the tokens beside one of weight 0.95 as
+// those of a flat softmax.
 //
 // What bounds it: with many tiles the instructions of the tile loop (packed; about 600 a tile and warp) or the
 // memory (float16: 32 sequences, 338 MB, 60.3 us, 5.6 TB/s); with few, the chain of latencies: lengths, table, first tile
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     Policy::load_query(qs, p, qbuf + (seg_k & 1) * QB, qfrag_u32, lane);
     Policy::reset(acc);
     // (finite, so that a first tile without any token is exp2(-inf) = 0 like any other masked one)
-    acc.m_ref0 = acc.m_ref1 = kNoReference;
+    acc.m_ref0 = acc.m_ref1 = acc.p_ref0 = acc.p_ref1 = kNoReference;
     const int my_tiles = seg.ntiles > warp ? (seg.ntiles - warp + WARPS - 1) / WARPS : 0;
     int left = seg.hi - (seg.lo_tile + warp) * kTok;
     auto scores = [&](typename Policy::Scores& sc, int slot, int left_of) {
