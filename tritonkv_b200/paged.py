@@ -216,7 +216,8 @@ _pages_words: dict = {}
 
 
 def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
-    """The plan's scratch, zero at first and kept in the caller's dict ``ws`` for one number of pages."""
+    """The plan's scratch, zero at first and kept in the caller's dict ``ws``, one for every number of pages on
+    every device (its layout goes by the first, and its zero words are left zero for the next call)."""
     need = _pages_words.get((B, NP))
     if need is None:
         n = ctypes.c_int64(0)
@@ -224,14 +225,16 @@ def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
         need = n.value
         if len(_pages_words) < 4096:
             _pages_words[(B, NP)] = need
-    kept = None if ws is None else ws.get("pages")
-    if kept is None or kept[0] != NP or kept[1].numel() < need or kept[1].device != dev:
+    if ws is None:
+        return torch.zeros(need, dtype=torch.int32, device=dev)
+    scratch = ws.setdefault("pages", {})
+    kept = scratch.get((NP, dev))
+    if kept is None or kept.numel() < need:
         if kept is not None:  # a captured graph may still use it
             ws.setdefault("outgrown", []).append(kept)
-        kept = (NP, torch.zeros(need, dtype=torch.int32, device=dev))
-        if ws is not None:
-            ws["pages"] = kept
-    return kept[1]
+        # (2 words a row: room for twice the rows, so that rows added one by one leave few of them behind)
+        kept = scratch[NP, dev] = torch.zeros(need + 2 * B, dtype=torch.int32, device=dev)
+    return kept
 
 
 def _pool_args(ts, NP: int):
