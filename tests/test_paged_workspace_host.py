@@ -42,3 +42,44 @@ def test_page_scratch_of_a_growing_batch():
         assert t.numel() >= 4 + 2 * 4 + 300 + 2 * B
     assert len({id(t) for t in kept_tensors(ws)}) <= 12
     assert paged._pages_workspace(ws, 3, 100, CPU) is t
+
+
+@pytest.fixture(autouse=True)
+def sizes(monkeypatch):
+    """(the library's sizes need a device: stand-ins for the time of a test)"""
+    monkeypatch.setattr(_cabi, "_paged_bytes", {})
+
+
+def decode_key(B, dev=0):
+    key = (B, 8, 8, 16, 128, 4, 32, dev)
+    _cabi._paged_bytes[key] = (min(B, 512) * 8 + 444) * 8 * 130 * 4
+    return key
+
+
+def test_partials_of_a_growing_batch():
+    """A batch that climbs by ones: what is outgrown stays for the graphs that may use it, and is bounded."""
+    ws, tickets = {}, None
+    for B in range(1, 513):
+        key = decode_key(B)
+        kept = _cabi.paged_workspace(ws, key, CPU)
+        assert kept[0] == key and kept[4].numel() == kept[2] >= _cabi._paged_bytes[key] and kept[1] == kept[4].data_ptr()
+        tickets = kept[5] if tickets is None else tickets
+        assert kept[5] is tickets and kept[3] == tickets.data_ptr()
+    assert kept_bytes(ws) <= 4 * _cabi._paged_bytes[key] + tickets.nbytes
+    assert _cabi.paged_workspace(ws, key, CPU) is kept
+    assert _cabi.paged_workspace(ws, decode_key(5), CPU)[4] is kept[4]
+
+
+def test_partials_of_two_devices_in_turn():
+    """One dict used on two devices: each finds its own buffers again."""
+    ws, first = {}, {}
+    for i in range(40):
+        dev = i % 3
+        kept = _cabi.paged_workspace(ws, decode_key(16, dev), CPU if dev else META)
+        assert first.setdefault(dev, kept[4]) is kept[4] and kept[0][7] == dev
+    assert len({id(t) for t in kept_tensors(ws)}) == 6
+
+
+def test_without_a_dict_nothing_is_kept():
+    a, b = (_cabi.paged_workspace(None, decode_key(2), CPU) for _ in range(2))
+    assert a[4] is not b[4] and not a[5].any() and not b[5].any()

@@ -271,10 +271,16 @@ PAGED_TICKETS = 8192
 def paged_workspace(ws: dict | None, key: tuple, device) -> tuple:
     """(key, address of the partials, their bytes, address of the tickets, partials, tickets) of a paged decode
     call with ``key`` = (B, HQ, HKV, page, D, nbits, group_size, device index), kept in the caller's dict
-    ``ws`` (as ``paged``).  The tickets are zero at first, and left zero by every call."""
+    ``ws`` (as ``paged``; those of other devices aside).  The tickets are zero at first, and left zero by
+    every call."""
     kept = None if ws is None else ws.get("paged")
-    if kept is not None and kept[0] == key:
-        return kept
+    if kept is not None:
+        if kept[0] == key:
+            return kept
+        if kept[0][7] != key[7]:
+            aside = ws.setdefault("paged_aside", {})
+            aside[kept[0][7]] = kept
+            kept = aside.pop(key[7], None)
     need = _paged_bytes.get(key)
     if need is None:
         v = c_int64(0)
@@ -282,14 +288,16 @@ def paged_workspace(ws: dict | None, key: tuple, device) -> tuple:
         need = v.value
         if len(_paged_bytes) < 4096:
             _paged_bytes[key] = need
-    if kept is not None and kept[2] >= need and kept[0][7] == key[7]:
+    if kept is not None and kept[2] >= need:
         kept = (key, *kept[1:])
     else:
-        # what a captured graph may still use stays with the dict: the tickets, and smaller buffers
-        if kept is not None:
+        if kept is None:
+            tickets = torch.zeros(PAGED_TICKETS, dtype=torch.int32, device=device)
+        else:
+            # What a captured graph may still use stays with the dict: the tickets, and the smaller buffers.
+            # Doubled, all of those together are no larger than the one in use.
             ws.setdefault("outgrown", []).append(kept)
-        tickets = kept[5] if kept is not None and kept[0][7] == key[7] else torch.zeros(
-            PAGED_TICKETS, dtype=torch.int32, device=device)
+            tickets, need = kept[5], max(need, 2 * kept[2])
         partials = torch.empty(need, dtype=torch.uint8, device=device)
         kept = (key, partials.data_ptr(), need, tickets.data_ptr(), partials, tickets)
     if ws is not None:
