@@ -83,3 +83,21 @@ def test_partials_of_two_devices_in_turn():
 def test_without_a_dict_nothing_is_kept():
     a, b = (_cabi.paged_workspace(None, decode_key(2), CPU) for _ in range(2))
     assert a[4] is not b[4] and not a[5].any() and not b[5].any()
+
+
+def test_what_a_capture_makes_is_its_own(monkeypatch):
+    """Memory that is cleared by a node of a graph holds anything until the graph has run: neither another call nor
+    another graph may find it."""
+    ws = {}
+    monkeypatch.setattr(_cabi, "capturing", lambda: True)
+    seen = [paged._pages_workspace(ws, 4, 100, CPU), _cabi.paged_workspace(ws, decode_key(4), CPU)[5]]
+    assert not kept_tensors(ws)
+    monkeypatch.setattr(_cabi, "capturing", lambda: False)
+    mine = [paged._pages_workspace(ws, 4, 100, CPU), _cabi.paged_workspace(ws, decode_key(4), CPU)]
+    assert mine[0] is not seen[0] and mine[1][5] is not seen[1]
+    monkeypatch.setattr(_cabi, "capturing", lambda: True)  # what was there before the capture serves it
+    assert paged._pages_workspace(ws, 3, 100, CPU) is mine[0]
+    assert _cabi.paged_workspace(ws, decode_key(3), CPU)[4] is mine[1][4]
+    more = _cabi.paged_workspace(ws, decode_key(300), CPU)  # (cleared tickets are there; partials need no clearing)
+    assert more[4] is not mine[1][4] and more[5] is mine[1][5] and ws["paged"][4] is mine[1][4]
+    assert paged._pages_workspace(ws, 300, 100, CPU) is not mine[0] and len(kept_tensors(ws)) == 3

@@ -262,6 +262,11 @@ def decode_plan(kernel_id: int, nbits: int, D: int, gs: int, B: int, HQ: int, HK
     return r
 
 
+def capturing() -> bool:
+    """Whether the current stream is being captured into a graph."""
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 _paged_bytes: dict = {}
 
 
@@ -272,7 +277,8 @@ def paged_workspace(ws: dict | None, key: tuple, device) -> tuple:
     """(key, address of the partials, their bytes, address of the tickets, partials, tickets) of a paged decode
     call with ``key`` = (B, HQ, HKV, page, D, nbits, group_size, device index), kept in the caller's dict
     ``ws`` (as ``paged``; those of other devices aside).  The tickets are zero at first, and left zero by
-    every call."""
+    every call.  What is made during a capture is the graph's own: it is cleared when the graph runs, so it is
+    not kept for other calls."""
     kept = None if ws is None else ws.get("paged")
     if kept is not None:
         if kept[0] == key:
@@ -280,7 +286,7 @@ def paged_workspace(ws: dict | None, key: tuple, device) -> tuple:
         if kept[0][7] != key[7]:
             aside = ws.setdefault("paged_aside", {})
             aside[kept[0][7]] = kept
-            kept = aside.pop(key[7], None)
+            kept = aside.get(key[7])
     need = _paged_bytes.get(key)
     if need is None:
         v = c_int64(0)
@@ -291,8 +297,12 @@ def paged_workspace(ws: dict | None, key: tuple, device) -> tuple:
     if kept is not None and kept[2] >= need:
         kept = (key, *kept[1:])
     else:
+        if capturing():
+            ws = None
         if kept is None:
             tickets = torch.zeros(PAGED_TICKETS, dtype=torch.int32, device=device)
+        elif ws is None:
+            tickets = kept[5]
         else:
             # What a captured graph may still use stays with the dict: the tickets, and the smaller buffers.
             # Doubled, all of those together are no larger than the one in use.

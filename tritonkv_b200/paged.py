@@ -217,7 +217,8 @@ _pages_words: dict = {}
 
 def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
     """The plan's scratch, zero at first and kept in the caller's dict ``ws``, one for every number of pages on
-    every device (its layout goes by the first, and its zero words are left zero for the next call)."""
+    every device (its layout goes by the first, and its zero words are left zero for the next call).  What is made
+    during a capture is the graph's own: it is cleared when the graph runs, so it is not kept for other calls."""
     need = _pages_words.get((B, NP))
     if need is None:
         n = ctypes.c_int64(0)
@@ -225,11 +226,11 @@ def _pages_workspace(ws: dict | None, B: int, NP: int, dev) -> torch.Tensor:
         need = n.value
         if len(_pages_words) < 4096:
             _pages_words[(B, NP)] = need
-    if ws is None:
-        return torch.zeros(need, dtype=torch.int32, device=dev)
-    scratch = ws.setdefault("pages", {})
-    kept = scratch.get((NP, dev))
+    scratch = None if ws is None else ws.setdefault("pages", {})
+    kept = None if scratch is None else scratch.get((NP, dev))
     if kept is None or kept.numel() < need:
+        if scratch is None or _cabi.capturing():
+            return torch.zeros(need, dtype=torch.int32, device=dev)
         if kept is not None:  # a captured graph may still use it
             ws.setdefault("outgrown", []).append(kept)
         # (2 words a row: room for twice the rows, so that rows added one by one leave few of them behind)
