@@ -261,7 +261,7 @@ int tkv_paged_workspace(int B, int HQ, int HKV, int page_size, int D, int nbits,
  * tkv_quantize_pack.  nbits = 16: f16 pages, k_pool and v_pool are the pools and scale / zero are
  * not looked at.  k_values / v_values (null or of in_dtype, value_strides laid out like strides)
  * receive code*scale + zero.  Positions outside the table and entries that name no page drop
- * their tokens. */
+ * their tokens.  Two tokens of one call that go to one place leave an undefined row there. */
 typedef struct {
   const void *k, *v;
   void *k_pool, *k_scale, *k_zero, *v_pool, *v_scale, *v_zero, *k_values, *v_values;

@@ -128,7 +128,8 @@ def append_kv_paged(kq, vq, k_new: torch.Tensor, v_new: torch.Tensor, block_tabl
     ``k_values`` / ``v_values`` (optional, shape and dtype of ``k_new``, rows contiguous): receive
     ``code * scale + zero`` of every written token -- what the cache now stands for, so that a
     prompt's own attention can see the same keys and values as the tokens that follow it.
-    Two tokens that go to one place in the same call leave either of them there.
+    Two tokens that go to one place in the same call leave an undefined row there (in a packed pool even the
+    codes of one beside the scale of the other), and undefined ``k_values`` / ``v_values`` where those overlap.
     Returns ``(kq, vq)``."""
     kt, vt = pool_tensors(kq, "kq"), pool_tensors(vq, "vq")
     packed = len(kt) == 3
