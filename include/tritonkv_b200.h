@@ -287,7 +287,7 @@ int tkv_pages_workspace(int B, int num_pages, int64_t* words);
  * kept by the first row that continues this parent and copied for the others in all n_pools
  * tensors, pages added for reserve[b] (reserve0 if null) further tokens.  Fresh pages are the
  * lowest that no kept entry names, in order of (row, position); `missing` (1,) receives how many
- * the pool was short of.  The outputs must not overlap the inputs. */
+ * the pool was short of.  The outputs must not overlap the inputs or each other. */
 typedef struct {
   const int32_t *block_table, *seq_lens, *parents, *reserve;
   int32_t *new_table, *new_lens, *missing, *workspace;

@@ -108,6 +108,8 @@ def _place(values: torch.Tensor, new: torch.Tensor, what: str) -> tuple[int, tup
     strides = _row_strides(values)
     if strides is None:
         raise ValueError(f"{what} must have contiguous rows that start on 16-byte boundaries: it is written in place")
+    if 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, values.shape)):
+        raise ValueError(f"{what} must have a row for every token: it is written in place")
     return values.data_ptr(), strides
 
 
@@ -271,7 +273,8 @@ def _no_overlap(outs, ins) -> None:
         a0, a1 = _span(t)
         for b0, b1 in ins:
             if a0 < b1 and b0 < a1:
-                raise ValueError(f"out[{i}] must not share memory with a tensor it is made from")
+                raise ValueError(f"out[{i}] must not share memory with a tensor it is made from or another out")
+        ins.append((a0, a1))
 
 
 def fork_pages(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, reserve=0,
@@ -291,7 +294,7 @@ def fork_pages(pools, block_table: torch.Tensor, seq_lens: torch.Tensor, parents
     Entries behind a row's last page are -1.  Returns ``(table, lens, missing)``: int32
     ``(B_new, max_pages)``, ``(B_new,)``, and ``(1,)``, the number of pages that the pool was short of
     (their entries are -1, and what is appended there is dropped).  ``out``: these three
-    tensors, supplied by the caller; they must not share memory with the inputs.  The old
+    tensors, supplied by the caller; they must not share memory with the inputs or each other.  The old
     table is not changed.  A partly filled page that two different rows name (which this
     function never makes) stays shared."""
     ts, NP, page, where = _pool_list(pools)
