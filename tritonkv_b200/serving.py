@@ -21,8 +21,9 @@ class GraphedDecodeStep:
     ``q_host`` (B, HQ, D) and ``out_host`` (B, HQ, D) float32 are the pinned buffers the
     graph reads and writes; fill ``q_host`` (or pass ``q`` to :meth:`run`), call
     :meth:`run`, then :meth:`result` to wait for and get the step's output.  The cache
-    tensors must stay where they were at capture (append in place with
-    ``quantize.append_kv`` and grow ``seq_lens`` on the device to lengthen the history).
+    tensors and ``seq_lens`` must stay where they were at capture (append in place with
+    ``quantize.append_kv`` and grow ``seq_lens`` on the device to lengthen the history); the
+    step keeps them alive.
 
     ``zero_copy=True`` takes the device-to-host copy off the step: the last kernel stores the
     result straight into ``out_host`` (pinned host memory is addressable from the device).
@@ -51,6 +52,7 @@ class GraphedDecodeStep:
         self.q_dev = torch.zeros(B, HQ, D, dtype=q_dtype, device=dev)
         self.out_dev = torch.zeros(B, HQ, D, dtype=torch.float32, device=dev)
         self._ws: dict = {}
+        self._reads = (kq, vq, seq_lens, block_table)  # the graph has their addresses: they live as long as it
         self._dev = dev
         self._stream = torch.cuda.Stream(device=dev)  # capture stream only
 
