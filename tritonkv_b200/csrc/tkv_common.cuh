@@ -258,6 +258,22 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
   return false;
 }
 
+// After a wait that gave up: the copies that a warp has in flight end before the CTA's shared memory is
+// given back.  `slot` and `phase`: the stage to be consumed next and its barrier's phase; stages that
+// nothing was issued for take a short limit.
+template <int STAGES>
+__device__ __forceinline__ void drain_ring(uint32_t bars, int slot, int phase) {
+#pragma unroll 1
+  for (int s = 0; s < STAGES; ++s) {
+    mbar_wait_bounded(bars + 8 * slot, phase, 1 << 14);
+    if (++slot == STAGES) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+  asm volatile("cp.async.wait_all;\n" ::: "memory");
+}
+
 // 3-D tiled TMA load (c0 innermost, a multiple of 16 bytes).
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tensor_map, int c0, int c1, int c2,
                                             uint32_t bar) {

@@ -704,7 +704,10 @@ __global__ void __launch_bounds__(Policy::WARPS * 32, Policy::MIN_CTAS)
     }
     ++seg_k;
   }
-  if (timed_out && lane == 0) Policy::report_timeout();
+  if (timed_out) {
+    if (lane == 0) Policy::report_timeout();
+    drain_ring<STAGES>(bar_u32, c_slot, c_phase);
+  }
   if (n_shared == 0) return;
   if (threadIdx.x == 0) {
     s_shared[0].ticket = ticket[0];
