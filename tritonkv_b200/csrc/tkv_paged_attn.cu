@@ -12,7 +12,7 @@
 // tokens, else two runs of 16 (PIECES: 64 sequences at 4 bits 57 us against 53.8 in one).  The lanes of a warp look
 // up the pool rows of the warp's next 32 tiles, one each, across the segments to come; an issue takes
 // its row by a shuffle, so the table's latency is paid once per 32 tiles, behind tiles in flight, and the
-// tile loop holds no cursor (with one, 100 instructions a tile more, and spills).
+// tile loop holds no cursor (with one, 100 instructions a tile more).
 //
 // Lengths live on the device, so the plan is made there, by every CTA for itself: the prefix of the
 // sequences' work in shared memory, then either
@@ -33,8 +33,8 @@
 // on packed pages and 2.5e-4 on float16 ones (2-norm), where rounding it to f16 alone is 2.0e-4.  The
 // larger figure is that of one sequence of 65536: codes run from 0, so the mean of many tokens is a
 // difference of two larger sums, of scale * code and of the zero points, and only the first has the
-// second rounding in it.  Carrying the second rounding's error through a second product took 8-10 %
-// (64 sequences: 53.1 -> 58.5 us) for 2.4e-4.  Small weights and small values keep their bits (FusedPolicy::kTopMax,
+// second rounding in it.  Carrying the second rounding's error through a second product took 8-12 % with
+// many tiles (64 sequences at 2 bits: 51.4 -> 57.7 us) for 2.4e-4.  Small weights and small values keep their bits (FusedPolicy::kTopMax,
 // Fp16Policy::kTop): 4-bit values of 1/256 are as far off as values of 1, and the tokens beside one of weight 0.95 as
 // those of a flat softmax.
 //
@@ -58,7 +58,7 @@ struct PagedParams {
   int64_t table_stride;
   void* out;
   int out_dtype;
-  int num_pages, page, max_pages, HKVc;
+  int num_pages, page, HKVc;
   int whole;              // a CTA takes part of one unit only: how many a unit can have; 0: equal ranges of all tiles
   FastDiv dpage, dHch, dHKVc, dHQ, dgroup, dgrid;
   float *acc, *m, *l;     // (slots, 8, D), (slots, 8), (slots, 8)
@@ -955,11 +955,13 @@ struct PagedLaunch {
       const int64_t units_now = (int64_t)n * pp.HKVc;
       pp.whole = units_now * 2 <= w && tiles * Policy::WARPS < (1 << 23) ? (int)(w / units_now) : 0;
       // Who merges.  With at least a CTA per unit and few partials of each, the CTA that finishes a unit:
-      // one launch instead of two, 2.4 us of host time (17.0 -> 14.6 us per call), for the same time on the
-      // device (1 sequence of 500 tokens 7.9 / 7.9 us, 8 of 4096 20.1 / 21.0, 16 of 4096 26.6 / 27.1).  Else a
-      // kernel that spreads the partials over the device: one sequence of 65536 (222 partials a unit)
-      // 13.1 us against 23.2, and with more units than CTAs, where every CTA would draw two tickets,
-      // 53.1 against 53.8 (64 sequences at 2 bits).
+      // one launch instead of two, 2.3 us of host time (14.4 -> 12.1 us per call), and no more time on the
+      // device (1 sequence of 500 tokens 7.9 / 7.9 us, 8 of 4096 18.1 / 18.6, 16 of 4096 25.3 / 26.1).  Else a
+      // kernel that spreads the partials over the device: one sequence of 65536 with 2 KV heads (128 partials a
+      // unit) 12.8 us against 22.0, of 8000 8.7 against 11.5, and with more units than CTAs, where every CTA would
+      // draw two tickets, 51.5 against 52.3 (64 sequences at 2 bits).  The lengths are on the device: what counts here is
+      // the width of the table, so a short sequence under a wide table takes the second launch (500 tokens, 2048 pages of
+      // 16: 8.3 us against 8.1 on the device, 14.4 against 11.9 per call).
       const int64_t partials = 2 + (w / units_now < tiles / Policy::WARPS ? w / units_now : tiles / Policy::WARPS);
       pp.tickets = units_now <= w && partials <= kFewPartials && units_now <= kTickets ? c.tickets : nullptr;
       TKV_CUDA(launch_pdl(paged_split_kernel<Policy>, dim3(w), dim3(Policy::WARPS * 32), (size_t)smem_bytes(n), stream,
@@ -1005,7 +1007,9 @@ static int f16_run(const PagedCall& c, cudaStream_t stream) {
 
 // Two families per format, as for contiguous caches (tkv_decode_fused.cu): 4 warps with rings of 3
 // stages in a software pipeline, 3 CTAs per SM; and 8 warps with rings of 2, one tile at a time, 2 CTAs per
-// SM, where few long units are to be spread thin.
+// SM, where few long units are to be spread thin.  At head_dim 128 some of them spill (bytes stored): of the 4-warp ones
+// 2 bits in groups of 32 (16), of the 8-warp ones 2 bits in groups of 64 (68, 80) and 32 (52), 4 bits in groups of 128
+// (40) and 16 (16).
 template <int NB, int DD, int GG, int PIECES>
 using PagedPolicy = FusedPolicy<NB, DD, GG, true, 32, 4, 3, 3, true, false, PIECES>;
 template <int NB, int DD, int GG, int PIECES>
@@ -1116,7 +1120,6 @@ static int paged_fill(PagedCall& c, const tkv_paged_decode_args& a) {
   pp.out_dtype = a.out_dtype;
   pp.num_pages = a.num_pages;
   pp.page = a.page_size;
-  pp.max_pages = a.max_pages;
   pp.HKVc = a.HKV * p.hchunks;
   pp.dpage = make_fastdiv(a.page_size);
   pp.dHch = make_fastdiv(p.hchunks);

@@ -182,8 +182,9 @@ __global__ void __launch_bounds__(256)
     const int64_t mrow = gb * D + 2 * dp;
     *reinterpret_cast<__half2*>(scale + mrow) = __halves2half2(c0.sc16, c1.sc16);
     *reinterpret_cast<__half2*>(zero + mrow) = __halves2half2(c0.ze16, c1.ze16);
-    // codes by the reciprocal, those next to a tie redone with the IEEE division (see
-    // quantize_pack_kernel)
+    // Codes by the reciprocal: a * (1/s) is within 1e-5 of the IEEE quotient wherever the clamp does not decide
+    // the code (|q| <= 17), so it rounds alike unless it lies within 1e-4 of a half-integer; those are redone
+    // with the IEEE division.
     uint8_t* crow = codes + (lb * kChanTok) * D + 2 * dp;
     uint32_t near_tie = 0;  // bit t: token t holds a code next to a tie
 #pragma unroll
