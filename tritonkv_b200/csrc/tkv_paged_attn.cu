@@ -29,7 +29,7 @@
 // What is rounded: q to f16; the probabilities, formed in f32 against a running maximum, to f16 for
 // the second product (on packed pages their sum counts the rounded ones, and they are rounded once
 // more when the values' scale is multiplied in, since the codes are exact in f16 and the scales differ
-// by token); the output once.  All sums are f32.  Against float64 the output is 3.3e-4 to 5.0e-4 off
+// by token); the output once.  All sums are f32.  Against float64 the output is 3.1e-4 to 5.0e-4 off
 // on packed pages and 2.5e-4 on float16 ones (2-norm), where rounding it to f16 alone is 2.0e-4.  The
 // larger figure is that of one sequence of 65536: codes run from 0, so the mean of many tokens is a
 // difference of two larger sums, of scale * code and of the zero points, and only the first has the
