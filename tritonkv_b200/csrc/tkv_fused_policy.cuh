@@ -446,11 +446,11 @@ struct FusedPolicy {
 
   // Where the probabilities stand.  A token's p = 2^(score - m_ref + top) and its products with the value
   // scales are f16 operands, so what is far below the largest p of the warp's tokens leaves the normal range:
-  // with p at most 1, one token of weight 0.74 with values near 0 beside 4095 others with values of 1 (of 1/16)
-  // put the output 1.2e-2 (0.41) off, in the 2-norm.  `top` is as high as f16 allows: p <= 2^15, and the products
-  // with scales below 2 are below 2^16.  Where a tile has a scale x in [2^e, 2^(e+1)), e >= 1, `top` comes
-  // down to 15 - e for the rest of the segment.  In the same place: 5.5e-4 (5.6e-4).  The look at the scales
-  // costs 1.1 % with 4 bits and 1.2 % with 2 (64 sequences of 4096: 61.3 -> 61.9 us, 55.3 -> 56.0; paged 0.3 %).
+  // with p at most 1, two tokens of weight 0.95 with values near 0 in each of 40 sequences of 2048 put the output
+  // 1.1e-2 off where the other values are of 1, and 0.63 where they are of 1/16 (4 bits, 2-norm).  `top` is as high
+  // as f16 allows: p <= 2^15, and the products with scales below 2 are below 2^16.  Where a tile has a scale x in
+  // [2^e, 2^(e+1)), e >= 1, `top` comes down to 15 - e for the rest of the segment.  Both are then 4.5e-4, as a flat
+  // softmax is 5.2e-4.  The look at the scales costs 1.1 % with 4 bits and 1.2 % with 2 (64 sequences of 4096: 61.3 -> 61.9 us, 55.3 -> 56.0; paged 0.3 %).
   static constexpr float kTopMax = 15.f;
   // The bits of a half x >= 0 plus this stay below 2^15 where x < 2^(16 - top); for a pair of them.
   __device__ static __forceinline__ uint32_t room_for(float top) { return (uint32_t)((int)top + 1) * 0x04000400u; }

@@ -34,9 +34,9 @@
 // larger figure is that of one sequence of 65536: codes run from 0, so the mean of many tokens is a
 // difference of two larger sums, of scale * code and of the zero points, and only the first has the
 // second rounding in it.  Carrying the second rounding's error through a second product took 8-12 % with
-// many tiles (64 sequences at 2 bits: 51.4 -> 57.7 us) for 2.4e-4.  Small weights and small values keep their bits (FusedPolicy::kTopMax,
-// Fp16Policy::kTop): 4-bit values of 1/256 are as far off as values of 1, and the tokens beside one of weight 0.95 as
-// those of a flat softmax.
+// many tiles (64 sequences at 2 bits: 51.4 -> 57.7 us) for 2.4e-4.  Small weights and small values keep their
+// bits (FusedPolicy::kTopMax, Fp16Policy::kTop): 4-bit values of 1/256 are as far off as values of 1, and the
+// tokens beside one of weight 0.95 as those of a flat softmax.
 //
 // What bounds it: with many tiles the instructions of the tile loop (packed; about 600 a tile and warp) or the
 // memory (float16: 32 sequences, 338 MB, 60.3 us, 5.6 TB/s); with few, the chain of latencies: lengths, table, first tile
